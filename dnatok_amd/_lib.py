@@ -27,6 +27,8 @@ EXPORTS = [
     "dnatok_bpe_static_scratch_bytes", "dnatok_bpe_encode_static",
     "dnatok_bpe_table_set_chunk_geometry", "dnatok_bpe_table_set_placement", "dnatok_pack_ragged", "dnatok_pad_rows", "dnatok_pad_rows_as",
     "dnatok_normalize_bounds", "dnatok_normalize_rows",
+    "dnatok_gated_scan_states_bytes", "dnatok_gated_scan_work_bytes", "dnatok_gated_scan",
+    "dnatok_gated_scan_backward", "dnatok_gated_step", "dnatok_w4_matvec", "dnatok_logits_process",
 ]
 
 
@@ -134,6 +136,21 @@ def lib() -> ctypes.CDLL:
                                           POINTER(c_int64), POINTER(c_size_t)]
     L.dnatok_normalize_rows.argtypes = [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                         c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
+    for fn in (L.dnatok_gated_scan_states_bytes, L.dnatok_gated_scan_work_bytes):
+        fn.argtypes = [c_int64, c_int64, c_int32]
+        fn.restype = c_size_t
+    L.dnatok_gated_scan.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64, c_int64,
+                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    L.dnatok_gated_scan_backward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64,
+                                             c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_size_t,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    L.dnatok_gated_step.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p,
+                                    c_void_p, c_void_p]
+    L.dnatok_w4_matvec.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                   c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_void_p]
+    L.dnatok_logits_process.argtypes = [c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_void_p, c_int64, c_int32, c_void_p]
     for name in EXPORTS:
         getattr(L, name)          # AttributeError here means the library is stale
     _lib = L

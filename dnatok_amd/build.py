@@ -8,7 +8,8 @@ import sys
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libdnatok_hip.so")
-SOURCES = ["errors.hip", "char_encode.hip", "kmer_encode.hip", "bpe_encode.hip", "pack.hip", "host_ingest.hip", "normalize.hip"]
+SOURCES = ["errors.hip", "char_encode.hip", "kmer_encode.hip", "bpe_encode.hip", "pack.hip", "host_ingest.hip", "normalize.hip",
+           "gated_scan.hip", "w4_matvec.hip", "logits.hip"]
 # bench.py's memory-only kernels: a library of their own (include/dnatok_diag.h), not part of the product
 DIAG_LIB_PATH = os.path.join(_HERE, "libdnatok_diag.so")
 DIAG_SOURCES = ["diag.hip", "errors.hip"]

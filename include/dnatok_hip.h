@@ -414,6 +414,74 @@ int dnatok_normalize_rows(const dnatok_norm_step *steps_h, int32_t n_steps, cons
                           uint8_t *out_bytes, int64_t out_capacity, int64_t *out_offsets,
                           void *scratch, size_t scratch_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Model operators: what a model at base or token resolution runs on the rows that the encoders
+ * write.  The reference has none of them; its embedders hand the ids or embeddings to a model of
+ * the user's (DNATok.embed_from_strings, src/dna_tokenizer.py).  Element types are the codes
+ * below; strides count elements between rows, whose elements lie next to each other.
+ * ------------------------------------------------------------------------------------- */
+
+#define DNATOK_F32   0
+#define DNATOK_BF16  1
+#define DNATOK_F16   2
+
+/* Gated linear recurrence over packed rows, in every channel:
+ *   f_t = sigmoid(gate_t),  h_t = f_t h_(t-1) + (1 - f_t) x_t,  y_t = h_t
+ * x, gate and y are [total, dim] of `dtype`; y's rows lie back to back.  Row b is the tokens offsets[b] .. offsets[b+1]
+ * (offsets[0] = 0, offsets[n_rows] = total); without offsets the n_rows rows have one length.
+ * reverse = 1 runs every row from its last token to its first.  h0 float[n_rows, dim] (NULL: zeros)
+ * is the state in front of a row's first step, last float[n_rows, dim] (NULL allowed) receives the
+ * state behind its last one: h0 again for an empty row.  states receives what the backward pass
+ * needs and is also the call's work space; it must hold dnatok_gated_scan_states_bytes(). */
+size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim, int32_t dtype);
+int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
+                      const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
+                      const float *h0, void *y, float *last, void *states, size_t states_bytes, void *stream);
+
+/* Gradients of the same call: dy [total, dim] of `dtype` and dlast float[n_rows, dim] (either may be
+ * NULL: zeros) are those of y and last; dx and dgate [total, dim] of `dtype` and dh0
+ * float[n_rows, dim] (NULL allowed) are written.  states as the forward call left them; work must
+ * hold dnatok_gated_scan_work_bytes(). */
+size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype);
+int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
+                               const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
+                               const float *h0, const void *dy, int64_t dy_stride, const float *dlast,
+                               const void *states, size_t states_bytes, void *dx, void *dgate, float *dh0,
+                               void *work, size_t work_bytes, void *stream);
+
+/* One step of the recurrence for one token of each row: x, gate, y [n_rows, dim], state (NULL: zeros)
+ * and new_state float[n_rows, dim], which may be the same buffer. */
+int dnatok_gated_step(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
+                      const float *state, int64_t n_rows, int64_t dim, void *y, float *new_state, void *stream);
+
+/* y[m, n] = sum_k x[m, k] W[n, k] + bias[n] for few rows of x, with weights of 4 bits:
+ * W[n, k] = (q[n, k] - zero[n, k / group]) scale[n, k / group].  q is uint32[n, weight_stride], eight
+ * values to a word, the lowest bits first (what lies behind the k-th is not used); scales
+ * [n, ceil(k / group)] are of x's type (bfloat16 or float16); zeros uint8[n, ceil(k / group)] hold
+ * 0 .. 15 (NULL: 8 everywhere); group is a multiple of 32; bias float[n] or NULL; y is of x's type or
+ * float32.  Sums are held in 32 bits and rounded once. */
+int dnatok_w4_matvec(const void *x, int64_t x_stride, int32_t dtype, const uint32_t *weights, int64_t weight_stride,
+                     const void *scales, const uint8_t *zeros, int64_t m, int64_t n, int64_t k, int32_t group,
+                     const float *bias, void *y, int64_t y_stride, int32_t y_dtype, void *stream);
+
+/* Logits on their way to the choice of a token, [n_rows, vocab]:
+ *   z = logit;  seen: z = z > 0 ? z / repetition : z repetition;
+ *   z -= presence [c > 0] + frequency c;  z += bias;  -inf where the mask forbids the token.
+ * The history of row r is history[history_offsets[r] .. history_offsets[r+1]] (ids as the encoders pack
+ * them; ids outside the vocabulary count for nothing); `seen` means anywhere in it, c counts what lies
+ * behind its first prompt_lengths[r] ids (NULL: 0).  repetition (> 0), presence and frequency are
+ * float[n_rows], each NULL for none; bias is float, bias_stride 0 for one row shared by all.  allowed
+ * holds n_states bit masks, bit v & 31 of word v >> 5 for token v, allowed_stride words apart; state[r]
+ * is the row's mask (negative: nothing is forbidden, n_states or more: everything is); without
+ * state, n_states must be 1 (shared) or n_rows (one each).  out has the logits' type or float32 and may
+ * be the logits themselves.  A row whose mask forbids everything is -inf throughout. */
+int dnatok_logits_process(const void *logits, int64_t logits_stride, int32_t dtype, int64_t n_rows, int64_t vocab,
+                          const int32_t *history, const int64_t *history_offsets, const int32_t *prompt_lengths,
+                          const float *repetition, const float *presence, const float *frequency,
+                          const float *bias, int64_t bias_stride, const uint32_t *allowed, int64_t allowed_stride,
+                          int64_t n_states, const int32_t *state, void *out, int64_t out_stride, int32_t out_dtype,
+                          void *stream);
+
 #ifdef __cplusplus
 }
 #endif
