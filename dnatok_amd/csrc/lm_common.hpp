@@ -24,32 +24,35 @@ inline void with_type(int32_t dtype, Fn fn)
 // Row b of a packed batch is the tokens at(b) .. at(b + 1); without offsets all rows have one length.
 struct Rows {
     const int64_t *offsets;
-    int64_t n, total;
-    __device__ __forceinline__ int64_t at(int64_t b) const { return offsets ? offsets[b] : b * (total / n); }
+    int64_t n, total, length;
+    __device__ __forceinline__ int64_t at(int64_t b) const { return offsets ? offsets[b] : b * length; }
 };
 
-// sigmoid(g) and 1 - sigmoid(g), each to full relative precision: with e = exp(-|g|) they are 1 / (1 + e) and
-// e / (1 + e), and only the one that is at most a half (`small`) enters the state's update, so that a channel
-// that forgets once in a million tokens keeps its rate and a channel that forgets at once keeps x.
-struct Gate {
-    float small, big;
-    bool mostly_kept;                                   // g >= 0: the old state has the larger share
-
-    __device__ __forceinline__ explicit Gate(float g)
-    {
-        const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
-        big = __builtin_amdgcn_rcpf(1.0f + e);
-        small = e * big;
-        mostly_kept = g >= 0.0f;
-    }
-    // f h + (1 - f) x
-    __device__ __forceinline__ float next(float h, float x) const
-    {
-        return mostly_kept ? fmaf(small, x - h, h) : fmaf(small, h - x, x);
-    }
-    __device__ __forceinline__ float keep() const { return mostly_kept ? small : big; }              // 1 - f
-    __device__ __forceinline__ float forget(float v) const { return mostly_kept ? fmaf(-small, v, v) : small * v; }   // f v
-    __device__ __forceinline__ float slope() const { return small * big; }                           // f (1 - f)
-};
+// The gate of the recurrence as one signed number: of f = sigmoid(g) and 1 - f the one that is at most a half, e / (1 + e)
+// with e = exp(-|g|), with g's sign.  The state's update uses only that one, so that a channel that forgets
+// once in a million tokens keeps its rate (1 - f is not what is left of a rounded f), and a channel that forgets at once
+// keeps x.
+__device__ __forceinline__ float gate_share(float g)
+{
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
+    return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
+}
+__device__ __forceinline__ bool mostly_kept(float share) { return (int32_t)__float_as_uint(share) >= 0; }   // (f >= 1/2)
+__device__ __forceinline__ float next_state(float share, float h, float x)        // f h + (1 - f) x
+{
+    return fmaf(share, x - h, mostly_kept(share) ? h : x);
+}
+__device__ __forceinline__ float forget(float share, float v)                     // f v
+{
+    return fmaf(-share, v, mostly_kept(share) ? v : 0.0f);
+}
+__device__ __forceinline__ float taken(float share)                               // 1 - f
+{
+    return mostly_kept(share) ? share : 1.0f + share;
+}
+__device__ __forceinline__ float slope(float share)                               // f (1 - f)
+{
+    return fabsf(share) * (1.0f - fabsf(share));
+}
 
 }  // namespace dnatok
