@@ -136,14 +136,15 @@ def lib() -> ctypes.CDLL:
                                           POINTER(c_int64), POINTER(c_size_t)]
     L.dnatok_normalize_rows.argtypes = [c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                         c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
-    for fn in (L.dnatok_gated_scan_states_bytes, L.dnatok_gated_scan_work_bytes):
-        fn.argtypes = [c_int64, c_int64, c_int32]
-        fn.restype = c_size_t
+    L.dnatok_gated_scan_states_bytes.argtypes = [c_int64, c_int64]
+    L.dnatok_gated_scan_states_bytes.restype = c_size_t
+    L.dnatok_gated_scan_work_bytes.argtypes = [c_int64, c_int64, c_int32]
+    L.dnatok_gated_scan_work_bytes.restype = c_size_t
     L.dnatok_gated_scan.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64, c_int64,
-                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+                                    c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     L.dnatok_gated_scan_backward.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64,
-                                             c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_size_t,
-                                             c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+                                             c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                             c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
     L.dnatok_gated_step.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p,
                                     c_void_p, c_void_p]
     L.dnatok_w4_matvec.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,

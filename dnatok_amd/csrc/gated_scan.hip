@@ -14,25 +14,32 @@
 // over them gives the wave's (A, H); these are composed in LDS; the tile's own goes to memory for the tiles behind it;
 // the state in front of the tile comes from the tiles before it; a second pass over the registers gives the
 // states.  So every value and gate is read from memory once.  The backward pass does the same from the other side
-// with what flows towards earlier tokens, and runs the states of its tile again from the one that the forward pass
-// left at the end of the tile in front, which costs a 64-bit word per tile and channel instead of a state per token.
+// with what flows towards earlier tokens, and runs the states of a wave's tokens again from the one in front of them,
+// which the forward pass has left: 4 bytes for 16 tokens instead of a state for each.
 //
-// The tiles in front: a 64-bit word per tile and channel holds (A, H) once its tile knows them and the state h at its end
-// (marked) once it knows that.  A word says by itself whether it is there (a fill kernel has put a pattern that none has), so
-// nothing has to be ordered by a fence.  A tile looks at the 64 words in front of it until they hold a state with
-// nothing missing behind it, and runs that state through the tiles between one by one.  The result is
-// therefore the same to the last bit, wherever the state is found and whoever came first.  A wait ends after
-// a bounded number of looks; then the workgroup runs the row from its start itself, by the same steps.
+// The state in front of a tile: a 64-bit word per tile and channel holds the tile's (A, H); the sixteenth tile of a group
+// leaves the same for the group, and then the state at the group's end in its place (marked).  A word says by itself
+// whether it is there (a fill kernel has put a pattern that none has), so nothing has to be ordered by a fence.  A tile
+// takes the nearest group in front whose state is there, and runs that state through the groups and then the tiles
+// between, one after the other.  These are the same steps in the same order wherever the state is found and whoever came
+// first, so the result is the same to the last bit.  (With tiles alone, states one by one, a contig's tiles
+// followed each other every 0.2 us: 2.6 times the time that its bytes take.)
 #include "lm_common.hpp"
+
+#include <algorithm>
 
 namespace dnatok {
 
 constexpr uint64_t kNoWord = ~0ull;
-constexpr int kLooks = 1 << 14;
+constexpr int kLooks = 1 << 20;
+constexpr int kGroup = 16;                        // tiles of a group, and groups that a tile looks back
+constexpr int kCounterStride = 32;                // (a 128-byte line to a counter)
 
-__global__ __launch_bounds__(256) void fill_words_kernel(uint64_t *words, int64_t n)
+__global__ __launch_bounds__(256) void fill_words_kernel(uint64_t *words, int64_t n, int64_t n_counters)
 {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) words[i] = kNoWord;
+    const int64_t all = n + n_counters * kCounterStride / 2;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256)
+        words[i] = i < n ? kNoWord : 0;
 }
 
 template <typename T>
@@ -43,8 +50,9 @@ struct ScanArgs {
     int64_t dim, n_tiles;
     uint32_t n_slabs;
     const float *h0;
-    uint64_t *words;                              // [n_tiles, dim]: states at the tiles' ends
-    int looks;
+    float *states;                                // [waves' pieces, dim] or NULL: the state in front of each piece
+    uint64_t *tile_words, *group_words;           // [n_tiles, dim], [n_groups, dim]
+    uint32_t *counters;                           // [n_slabs], kCounterStride apart: tiles that have been taken
     T *y;
     float *last;
     // the backward pass
@@ -53,35 +61,28 @@ struct ScanArgs {
     const float *dlast;
     T *dx, *dgate;
     float *dh0;
-    uint64_t *back_words;                         // [n_tiles, dim]: what flows from a tile to the tile in front of it
 };
 
 // V channels of one token as they lie in memory.
 template <typename T, int V> struct Cell { T v[V]; };
-template <typename T, int V>
-__device__ __forceinline__ Cell<T, V> load_cell(const T *p)
+
+// The cells go on as they lie in memory: without this the compiler keeps their 32-bit forms, twice the registers.
+template <typename T, int V, int S>
+__device__ __forceinline__ void keep_raw(Cell<T, V> (&c)[S])
 {
-    Cell<T, V> c;
-    if constexpr (V * sizeof(T) == 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
-        __builtin_memcpy(&c, &w, 4);
-    } else {
-        c.v[0] = p[0];
-    }
-    return c;
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_cell(T *p, const float *v)
-{
-    Cell<T, V> c;
 #pragma unroll
-    for (int j = 0; j < V; ++j) c.v[j] = from_float<T>(v[j]);
-    if constexpr (V * sizeof(T) == 4) {
-        uint32_t w;
-        __builtin_memcpy(&w, &c, 4);
-        *reinterpret_cast<uint32_t *>(p) = w;
-    } else {
-        p[0] = c.v[0];
+    for (int i = 0; i < S; ++i) {
+        if constexpr (V * sizeof(T) == 4) {
+            uint32_t w;
+            __builtin_memcpy(&w, &c[i], 4);
+            asm volatile("" : "+v"(w));
+            __builtin_memcpy(&c[i], &w, 4);
+        } else {
+            uint16_t w;
+            __builtin_memcpy(&w, &c[i], 2);
+            asm volatile("" : "+v"(w));
+            __builtin_memcpy(&c[i], &w, 2);
+        }
     }
 }
 template <int V>
@@ -165,62 +166,49 @@ __device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, in
     ends = __ballot(lane <= S && e.end[i] >= 0);
 }
 
-// A piece of the axis: c -> a c + h in every channel, with b = 1 - a beside a, each multiplied up on its own: a rounded
-// product of factors next to 1 would lose what slow channels forget (always in the same direction where the gate is
-// constant).  Where a row begins inside (or ends, for what flows backwards) the piece is a reset: h comes out, and nothing
-// of what comes in, be it infinite.
+// A piece of the axis: c -> (1 - b) c + h in every channel.  (b and not 1 - b is multiplied up: a rounded product of
+// factors next to 1 would lose what slow channels forget, always in the same direction where the gate is constant.)
+// Where a row begins inside (or ends, for what flows backwards) the piece is a reset: h comes out, and nothing of what
+// comes in, be it infinite.
 constexpr float kReset = 2.0f;
 
-__device__ __forceinline__ float carry_through(float s, float h, float c)          // s: kReset, b, or -a where a < 1/2
-{
-    const float f = mostly_kept(s) ? fmaf(-s, c, c) + h : fmaf(-s, c, h);
-    return s == kReset ? h : f;
-}
+__device__ __forceinline__ float carry_through(float b, float h, float c) { return b == kReset ? h : fmaf(-b, c, c) + h; }
 
 template <int V>
 struct Piece {
-    float a[V], b[V], h[V];
+    float b[V], h[V];
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = h[v] = 0.0f;
+        for (int v = 0; v < V; ++v) b[v] = h[v] = 0.0f;
     }
-    __device__ __forceinline__ void factor(int v, float share)
-    {
-        b[v] = next_state(share, b[v], 1.0f);
-        a[v] = forget(share, a[v]);
-    }
+    __device__ __forceinline__ void factor(int v, float k) { b[v] = next_state(k, b[v], 1.0f); }
     __device__ __forceinline__ void close(bool edge)
     {
 #pragma unroll
         for (int v = 0; v < V; ++v) b[v] = edge ? kReset : b[v];
     }
-    __device__ __forceinline__ float small(int v) const { return a[v] < 0.5f && b[v] != kReset ? -a[v] : b[v]; }
     __device__ __forceinline__ void through(float (&c)[V]) const
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = carry_through(small(v), h[v], c[v]);
+        for (int v = 0; v < V; ++v) c[v] = carry_through(b[v], h[v], c[v]);
     }
     __device__ __forceinline__ void then(const Piece &p)
     {
         p.through(h);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            b[v] = b[v] == kReset || p.b[v] == kReset ? kReset : fmaf(p.b[v], a[v], b[v]);
-            a[v] *= p.a[v];
-        }
+        for (int v = 0; v < V; ++v) b[v] = b[v] == kReset || p.b[v] == kReset ? kReset : next_state(p.b[v], b[v], 1.0f);
     }
 };
 
-// A word of the tiles: low s of carry_through, high h.  (s is never the NaN of an absent word.)
+// A word of the tiles: low b, high h.  (b is never the NaN of an absent word.)
 template <int V>
 __device__ __forceinline__ void put_words(uint64_t *to, const Piece<V> &p)
 {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        float s = p.small(v);
-        if (!(s == s)) s = __builtin_nanf("");
-        __hip_atomic_store(to + v, (uint64_t)__float_as_uint(p.h[v]) << 32 | __float_as_uint(s), __ATOMIC_RELAXED,
+        const float b = p.b[v] == p.b[v] ? p.b[v] : __builtin_nanf("");
+        __hip_atomic_store(to + v, (uint64_t)__float_as_uint(p.h[v]) << 32 | __float_as_uint(b), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     }
 }
@@ -237,193 +225,311 @@ __device__ __forceinline__ uint64_t get_word(const uint64_t *p)
 {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float word_s(uint64_t w) { return __uint_as_float((uint32_t)w); }
+__device__ __forceinline__ float word_b(uint64_t w) { return __uint_as_float((uint32_t)w); }
 __device__ __forceinline__ float word_h(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
 __device__ __forceinline__ bool is_there(uint64_t w) { return (uint32_t)w != 0xFFFFFFFFu; }
 
-// One wave: what reaches a tile from the tiles next to it (step = -1: those in front, 1: those behind).  `words` is the
-// tile's own place.  False if the words did not come.
-template <int V>
-__device__ __forceinline__ bool wait_for_carry(const uint64_t *words, int64_t step_words, int64_t n_near, int64_t slab0,
-                                               int64_t c, int looks, int lane, float (&carry)[V])
+// One wave: what reaches the tile that is the `at`-th in order from the tiles in front of it.  own() waits for what the tile
+// itself does and returns it; where the tile is the last of its group it is needed for the group's word, which is left
+// here.  NaN should the words never come.
+template <int V, typename Own>
+__device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], const uint64_t *tile_words,
+                                           uint64_t *group_words, int64_t dim, uint32_t at, uint32_t slab0, uint32_t c,
+                                           Own own, int lane, float (&carry)[V])
 {
-    for (int look = 0; look < looks; ++look) {
-        // one channel's words say how far the nearest state is (behind the last tile of the axis none is looked for)
-        const uint64_t w = lane < n_near ? get_word(words + step_words * (lane + 1) + slab0) : kNoWord;
-        const uint64_t there = __ballot(is_there(w)), states = __ballot(word_s(w) == kReset);
-        const int d = states ? __builtin_ctzll(states) : 63;
-        if (!states || (~there & ((1ull << d) - 1))) {
-            __builtin_amdgcn_s_sleep(2);
-            continue;
+    const int pos = (int)(at % kGroup), n_groups = (int)(at / kGroup < kGroup ? at / kGroup : kGroup);
+    const uint64_t *tiles = tile_words + (int64_t)at * dim;
+    uint64_t *groups = group_words + (int64_t)(at / kGroup) * dim;
+    // what one channel's words say: lanes 0 .. look at the tiles of the group in front, lanes kGroup .. at the groups
+    const bool group = lane >= kGroup;
+    const int back = (lane & (kGroup - 1)) + 1;
+    const bool wanted = group ? lane < 2 * kGroup && back <= n_groups : back <= pos;
+    const uint64_t *const mine = (group ? groups : tiles) - back * dim + slab0;
+    int looks = kLooks, need, nearest;                                 // tiles that count; the nearest group with a state, or -1
+    const auto look = [&] {
+        const uint64_t w = wanted ? get_word(mine) : kNoWord;
+        const uint64_t there = __ballot(is_there(w)), resets = __ballot(word_b(w) == kReset);
+        const uint32_t t = (uint32_t)resets & ((1u << kGroup) - 1), g = (uint32_t)(resets >> kGroup);
+        need = t ? __builtin_ctz(t) + 1 : pos;
+        nearest = g ? __builtin_ctz(g) : -1;
+        if (g && (~(uint32_t)(there >> kGroup) & ((1u << nearest) - 1))) nearest = -1;
+        return (~(uint32_t)there & ((1u << need) - 1)) == 0;
+    };
+    load_floats<V>(carry, nullptr);
+    for (bool ok = false; !ok;) {
+        while (!look() && --looks > 0) __builtin_amdgcn_s_sleep(1);
+        ok = true;
+        for (int e0 = 0; e0 < need; e0 += 8) {
+            uint64_t q[8][V];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) q[k][v] = e0 + k < need ? get_word(tiles - (e0 + k + 1) * dim + c + v) : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    ok = ok && is_there(q[k][v]);
+                    if (e0 + k < kGroup) window[e0 + k][v][lane] = q[k][v];
+                }
         }
-        bool ok = true;
-        for (int far = d; far >= 0; far -= 4) {
+        ok = __all(ok) || looks <= 0;
+    }
+    const bool reset = need > 0 && word_b(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
+    if (pos == kGroup - 1 && !reset) {
+        const Piece<V> last = own();
+        if (last.b[0] != kReset) {                                     // (otherwise the tile has left the group's state)
+            Piece<V> sum;
+            sum.clear();
+#pragma unroll 3
+            for (int e = need - 1; e >= 0; --e) {
+                Piece<V> p;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    p.b[v] = word_b(window[e][v][lane]);
+                    p.h[v] = word_h(window[e][v][lane]);
+                }
+                sum.then(p);
+            }
+            sum.then(last);
+            put_words<V>(groups + c, sum);
+        }
+    }
+    for (bool ok = reset; !ok;) {
+        while (nearest < 0 && --looks > 0) {
+            __builtin_amdgcn_s_sleep(1);
+            look();
+        }
+        ok = true;
+        for (int far = nearest; far >= 0; far -= 4) {
             uint64_t q[4][V];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int v = 0; v < V; ++v) q[k][v] = far >= k ? get_word(words + step_words * (far - k + 1) + c + v) : 0;
+                for (int v = 0; v < V; ++v) q[k][v] = far >= k ? get_word(groups - (far - k + 1) * dim + c + v) : 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 if (far < k) continue;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float s = word_s(q[k][v]);
-                    ok = ok && is_there(q[k][v]) && (s == kReset || far - k < d);
-                    carry[v] = carry_through(s, word_h(q[k][v]), carry[v]);
+                    const float b = word_b(q[k][v]);
+                    ok = ok && is_there(q[k][v]) && (b == kReset || far - k < nearest);
+                    carry[v] = carry_through(b, word_h(q[k][v]), carry[v]);
                 }
             }
         }
-        if (__all(ok)) return true;
+        ok = __all(ok);
+        if (!ok) nearest = -1;
+        if (looks <= 0) break;
     }
-    return false;
+#pragma unroll 4
+    for (int e = need - 1; e >= 0; --e)
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = carry_through(word_b(window[e][v][lane]), word_h(window[e][v][lane]), carry[v]);
+    if (looks <= 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = __builtin_nanf("");
 }
 
 // The pieces of a tile's waves, in LDS (array by array: lanes read neighbouring words).
 template <int W, int V>
 struct Pieces {
-    float a[W][V][64], b[W][V][64], h[W][V][64];
+    float b[W][V][64], h[W][V][64];
     __device__ __forceinline__ void put(int wave, int lane, const Piece<V> &p)
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[wave][v][lane] = p.a[v], b[wave][v][lane] = p.b[v], h[wave][v][lane] = p.h[v];
+        for (int v = 0; v < V; ++v) b[wave][v][lane] = p.b[v], h[wave][v][lane] = p.h[v];
     }
     __device__ __forceinline__ Piece<V> get(int wave, int lane) const
     {
         Piece<V> p;
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.a[v] = a[wave][v][lane], p.b[v] = b[wave][v][lane], p.h[v] = h[wave][v][lane];
+        for (int v = 0; v < V; ++v) p.b[v] = b[wave][v][lane], p.h[v] = h[wave][v][lane];
+        return p;
+    }
+    // waves 0 .. n - 1 one after the other, n > 0
+    __device__ __forceinline__ Piece<V> front(int n, int lane) const
+    {
+        Piece<V> p = get(0, lane);
+#pragma unroll 3
+        for (int w = 1; w < n; ++w) p.then(get(w, lane));
+        return p;
+    }
+    // waves W - 1 .. first one after the other, first < W
+    __device__ __forceinline__ Piece<V> behind(int first, int lane) const
+    {
+        Piece<V> p = get(W - 1, lane);
+#pragma unroll 3
+        for (int w = W - 2; w >= first; --w) p.then(get(w, lane));
         return p;
     }
 };
 
 template <int S, int W, int V>
 struct ScanShared {
-    Pieces<W, V> parts;
+    Pieces<W, V> parts;                           // of what the tile hands on: states forwards, gradients backwards
+    uint64_t window[kGroup][V][64];
     float carry[V][64];
-    int inside;                                   // a row starts (backward: ends) in the tile
+    uint32_t tile;
+    int arrived;                                  // waves whose pieces are there
     Edges<S> edges[W];
+    // A wave's pieces are there.  True for the last of the waves.
+    __device__ __forceinline__ bool arrive(int lane)
+    {
+        int before = 0;
+        if (lane == 0) before = __hip_atomic_fetch_add(&arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
+        return __builtin_amdgcn_readfirstlane(before) == W - 1;
+    }
+    __device__ __forceinline__ void wait_for_all() const
+    {
+        while (__hip_atomic_load(&arrived, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) < W) __builtin_amdgcn_s_sleep(1);
+    }
 };
 
 // A wave's share of the axis: positions p0 .. p0 + n, its lanes V channels each.  Lanes behind the last channel take the
 // last ones once more and write the same values to the same places.
 template <int V, int S, int W, bool REV>
 struct Span {
-    int64_t p0;
+    int64_t p0, lowest;                           // lowest: the first in memory of the tokens
     uint32_t c, slab0;
     int n;
     __device__ __forceinline__ Span(const Rows &rows, int64_t dim, int64_t tile, uint32_t slab, int wave, int lane)
     {
         p0 = (tile * W + wave) * S;
         n = rows.total - p0 < S ? (rows.total > p0 ? (int)(rows.total - p0) : 0) : S;
+        lowest = n == 0 ? rows.total - 1 : REV ? rows.total - p0 - n : p0;
         slab0 = slab * 64 * V;
         const uint32_t first = slab0 + lane * V;
         c = first < dim ? first : (uint32_t)dim - V;
     }
-    // base + the token of position p0 + i; of the last one there is for positions behind it
-    template <typename T>
-    __device__ __forceinline__ T *at(T *base, int64_t stride, int64_t total, int i) const
+};
+
+// The tokens of a span in one array: a buffer resource and one 32-bit offset in the lanes, the token's offset from
+// the span's lowest in a scalar, so that a cell costs no address arithmetic in the lanes.
+template <typename T, int V, int S, bool REV>
+struct Strip {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int lane_bytes, token_bytes, n;
+    template <int W>
+    __device__ __forceinline__ Strip(const T *base, int64_t stride, const Span<V, S, W, REV> &span, int64_t dim)
     {
-        const int64_t from = n > 0 ? p0 : total - 1, step = i < n ? i : n > 0 ? n - 1 : 0;
-        return base + (REV ? total - 1 - from : from) * stride + (REV ? -step : step) * stride;
+        n = span.n > 0 ? span.n : 1;
+        lane_bytes = (int)(span.c * sizeof(T));
+        token_bytes = (int)(stride * sizeof(T));
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(base + span.lowest * stride), 0,
+                                                 (n - 1) * token_bytes + (int)(dim * sizeof(T)), 0x00020000);
+    }
+    __device__ __forceinline__ int offset(int i) const                 // (positions behind the last one: the last one)
+    {
+        const int k = i < n ? i : n - 1;
+        return (REV ? n - 1 - k : k) * token_bytes;
+    }
+    __device__ __forceinline__ Cell<T, V> load(int i) const
+    {
+        Cell<T, V> c;
+        if constexpr (V * sizeof(T) == 4) {
+            const uint32_t w = __builtin_amdgcn_raw_buffer_load_b32(rsrc, lane_bytes, offset(i), 0);
+            __builtin_memcpy(&c, &w, 4);
+        } else {
+            const uint16_t w = __builtin_amdgcn_raw_buffer_load_b16(rsrc, lane_bytes, offset(i), 0);
+            __builtin_memcpy(&c, &w, 2);
+        }
+        return c;
+    }
+    __device__ __forceinline__ void store(int i, const float (&v)[V]) const
+    {
+        Cell<T, V> c;
+#pragma unroll
+        for (int j = 0; j < V; ++j) c.v[j] = from_float<T>(v[j]);
+        if constexpr (V * sizeof(T) == 4) {
+            uint32_t w;
+            __builtin_memcpy(&w, &c, 4);
+            __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), 0);
+        } else {
+            uint16_t w;
+            __builtin_memcpy(&w, &c, 2);
+            __builtin_amdgcn_raw_buffer_store_b16(w, rsrc, lane_bytes, offset(i), 0);
+        }
     }
 };
 
 __device__ __forceinline__ int32_t one_row(int32_t row) { return __builtin_amdgcn_readfirstlane(row); }
 
-// The state in front of position p0, from the start of the row that p0 lies in: tile by tile, as the tiles' own
-// workgroups run it, so with the same bits.  One wave; `e` is written over.
-template <typename T, int V, int S, int W, bool REV>
-__device__ __forceinline__ void run_from_row_start(const ScanArgs<T> &a, const Axis<REV> &axis, int64_t p0, int64_t c, int lane,
-                                                Edges<S> &e, float (&state)[V])
+// The next tile of a slab, one to each workgroup in the order of their arrival: a tile waits for tiles that running
+// workgroups hold, the first of which waits for none, so every wait ends.
+template <int S, int W, int V>
+__device__ __forceinline__ uint32_t take_tile(ScanShared<S, W, V> &sh, uint32_t *counters, uint32_t slab, bool only_one)
 {
-    const int64_t j = axis.first_from(p0, lane);                       // (p0 is inside row j - 1)
-    for (int64_t q = axis.at(j > 0 ? j - 1 : 0) / (S * W) * (S * W); q < p0; q += S * W) {
-        Piece<V> tile;
-#pragma unroll 1
-        for (int w = 0; w < W; ++w) {
-            uint64_t starts, ends;
-            find_edges<S, REV>(axis, q + w * S, S, lane, e, starts, ends, [](int64_t) {});
-            Piece<V> p;
-            p.clear();
-#pragma unroll 1
-            for (int i = 0; i < S; ++i) {
-                if (starts >> i & 1) load_floats<V>(p.h, a.h0 ? a.h0 + axis.row(e.start[i]) * a.dim + c : nullptr);
-                const int64_t t = axis.token(q + w * S + i);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float share = gate_share(to_float(a.gate[t * a.gate_stride + c + v]));
-                    p.h[v] = next_state(share, p.h[v], to_float(a.x[t * a.x_stride + c + v]));
-                    p.factor(v, share);
-                }
-            }
-            p.close(starts != 0);
-            if (w == 0) tile = p;
-            else tile.then(p);
-        }
-        tile.through(state);
+    if (threadIdx.x == 0) {
+        sh.arrived = 0;
+        sh.tile = only_one ? 0 : atomicAdd(counters + slab * kCounterStride, 1u);
     }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(sh.tile);
 }
 
-// What flows to the position in front of p1 from the end of the row that it lies in, in the same way.
-template <typename T, int V, int S, int W, bool REV>
-__device__ __forceinline__ void run_from_row_end(const ScanArgs<T> &a, const Axis<REV> &axis, int64_t p1, int64_t c, int lane,
-                                              Edges<S> &e, float (&carry)[V])
+// The last wave of a workgroup looks for the carry while the others, W, compute; `nth`: the tile's place in the order of the
+// launch.  edge: position at which the carry comes in; nothing comes in where a row starts (ends) there.
+template <int S, int W, int V, bool REV, typename T, typename Own>
+__device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanArgs<T> &a, const Axis<REV> &axis,
+                                           uint32_t nth, uint32_t slab0, uint32_t c, int64_t edge, Own own, int lane)
 {
-    const int64_t total = a.rows.total, last = axis.at(axis.first_from(p1, lane)) - 1;   // (p1 is inside the row)
-    for (int64_t q = last / (S * W) * (S * W); q >= p1; q -= S * W) {
-        Piece<V> tile;
-#pragma unroll 1
-        for (int w = W - 1; w >= 0; --w) {
-            const int64_t p0 = q + w * S;
-            const int n = total - p0 < S ? (total > p0 ? (int)(total - p0) : 0) : S;
-            uint64_t starts, ends;
-            find_edges<S, REV>(axis, p0, n, lane, e, starts, ends, [](int64_t) {});
-            Piece<V> p;
-            p.clear();
-#pragma unroll 1
-            for (int i = 0; i < n; ++i)                                // (the factors in the order of the tile's own wave)
+    float carry[V];
+    load_floats<V>(carry, nullptr);
+    if (nth > 0 && axis.at(axis.first_from(edge, lane)) != edge) {
+        find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
+        if (nth % kGroup == kGroup - 1) {
+            const Piece<V> p = own();
+            if (p.b[0] != kReset) {
+                float end[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    p.factor(v, gate_share(to_float(a.gate[axis.token(p0 + i) * a.gate_stride + c + v])));
-#pragma unroll 1
-            for (int i = n - 1; i >= 0; --i) {
-                if (ends >> (i + 1) & 1)
-                    load_floats<V>(p.h, a.dlast ? a.dlast + axis.row(e.end[i + 1]) * a.dim + c : nullptr);
-                const int64_t t = axis.token(p0 + i);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float share = gate_share(to_float(a.gate[t * a.gate_stride + c + v]));
-                    p.h[v] = forget(share, p.h[v] + (a.dy ? to_float(a.dy[t * a.dy_stride + c + v]) : 0.0f));
-                }
+                for (int v = 0; v < V; ++v) end[v] = carry[v];
+                p.through(end);
+                put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, end);
             }
-            p.close(ends != 0);
-            if (w == W - 1) tile = p;
-            else tile.then(p);
         }
-        tile.through(carry);
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) sh.carry[v][lane] = carry[v];
+    __syncthreads();
+}
+
+// The word of a tile, and that of its group if the tile is the last of it and a row starts (ends) inside: then the state
+// at the end is known at once.
+template <int V, typename T>
+__device__ __forceinline__ void put_tile(const ScanArgs<T> &a, uint32_t nth, uint32_t c, const Piece<V> &p)
+{
+    put_words<V>(a.tile_words + (int64_t)nth * a.dim + c, p);
+    if (nth % kGroup == kGroup - 1 && p.b[0] == kReset)
+        put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, p.h);
 }
 
 template <typename T, int V, int S, int W, bool REV>
-__global__ __launch_bounds__(64 * W) void gated_scan_kernel(ScanArgs<T> a)
+__global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
 {
     __shared__ ScanShared<S, W, V> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x / a.n_slabs, slab = blockIdx.x - tile * a.n_slabs;
+    const uint32_t slab = blockIdx.x % a.n_slabs, tile = take_tile(sh, a.counters, slab, a.n_tiles == 1);
     const Axis<REV> axis{a.rows};
-    const int64_t total = a.rows.total;
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
     const uint32_t c = span.c;
+    if (wave == W) {
+        const auto own = [&] {
+            sh.wait_for_all();
+            return sh.parts.front(W, lane);
+        };
+        carry_wave<S, W, V>(sh, a, axis, tile, span.slab0, c, (int64_t)tile * (W * S), own, lane);
+        return;
+    }
     const int n = span.n;
-
+    typedef Strip<T, V, S, REV> strip;
+    const strip xs(a.x, a.x_stride, span, a.dim), gs(a.gate, a.gate_stride, span, a.dim);
     Cell<T, V> x[S], g[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        x[i] = load_cell<T, V>(span.at(a.x, a.x_stride, total, i) + c);
-        g[i] = load_cell<T, V>(span.at(a.gate, a.gate_stride, total, i) + c);
+        x[i] = xs.load(i);
+        g[i] = gs.load(i);
     }
-    if (threadIdx.x == 0) sh.inside = 0;
     Edges<S> &edges = sh.edges[wave];
     uint64_t starts, ends;
     find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
@@ -434,7 +540,7 @@ __global__ __launch_bounds__(64 * W) void gated_scan_kernel(ScanArgs<T> a)
     const bool plain = n == S && (starts | ends) == 0;                 // no row starts or ends here: no step has to look
     const auto initial = [&](int i) { return a.h0 ? a.h0 + axis.row(one_row(edges.start[i])) * a.dim + c : nullptr; };
 
-    float share[S][V];
+    float k[S][V];
     Piece<V> own;
     own.clear();
     const auto first_pass = [&](auto with_edges) {
@@ -444,65 +550,39 @@ __global__ __launch_bounds__(64 * W) void gated_scan_kernel(ScanArgs<T> a)
             if (with_edges && (starts >> i & 1)) load_floats<V>(own.h, initial(i));
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                share[i][v] = gate_share(to_float(g[i].v[v]));
-                own.h[v] = next_state(share[i][v], own.h[v], to_float(x[i].v[v]));
-                own.factor(v, share[i][v]);
+                k[i][v] = gate_taken(to_float(g[i].v[v]));
+                own.h[v] = next_state(k[i][v], own.h[v], to_float(x[i].v[v]));
+                own.factor(v, k[i][v]);
             }
         }
     };
     if (plain) first_pass(std::false_type{});
     else first_pass(std::true_type{});
+    keep_raw<T, V, S>(x);
     own.close(starts != 0);
     sh.parts.put(wave, lane, own);
-    __syncthreads();
-    if (starts && lane == 0) sh.inside = 1;
+    if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, tile, c, sh.parts.front(W, lane));
     Piece<V> front;                                                    // the tile's waves in front of this one
+    front.clear();
     if (wave > 0) {
-        front = sh.parts.get(0, lane);
-        for (int w = 1; w < wave; ++w) front.then(sh.parts.get(w, lane));
+        sh.wait_for_all();
+        front = sh.parts.front(wave, lane);
     }
-    uint64_t *const words = a.words + (int64_t)tile * a.dim;
-    if (wave == W - 1 && a.n_tiles > 1) {
-        Piece<V> all = front;
-        all.then(own);
-        put_words<V>(words + c, all);
-    }
-    const bool at_row = sh.edges[0].start[0] >= 0;                     // the tile's first position starts a row
     __syncthreads();
     float h[V];
-    load_floats<V>(h, nullptr);
-    if (!at_row) {
-        if (wave == 0) {
-            if (!wait_for_carry<V>(words, -a.dim, tile, span.slab0, c, a.looks, lane, h)) {
-                load_floats<V>(h, nullptr);
-                run_from_row_start<T, V, S, W, REV>(a, axis, span.p0, c, lane, edges, h);
-                find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [](int64_t) {});
-            }
 #pragma unroll
-            for (int v = 0; v < V; ++v) sh.carry[v][lane] = h[v];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = sh.carry[v][lane];
-        if (wave == W - 1 && !sh.inside) {
-            Piece<V> all = front;
-            all.then(own);
-            float state[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) state[v] = h[v];
-            all.through(state);
-            put_states<V>(words + c, state);
-        }
-    }
+    for (int v = 0; v < V; ++v) h[v] = sh.carry[v][lane];
     if (wave > 0) front.through(h);
+    if (a.states && n > 0) store_floats<V>(a.states + span.p0 / S * a.dim + c, h);
+    const strip ys(a.y, a.dim, span, a.dim);
     const auto second_pass = [&](auto with_edges) {
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             if (with_edges && i >= n) break;
             if (with_edges && (starts >> i & 1)) load_floats<V>(h, initial(i));
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = next_state(share[i][v], h[v], to_float(x[i].v[v]));
-            store_cell<T, V>(span.at(a.y, a.dim, total, i) + c, h);
+            for (int v = 0; v < V; ++v) h[v] = next_state(k[i][v], h[v], to_float(x[i].v[v]));
+            ys.store(i, h);
             if (with_edges && (ends >> (i + 1) & 1) && a.last)
                 store_floats<V>(a.last + axis.row(one_row(edges.end[i + 1])) * a.dim + c, h);
         }
@@ -513,30 +593,40 @@ __global__ __launch_bounds__(64 * W) void gated_scan_kernel(ScanArgs<T> a)
 
 //   dh_t = dy_t + f_(t+1) dh_(t+1),  dx_t = (1 - f_t) dh_t,  dgate_t = dh_t (h_(t-1) - x_t) f_t (1 - f_t)
 template <typename T, int V, int S, int W, bool REV>
-__global__ __launch_bounds__(64 * W) void gated_scan_backward_kernel(ScanArgs<T> a)
+__global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanArgs<T> a)
 {
     __shared__ ScanShared<S, W, V> sh;
-    __shared__ float back_h[W][V][64];            // (a wave's factors are those of its forward piece)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t nth = blockIdx.x / a.n_slabs, slab = blockIdx.x - nth * a.n_slabs, tile = (uint32_t)a.n_tiles - 1 - nth;
+    const uint32_t slab = blockIdx.x % a.n_slabs, nth = take_tile(sh, a.counters, slab, a.n_tiles == 1);
+    const uint32_t tile = (uint32_t)a.n_tiles - 1 - nth;
     const Axis<REV> axis{a.rows};
-    const int64_t total = a.rows.total;
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
     const uint32_t c = span.c;
+    if (wave == W) {
+        const auto own = [&] {
+            sh.wait_for_all();
+            return sh.parts.behind(0, lane);
+        };
+        carry_wave<S, W, V>(sh, a, axis, nth, span.slab0, c, ((int64_t)tile + 1) * (W * S), own, lane);
+        return;
+    }
     const int n = span.n;
-
+    typedef Strip<T, V, S, REV> strip;
+    const strip xs(a.x, a.x_stride, span, a.dim), gs(a.gate, a.gate_stride, span, a.dim);
     Cell<T, V> x[S], g[S], dy[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-        x[i] = load_cell<T, V>(span.at(a.x, a.x_stride, total, i) + c);
-        g[i] = load_cell<T, V>(span.at(a.gate, a.gate_stride, total, i) + c);
-        if (a.dy) dy[i] = load_cell<T, V>(span.at(a.dy, a.dy_stride, total, i) + c);
-        else dy[i] = Cell<T, V>{};
+        x[i] = xs.load(i);
+        g[i] = gs.load(i);
     }
-    float h[V];                                                        // the state in front of the tile
+    if (a.dy) {
+        const strip ds(a.dy, a.dy_stride, span, a.dim);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = tile > 0 ? word_h(a.words[((int64_t)tile - 1) * a.dim + c + v]) : 0.0f;
-    if (threadIdx.x == 0) sh.inside = 0;
+        for (int i = 0; i < S; ++i) dy[i] = ds.load(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) dy[i] = Cell<T, V>{};
+    }
     Edges<S> &edges = sh.edges[wave];
     uint64_t starts, ends;
     find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
@@ -550,97 +640,43 @@ __global__ __launch_bounds__(64 * W) void gated_scan_backward_kernel(ScanArgs<T>
         return a.dlast ? a.dlast + axis.row(one_row(edges.end[i + 1])) * a.dim + c : nullptr;
     };
 
-    float share[S][V];
-    Piece<V> own, back;
+    float k[S][V];
+    Piece<V> own;
     own.clear();
-    load_floats<V>(back.h, nullptr);
     const auto first_pass = [&](auto with_edges) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (with_edges && i >= n) break;
-            if (with_edges && (starts >> i & 1)) load_floats<V>(own.h, initial(i));
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                share[i][v] = gate_share(to_float(g[i].v[v]));
-                own.h[v] = next_state(share[i][v], own.h[v], to_float(x[i].v[v]));
-                own.factor(v, share[i][v]);
-            }
-        }
 #pragma unroll
         for (int i = S - 1; i >= 0; --i) {
             if (with_edges && i >= n) continue;
-            if (with_edges && (ends >> (i + 1) & 1)) load_floats<V>(back.h, final_grad(i));
+            if (with_edges && (ends >> (i + 1) & 1)) load_floats<V>(own.h, final_grad(i));
 #pragma unroll
-            for (int v = 0; v < V; ++v) back.h[v] = forget(share[i][v], back.h[v] + to_float(dy[i].v[v]));
+            for (int v = 0; v < V; ++v) {
+                k[i][v] = gate_taken(to_float(g[i].v[v]));
+                own.h[v] = forget(k[i][v], own.h[v] + to_float(dy[i].v[v]));
+                own.factor(v, k[i][v]);
+            }
         }
     };
     if (plain) first_pass(std::false_type{});
     else first_pass(std::true_type{});
-#pragma unroll
-    for (int v = 0; v < V; ++v) back.a[v] = own.a[v], back.b[v] = own.b[v], back_h[wave][v][lane] = back.h[v];
+    keep_raw<T, V, S>(x);
+    keep_raw<T, V, S>(dy);
+    own.close(ends != 0);
     sh.parts.put(wave, lane, own);
-    own.close(starts != 0);
-    back.close(ends != 0);
-    __shared__ uint8_t resets[W][2];              // the wave's piece is one forwards, backwards
-    if (lane == 0) resets[wave][0] = starts != 0, resets[wave][1] = ends != 0;
-    __syncthreads();
-    if (ends && lane == 0) sh.inside = 1;
-    if (wave > 0) {
-        Piece<V> front = sh.parts.get(0, lane);
-        front.close(resets[0][0]);
-        for (int w = 1; w < wave; ++w) {
-            Piece<V> p = sh.parts.get(w, lane);
-            p.close(resets[w][0]);
-            front.then(p);
-        }
-        front.through(h);
-    }
+    if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, nth, c, sh.parts.behind(0, lane));
     Piece<V> behind;                                                   // the tile's waves behind this one
-    const auto back_piece = [&](int w) {
-        Piece<V> p = sh.parts.get(w, lane);
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.h[v] = back_h[w][v][lane];
-        p.close(resets[w][1]);
-        return p;
-    };
+    behind.clear();
     if (wave < W - 1) {
-        behind = back_piece(W - 1);
-        for (int w = W - 2; w > wave; --w) behind.then(back_piece(w));
+        sh.wait_for_all();
+        behind = sh.parts.behind(wave + 1, lane);
     }
-    uint64_t *const words = a.back_words + (int64_t)tile * a.dim;
-    if (wave == 0 && a.n_tiles > 1) {
-        Piece<V> all = behind;
-        all.then(back);
-        put_words<V>(words + c, all);
-    }
-    const bool at_end = tile == (uint32_t)a.n_tiles - 1 || sh.edges[W - 1].end[S] >= 0;      // the tile's last position ends a row
+    float h[V];                                                        // the state in front of the wave's first token
+    load_floats<V>(h, n > 0 ? a.states + span.p0 / S * a.dim + c : nullptr);
     __syncthreads();
     float carry[V];
-    load_floats<V>(carry, nullptr);
-    if (!at_end) {
-        if (wave == W - 1) {
-            if (!wait_for_carry<V>(words, a.dim, a.n_tiles - 1 - tile, span.slab0, c, a.looks, lane, carry)) {
-                load_floats<V>(carry, nullptr);
-                run_from_row_end<T, V, S, W, REV>(a, axis, span.p0 + S, c, lane, edges, carry);
-                find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [](int64_t) {});
-            }
 #pragma unroll
-            for (int v = 0; v < V; ++v) sh.carry[v][lane] = carry[v];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = sh.carry[v][lane];
-        if (wave == 0 && !sh.inside) {
-            Piece<V> all = behind;
-            all.then(back);
-            float out[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) out[v] = carry[v];
-            all.through(out);
-            put_states<V>(words + c, out);
-        }
-    }
+    for (int v = 0; v < V; ++v) carry[v] = sh.carry[v][lane];
     if (wave < W - 1) behind.through(carry);
+    const strip dxs(a.dx, a.dim, span, a.dim), dgs(a.dgate, a.dim, span, a.dim);
     const auto second_pass = [&](auto with_edges) {
         float from_x[S][V];                                            // h_(t-1) - x_t
 #pragma unroll
@@ -651,7 +687,7 @@ __global__ __launch_bounds__(64 * W) void gated_scan_backward_kernel(ScanArgs<T>
             for (int v = 0; v < V; ++v) {
                 const float xv = to_float(x[i].v[v]);
                 from_x[i][v] = h[v] - xv;
-                h[v] = next_state(share[i][v], h[v], xv);
+                h[v] = fmaf(-k[i][v], from_x[i][v], h[v]);
             }
         }
 #pragma unroll
@@ -662,12 +698,12 @@ __global__ __launch_bounds__(64 * W) void gated_scan_backward_kernel(ScanArgs<T>
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float dh = to_float(dy[i].v[v]) + carry[v];
-                dx[v] = taken(share[i][v]) * dh;
-                dg[v] = dh * from_x[i][v] * slope(share[i][v]);
-                carry[v] = forget(share[i][v], dh);
+                dx[v] = k[i][v] * dh;
+                dg[v] = dh * from_x[i][v] * slope(k[i][v]);
+                carry[v] = forget(k[i][v], dh);
             }
-            store_cell<T, V>(span.at(a.dx, a.dim, total, i) + c, dx);
-            store_cell<T, V>(span.at(a.dgate, a.dim, total, i) + c, dg);
+            dxs.store(i, dx);
+            dgs.store(i, dg);
             if (with_edges && (starts >> i & 1) && a.dh0)
                 store_floats<V>(a.dh0 + axis.row(one_row(edges.start[i])) * a.dim + c, carry);
         }
@@ -690,8 +726,8 @@ __global__ __launch_bounds__(256) void gated_step_kernel(
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n_rows * dim) return;
     const int64_t b = i / dim, c = i - b * dim;
-    const float share = gate_share(to_float(gate[b * gate_stride + c]));
-    const float h = next_state(share, state ? state[i] : 0.0f, to_float(x[b * x_stride + c]));
+    const float k = gate_taken(to_float(gate[b * gate_stride + c]));
+    const float h = next_state(k, state ? state[i] : 0.0f, to_float(x[b * x_stride + c]));
     y[i] = from_float<T>(h);
     new_state[i] = h;
 }
@@ -706,12 +742,12 @@ namespace {
 
 constexpr int kSteps = 16;                        // tokens that a wave holds in registers
 
-// Waves to a tile: 16, or 4 where the batch would not give the chip's 256 CUs a tile each.  By sizes alone: the forward
+// Waves to a tile, beside the one that looks for the carry: 15, or 3 where the batch would not give the chip's 256 CUs a tile each.  By sizes alone: the forward
 // call's tiles are the backward call's.
 int waves_of(int64_t total, int64_t dim, int32_t dtype)
 {
     const int64_t channels = dtype == DNATOK_F32 ? 64 : 128;
-    return ((total + 255) / 256) * ((dim + channels - 1) / channels) >= 256 ? 16 : 4;
+    return ((total + 255) / 256) * ((dim + channels - 1) / channels) >= 256 ? 15 : 3;
 }
 
 int64_t tiles_of(int64_t total, int64_t dim, int32_t dtype)
@@ -720,11 +756,28 @@ int64_t tiles_of(int64_t total, int64_t dim, int32_t dtype)
     return (total + tile - 1) / tile;
 }
 
-size_t words_bytes(int64_t total, int64_t dim, int32_t dtype)
+// A launch's words, those of the tiles and of the groups, and its counters: each starting on a line of its own.
+struct Layout {
+    int64_t tiles, words, counters;               // tiles; 64-bit words of tiles and groups; counters
+    size_t bytes;                                 // 0 where one tile holds all
+    Layout(int64_t total, int64_t dim, int32_t dtype)
+    {
+        tiles = words = counters = 0;
+        bytes = 0;
+        if (total <= 0 || dim <= 0) return;
+        tiles = tiles_of(total, dim, dtype);
+        if (tiles == 1) return;
+        words = (tiles + (tiles + kGroup - 1) / kGroup) * dim;
+        words += -words & 15;
+        counters = (dim + 63) / 64;
+        bytes = (size_t)words * 8 + (size_t)counters * kCounterStride * 4;
+    }
+};
+
+// The states that the backward pass starts its pieces from.
+size_t states_bytes(int64_t total, int64_t dim)
 {
-    if (total <= 0 || dim <= 0) return 0;
-    const int64_t tiles = tiles_of(total, dim, dtype);
-    return tiles > 1 ? (size_t)tiles * (size_t)dim * 8 : 0;
+    return total > 0 && dim > 0 ? (size_t)((total + kSteps - 1) / kSteps) * (size_t)dim * 4 : 0;
 }
 
 int check_rows(const char *who, int32_t dtype, int64_t n_rows, int64_t total, int64_t dim, const int64_t *offsets)
@@ -736,10 +789,14 @@ int check_rows(const char *who, int32_t dtype, int64_t n_rows, int64_t total, in
     return DNATOK_OK;
 }
 
-int fill_words(void *words, size_t bytes, hipStream_t s)
+template <typename T>
+int fill_words(ScanArgs<T> &a, const Layout &l, void *at, hipStream_t s)
 {
-    const int64_t n = (int64_t)(bytes / 8), blocks = (n + 255) / 256;
-    fill_words_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>((uint64_t *)words, n);
+    const int64_t blocks = (l.words + 2047) / 2048;
+    a.tile_words = (uint64_t *)at;
+    a.group_words = a.tile_words + l.tiles * a.dim;
+    a.counters = (uint32_t *)(a.tile_words + l.words);
+    fill_words_kernel<<<(unsigned)std::min<int64_t>(blocks, 4096), 256, 0, s>>>(a.tile_words, l.words, l.counters);
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
 }
@@ -768,15 +825,17 @@ template <typename T, int V, int W>
 int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hipStream_t s)
 {
     a.n_slabs = (uint32_t)((a.dim + 64 * V - 1) / (64 * V));
+    const int64_t widest = std::max({a.x_stride, a.gate_stride, a.dy_stride, a.dim});
+    DNATOK_REQUIRE(widest * (int64_t)sizeof(T) * (kSteps + 1) < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: tokens too far apart", who);
     const int64_t blocks = a.n_slabs * a.n_tiles;
-    DNATOK_REQUIRE(blocks * 64 * W < (1ll << 32), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
+    DNATOK_REQUIRE(blocks * 64 * (W + 1) < (1ll << 32), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
     const unsigned grid = (unsigned)blocks;
     if (backward) {
-        if (reverse) gated_scan_backward_kernel<T, V, kSteps, W, true><<<grid, 64 * W, 0, s>>>(a);
-        else gated_scan_backward_kernel<T, V, kSteps, W, false><<<grid, 64 * W, 0, s>>>(a);
+        if (reverse) gated_scan_backward_kernel<T, V, kSteps, W, true><<<grid, 64 * (W + 1), 0, s>>>(a);
+        else gated_scan_backward_kernel<T, V, kSteps, W, false><<<grid, 64 * (W + 1), 0, s>>>(a);
     } else {
-        if (reverse) gated_scan_kernel<T, V, kSteps, W, true><<<grid, 64 * W, 0, s>>>(a);
-        else gated_scan_kernel<T, V, kSteps, W, false><<<grid, 64 * W, 0, s>>>(a);
+        if (reverse) gated_scan_kernel<T, V, kSteps, W, true><<<grid, 64 * (W + 1), 0, s>>>(a);
+        else gated_scan_kernel<T, V, kSteps, W, false><<<grid, 64 * (W + 1), 0, s>>>(a);
     }
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
@@ -785,28 +844,29 @@ int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hip
 template <typename T>
 int run_scan(const char *who, const ScanArgs<T> &a, int32_t dtype, bool backward, bool reverse, hipStream_t s)
 {
-    const bool wide = waves_of(a.rows.total, a.dim, dtype) == 16;
+    const bool wide = waves_of(a.rows.total, a.dim, dtype) == 15;
     if constexpr (sizeof(T) == 2)
         if (paired(a))
-            return wide ? launch_scan<T, 2, 16>(who, a, backward, reverse, s) : launch_scan<T, 2, 4>(who, a, backward, reverse, s);
-    return wide ? launch_scan<T, 1, 16>(who, a, backward, reverse, s) : launch_scan<T, 1, 4>(who, a, backward, reverse, s);
+            return wide ? launch_scan<T, 2, 15>(who, a, backward, reverse, s) : launch_scan<T, 2, 3>(who, a, backward, reverse, s);
+    return wide ? launch_scan<T, 1, 15>(who, a, backward, reverse, s) : launch_scan<T, 1, 3>(who, a, backward, reverse, s);
 }
 
 }  // namespace
 
-extern "C" size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim, int32_t dtype)
+extern "C" size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim)
 {
-    return words_bytes(total, dim, dtype);
+    return states_bytes(total, dim);
 }
 
 extern "C" size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype)
 {
-    return words_bytes(total, dim, dtype);
+    return Layout(total, dim, dtype).bytes;
 }
 
 extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
-                                 const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int flags,
-                                 const float *h0, void *y, float *last, void *states, size_t states_bytes, void *stream)
+                                 const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
+                                 const float *h0, void *y, float *last, float *states, void *work, size_t work_bytes,
+                                 void *stream)
 {
     static const char *who = "dnatok_gated_scan";
     if (int rc = check_rows(who, dtype, n_rows, total, dim, offsets)) return rc;
@@ -814,52 +874,49 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(h0, last, n_rows * dim, s);
     SCAN_REQUIRE(x && gate && y, "null buffer");
-    const size_t need = words_bytes(total, dim, dtype);
-    DNATOK_REQUIRE(need == 0 || (states && states_bytes >= need), DNATOK_E_SCRATCH, "%s: the states need %zu bytes", who, need);
-    if (need)
-        if (int rc = fill_words(states, need, s)) return rc;
+    const Layout l(total, dim, dtype);
+    DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
+                   who, l.bytes);
     int rc = DNATOK_OK;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         ScanArgs<T> a{};
         a.x = (const T *)x, a.x_stride = x_stride, a.gate = (const T *)gate, a.gate_stride = gate_stride;
         a.rows = Rows{offsets, n_rows, total, total / n_rows};
-        a.dim = dim, a.n_tiles = tiles_of(total, dim, dtype), a.h0 = h0, a.words = (uint64_t *)states;
-        a.looks = flags & DNATOK_SCAN_NO_WAIT ? 0 : kLooks;
+        a.dim = dim, a.n_tiles = l.tiles, a.h0 = h0, a.states = states;
         a.y = (T *)y, a.last = last;
-        rc = run_scan<T>(who, a, dtype, false, flags & DNATOK_SCAN_REVERSE, s);
+        if (l.bytes) rc = fill_words(a, l, work, s);
+        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, dtype, false, reverse != 0, s);
     });
     return rc;
 }
 
 extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride,
                                           int32_t dtype, const int64_t *offsets, int64_t n_rows, int64_t total,
-                                          int64_t dim, int flags, const float *h0, const void *dy, int64_t dy_stride,
-                                          const float *dlast, const void *states, size_t states_bytes, void *dx,
-                                          void *dgate, float *dh0, void *work, size_t work_bytes, void *stream)
+                                          int64_t dim, int reverse, const float *h0, const void *dy, int64_t dy_stride,
+                                          const float *dlast, const float *states, void *dx, void *dgate, float *dh0,
+                                          void *work, size_t work_bytes, void *stream)
 {
     static const char *who = "dnatok_gated_scan_backward";
     if (int rc = check_rows(who, dtype, n_rows, total, dim, offsets)) return rc;
     if (n_rows == 0) return DNATOK_OK;
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(dlast, dh0, n_rows * dim, s);
-    SCAN_REQUIRE(x && gate && dx && dgate, "null buffer");
-    const size_t need = words_bytes(total, dim, dtype);
-    DNATOK_REQUIRE(need == 0 || (states && states_bytes >= need), DNATOK_E_SCRATCH, "%s: the states need %zu bytes", who, need);
-    DNATOK_REQUIRE(need == 0 || (work && work_bytes >= need), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes", who, need);
-    if (need)
-        if (int rc = fill_words(work, need, s)) return rc;
+    SCAN_REQUIRE(x && gate && states && dx && dgate, "null buffer");
+    const Layout l(total, dim, dtype);
+    DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
+                   who, l.bytes);
     int rc = DNATOK_OK;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         ScanArgs<T> a{};
         a.x = (const T *)x, a.x_stride = x_stride, a.gate = (const T *)gate, a.gate_stride = gate_stride;
         a.rows = Rows{offsets, n_rows, total, total / n_rows};
-        a.dim = dim, a.n_tiles = tiles_of(total, dim, dtype), a.h0 = h0, a.words = (uint64_t *)states;
-        a.looks = flags & DNATOK_SCAN_NO_WAIT ? 0 : kLooks;
+        a.dim = dim, a.n_tiles = l.tiles, a.h0 = h0, a.states = const_cast<float *>(states);
         a.dy = (const T *)dy, a.dy_stride = dy ? dy_stride : 0, a.dlast = dlast;
-        a.dx = (T *)dx, a.dgate = (T *)dgate, a.dh0 = dh0, a.back_words = (uint64_t *)work;
-        rc = run_scan<T>(who, a, dtype, true, flags & DNATOK_SCAN_REVERSE, s);
+        a.dx = (T *)dx, a.dgate = (T *)dgate, a.dh0 = dh0;
+        if (l.bytes) rc = fill_words(a, l, work, s);
+        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, dtype, true, reverse != 0, s);
     });
     return rc;
 }

@@ -28,31 +28,15 @@ struct Rows {
     __device__ __forceinline__ int64_t at(int64_t b) const { return offsets ? offsets[b] : b * length; }
 };
 
-// The gate of the recurrence as one signed number: of f = sigmoid(g) and 1 - f the one that is at most a half, e / (1 + e)
-// with e = exp(-|g|), with g's sign.  The state's update uses only that one, so that a channel that forgets
-// once in a million tokens keeps its rate (1 - f is not what is left of a rounded f), and a channel that forgets at once
-// keeps x.
-__device__ __forceinline__ float gate_share(float g)
+// The gate of the recurrence: k = 1 - f = 1 / (1 + exp(g)), to full relative precision however small (1 - f would be what
+// is left of a rounded f).  The steps below use k alone, so that a channel that forgets once in a million tokens
+// keeps its rate; each rounds once, by at most half a unit of the larger of what goes in.
+__device__ __forceinline__ float gate_taken(float g)
 {
-    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(g));
-    return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(1.44269504f * g));
 }
-__device__ __forceinline__ bool mostly_kept(float share) { return (int32_t)__float_as_uint(share) >= 0; }   // (f >= 1/2)
-__device__ __forceinline__ float next_state(float share, float h, float x)        // f h + (1 - f) x
-{
-    return fmaf(share, x - h, mostly_kept(share) ? h : x);
-}
-__device__ __forceinline__ float forget(float share, float v)                     // f v
-{
-    return fmaf(-share, v, mostly_kept(share) ? v : 0.0f);
-}
-__device__ __forceinline__ float taken(float share)                               // 1 - f
-{
-    return mostly_kept(share) ? share : 1.0f + share;
-}
-__device__ __forceinline__ float slope(float share)                               // f (1 - f)
-{
-    return fabsf(share) * (1.0f - fabsf(share));
-}
+__device__ __forceinline__ float next_state(float k, float h, float x) { return fmaf(k, x - h, h); }     // f h + (1 - f) x
+__device__ __forceinline__ float forget(float k, float v) { return fmaf(-k, v, v); }                     // f v
+__device__ __forceinline__ float slope(float k) { return fmaf(-k, k, k); }                               // f (1 - f)
 
 }  // namespace dnatok

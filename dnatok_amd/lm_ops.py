@@ -57,7 +57,7 @@ def _require_floats(t: torch.Tensor, name: str, types=tuple(_DTYPES)) -> None:
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, offsets, n_rows, h0, reverse):
-        y, last, states = _scan_forward(x, gate, offsets, n_rows, h0, reverse)
+        y, last, states = _scan_forward(x, gate, offsets, n_rows, h0, reverse, True)
         ctx.save_for_backward(x, gate, offsets, h0, states)
         ctx.n_rows, ctx.reverse = n_rows, reverse
         ctx.set_materialize_grads(False)
@@ -83,21 +83,25 @@ class _GatedScan(torch.autograd.Function):
             _lib.check(L.dnatok_gated_scan_backward(
                 x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, _ptr(offsets), ctx.n_rows, total, dim,
                 int(ctx.reverse), _ptr(h0), _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dlast), states.data_ptr(),
-                states.numel(), dx.data_ptr(), dgate.data_ptr(), _ptr(dh0), _ptr(work), need, _stream(device)),
+                dx.data_ptr(), dgate.data_ptr(), _ptr(dh0), _ptr(work), need, _stream(device)),
                 "dnatok_gated_scan_backward")
         return dx, dgate, None, None, dh0, None
 
 
-def _scan_forward(x, gate, offsets, n_rows, h0, reverse):
+def _scan_forward(x, gate, offsets, n_rows, h0, reverse, keep_states):
     total, dim = x.shape
     device, code, L = x.device, _DTYPES[x.dtype], _lib.lib()
     y = torch.empty((total, dim), dtype=x.dtype, device=device)
     last = torch.empty((n_rows, dim), dtype=torch.float32, device=device)
-    states = torch.empty(L.dnatok_gated_scan_states_bytes(total, dim, code), dtype=torch.uint8, device=device)
+    states = None
+    if keep_states:
+        states = torch.empty(L.dnatok_gated_scan_states_bytes(total, dim) // 4, dtype=torch.float32, device=device)
+    need = L.dnatok_gated_scan_work_bytes(total, dim, code)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     with _on(device):
         _lib.check(L.dnatok_gated_scan(
             x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, _ptr(offsets), n_rows, total, dim,
-            int(reverse), _ptr(h0), y.data_ptr(), last.data_ptr(), states.data_ptr(), states.numel(), _stream(device)),
+            int(reverse), _ptr(h0), y.data_ptr(), last.data_ptr(), _ptr(states), _ptr(work), need, _stream(device)),
             "dnatok_gated_scan")
     return y, last, states
 
@@ -139,7 +143,7 @@ def _gated_scan(x, gate, offsets, n_rows, h0, reverse):
     _require(h0, "h0", (n_rows, dim), torch.float32, x.device)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedScan.apply(x, gate, offsets, n_rows, h0, reverse)
-    return _scan_forward(x, gate, offsets, n_rows, h0, reverse)[:2]
+    return _scan_forward(x, gate, offsets, n_rows, h0, reverse, False)[:2]
 
 
 def gated_step(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor] = None, *,

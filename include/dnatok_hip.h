@@ -429,30 +429,27 @@ int dnatok_normalize_rows(const dnatok_norm_step *steps_h, int32_t n_steps, cons
  *   f_t = sigmoid(gate_t),  h_t = f_t h_(t-1) + (1 - f_t) x_t,  y_t = h_t
  * x, gate and y are [total, dim] of `dtype`; y's rows lie back to back.  Row b is the tokens offsets[b] .. offsets[b+1]
  * (offsets[0] = 0, offsets[n_rows] = total); without offsets the n_rows rows have one length.
- * DNATOK_SCAN_REVERSE runs every row from its last token to its first.  h0 float[n_rows, dim] (NULL: zeros)
+ * reverse = 1 runs every row from its last token to its first.  h0 float[n_rows, dim] (NULL: zeros)
  * is the state in front of a row's first step, last float[n_rows, dim] (NULL allowed) receives the
- * state behind its last one: h0 again for an empty row.  states receives what the backward pass
- * needs and is also the call's work space; it must hold dnatok_gated_scan_states_bytes().
- * DNATOK_SCAN_NO_WAIT (for tests): parts of a row that other workgroups hold are computed again
- * instead of waited for; the results are the same. */
-#define DNATOK_SCAN_REVERSE  1
-#define DNATOK_SCAN_NO_WAIT  2
-
-size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim, int32_t dtype);
+ * state behind its last one: h0 again for an empty row.  states (NULL allowed) receives what the
+ * backward pass needs, dnatok_gated_scan_states_bytes(); work is the call's own space,
+ * dnatok_gated_scan_work_bytes(), at least 8-byte aligned. */
+size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim);
+size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype);
 int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
-                      const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int flags,
-                      const float *h0, void *y, float *last, void *states, size_t states_bytes, void *stream);
+                      const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
+                      const float *h0, void *y, float *last, float *states, void *work, size_t work_bytes,
+                      void *stream);
 
 /* Gradients of the same call: dy [total, dim] of `dtype` and dlast float[n_rows, dim] (either may be
  * NULL: zeros) are those of y and last; dx and dgate [total, dim] of `dtype` and dh0
- * float[n_rows, dim] (NULL allowed) are written.  states as the forward call left them; work must
- * hold dnatok_gated_scan_work_bytes(). */
-size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype);
+ * float[n_rows, dim] (NULL allowed) are written.  states as the forward call left them; work as
+ * there. */
 int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
-                               const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int flags,
+                               const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
                                const float *h0, const void *dy, int64_t dy_stride, const float *dlast,
-                               const void *states, size_t states_bytes, void *dx, void *dgate, float *dh0,
-                               void *work, size_t work_bytes, void *stream);
+                               const float *states, void *dx, void *dgate, float *dh0, void *work, size_t work_bytes,
+                               void *stream);
 
 /* One step of the recurrence for one token of each row: x, gate, y [n_rows, dim], state (NULL: zeros)
  * and new_state float[n_rows, dim], which may be the same buffer. */

@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 import torch
 
-from dnatok_amd import _lib, lm_ops
+from dnatok_amd import lm_ops
 from tests.support import lm_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -174,37 +174,6 @@ def test_scan_is_the_same_every_time():
             if first is None:
                 first = [t.detach().clone() for t in out]
             assert all(torch.equal(a, b) for a, b in zip(first, out))
-
-
-def _scan_by_hand(x, gate, off_d, h0, dy, dlast, flags):
-    """Forward and backward through the C ABI."""
-    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
-    (total, dim), rows, code = x.shape, off_d.numel() - 1, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[x.dtype]
-    y, dx, dgate = (torch.empty((total, dim), dtype=x.dtype, device=DEV) for _ in range(3))
-    last, dh0 = torch.empty_like(h0), torch.empty_like(h0)
-    states, work = (torch.empty(max(1, n), dtype=torch.uint8, device=DEV) for n in (
-        L.dnatok_gated_scan_states_bytes(total, dim, code), L.dnatok_gated_scan_work_bytes(total, dim, code)))
-    _lib.check(L.dnatok_gated_scan(x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, off_d.data_ptr(), rows,
-                                   total, dim, flags, h0.data_ptr(), y.data_ptr(), last.data_ptr(), states.data_ptr(),
-                                   states.numel(), stream), "dnatok_gated_scan")
-    _lib.check(L.dnatok_gated_scan_backward(
-        x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, off_d.data_ptr(), rows, total, dim, flags,
-        h0.data_ptr(), dy.data_ptr(), dy.stride(0), dlast.data_ptr(), states.data_ptr(), states.numel(), dx.data_ptr(),
-        dgate.data_ptr(), dh0.data_ptr(), work.data_ptr(), work.numel(), stream), "dnatok_gated_scan_backward")
-    return y, last, dx, dgate, dh0
-
-
-@pytest.mark.parametrize("dim,dtype", [(130, torch.bfloat16), (33, torch.float32), (600, torch.float16)])
-@pytest.mark.parametrize("reverse", [0, 1])
-def test_scan_without_waiting_is_the_same(dim, dtype, reverse):
-    """Workgroups that compute what others have not told them yet (DNATOK_SCAN_NO_WAIT) get the same bits."""
-    for lengths in ([3000], [700, 0, 1, 1500, 260, 256], [40000, 9]):
-        x, gate, off_d, off, h0, dy, dlast = scan_inputs(lengths, dim, dtype, 17)
-        print(f"gated_scan without waiting {lengths} dim={dim} {dtype} reverse={reverse}", flush=True)
-        want = _scan_by_hand(x, gate, off_d, h0, dy, dlast, reverse)
-        got = _scan_by_hand(x, gate, off_d, h0, dy, dlast, reverse | 2)
-        for name, a, b in zip(("y", "last", "dx", "dgate", "dh0"), want, got):
-            assert torch.equal(a, b), name
 
 
 def test_scan_of_dense_rows_is_that_of_packed_ones():

@@ -57,12 +57,13 @@ def test_argument_errors_without_a_gpu():
     buf = ctypes.create_string_buffer(64)
     p = ctypes.addressof(buf)
     scan = lambda dtype=0, rows=1, total=4, dim=4, x=p, off=p: L.dnatok_gated_scan(
-        x, 4, p, 4, dtype, off, rows, total, dim, 0, None, p, None, None, 0, None)
+        x, 4, p, 4, dtype, off, rows, total, dim, 0, None, p, None, None, None, 0, None)
     for kw, text in (({"dtype": 3}, b"type"), ({"dim": 0}, b"size"), ({"rows": -1}, b"size"), ({"rows": 0}, b"size"),
                      ({"x": None}, b"null"), ({"rows": 3, "off": None}, b"one length")):
         assert scan(**kw) == -1 and text in L.dnatok_last_error(), kw
-    assert L.dnatok_gated_scan_backward(None, 4, p, 4, 0, p, 1, 4, 4, 0, None, p, 4, None, p, 64, p, p, None, None, 0, None) == -1
-    assert L.dnatok_gated_scan_backward(p, 4, p, 4, 0, p, 1, 1 << 20, 4, 0, None, p, 4, None, p, 8, p, p, None, None, 0, None) == -4
+    assert L.dnatok_gated_scan_backward(None, 4, p, 4, 0, p, 1, 4, 4, 0, None, p, 4, None, p, p, p, None, None, 0, None) == -1
+    assert L.dnatok_gated_scan_backward(p, 4, p, 4, 0, p, 1, 1 << 20, 4, 0, None, p, 4, None, p, p, p, None, p, 64, None) == -4
+    assert scan(total=1 << 20) == -4 and b"bytes" in L.dnatok_last_error()
     assert L.dnatok_gated_step(p, 4, p, 4, 0, None, 1, 4, None, p, None) == -1 and b"null" in L.dnatok_last_error()
     w4 = lambda dtype=1, stride=8, group=32, y=1, x=p, k=64: L.dnatok_w4_matvec(
         x, 64, dtype, p, stride, p, None, 1, 4, k, group, None, p, 4, y, None)
