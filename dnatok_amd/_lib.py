@@ -138,7 +138,7 @@ def lib() -> ctypes.CDLL:
                                         c_void_p, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
     L.dnatok_gated_scan_states_bytes.argtypes = [c_int64, c_int64]
     L.dnatok_gated_scan_states_bytes.restype = c_size_t
-    L.dnatok_gated_scan_work_bytes.argtypes = [c_int64, c_int64, c_int32]
+    L.dnatok_gated_scan_work_bytes.argtypes = [c_int64, c_int64]
     L.dnatok_gated_scan_work_bytes.restype = c_size_t
     L.dnatok_gated_scan.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int64, c_int64,
                                     c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]

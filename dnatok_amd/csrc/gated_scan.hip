@@ -455,6 +455,13 @@ struct Strip {
 
 __device__ __forceinline__ int32_t one_row(int32_t row) { return __builtin_amdgcn_readfirstlane(row); }
 
+// The channels of a workgroup.  Workgroups go to the eight XCDs in turn, each with an L2 of its own; eight neighbours take
+// the same channels of eight tiles, so that a tile's slabs, which share the lines that they meet in, meet in one L2.
+__device__ __forceinline__ uint32_t slab_of(uint32_t n_slabs, bool only_one)
+{
+    return (only_one ? blockIdx.x : blockIdx.x >> 3) % n_slabs;
+}
+
 // The next tile of a slab, one to each workgroup in the order of their arrival: a tile waits for tiles that running
 // workgroups hold, the first of which waits for none, so every wait ends.
 template <int S, int W, int V>
@@ -509,7 +516,8 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
 {
     __shared__ ScanShared<S, W, V> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t slab = blockIdx.x % a.n_slabs, tile = take_tile(sh, a.counters, slab, a.n_tiles == 1);
+    const uint32_t slab = slab_of(a.n_slabs, a.n_tiles == 1), tile = take_tile(sh, a.counters, slab, a.n_tiles == 1);
+    if (tile >= a.n_tiles) return;
     const Axis<REV> axis{a.rows};
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
     const uint32_t c = span.c;
@@ -597,7 +605,8 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
 {
     __shared__ ScanShared<S, W, V> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t slab = blockIdx.x % a.n_slabs, nth = take_tile(sh, a.counters, slab, a.n_tiles == 1);
+    const uint32_t slab = slab_of(a.n_slabs, a.n_tiles == 1), nth = take_tile(sh, a.counters, slab, a.n_tiles == 1);
+    if (nth >= a.n_tiles) return;
     const uint32_t tile = (uint32_t)a.n_tiles - 1 - nth;
     const Axis<REV> axis{a.rows};
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
@@ -740,32 +749,20 @@ using namespace dnatok;
 
 namespace {
 
-constexpr int kSteps = 16;                        // tokens that a wave holds in registers
-
-// Waves to a tile, beside the one that looks for the carry: 15, or 3 where the batch would not give the chip's 256 CUs a tile each.  By sizes alone: the forward
-// call's tiles are the backward call's.
-int waves_of(int64_t total, int64_t dim, int32_t dtype)
-{
-    const int64_t channels = dtype == DNATOK_F32 ? 64 : 128;
-    return ((total + 255) / 256) * ((dim + channels - 1) / channels) >= 256 ? 15 : 3;
-}
-
-int64_t tiles_of(int64_t total, int64_t dim, int32_t dtype)
-{
-    const int64_t tile = (int64_t)kSteps * waves_of(total, dim, dtype);
-    return (total + tile - 1) / tile;
-}
+constexpr int kSteps = 24;                        // tokens that a wave holds in registers
+// Waves to a tile beside the one that looks for the carry.  On 64 rows of 8,192 tokens x 512 (bfloat16), us forward and
+// backward: 24 tokens x 7 waves 411, 691; x 11 432, 632; 16 tokens x 15 476, 651; x 7 506, 724; 32 tokens x 7 472, 691.
+// Small batches differ by 1 us in 15.
+constexpr int kForwardWaves = 7, kBackwardWaves = 11;
 
 // A launch's words, those of the tiles and of the groups, and its counters: each starting on a line of its own.
 struct Layout {
-    int64_t tiles, words, counters;               // tiles; 64-bit words of tiles and groups; counters
-    size_t bytes;                                 // 0 where one tile holds all
-    Layout(int64_t total, int64_t dim, int32_t dtype)
+    int64_t tiles = 0, words = 0, counters = 0;   // tiles; 64-bit words of tiles and groups; counters
+    size_t bytes = 0;                             // 0 where one tile holds all
+    Layout(int64_t total, int64_t dim, int waves)
     {
-        tiles = words = counters = 0;
-        bytes = 0;
         if (total <= 0 || dim <= 0) return;
-        tiles = tiles_of(total, dim, dtype);
+        tiles = (total + kSteps * waves - 1) / (kSteps * waves);
         if (tiles == 1) return;
         words = (tiles + (tiles + kGroup - 1) / kGroup) * dim;
         words += -words & 15;
@@ -821,34 +818,34 @@ bool paired(const ScanArgs<T> &a)
            ((a.dim | a.x_stride | a.gate_stride | a.dy_stride) & 1) == 0;
 }
 
-template <typename T, int V, int W>
+template <typename T, int V>
 int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hipStream_t s)
 {
     a.n_slabs = (uint32_t)((a.dim + 64 * V - 1) / (64 * V));
     const int64_t widest = std::max({a.x_stride, a.gate_stride, a.dy_stride, a.dim});
     DNATOK_REQUIRE(widest * (int64_t)sizeof(T) * (kSteps + 1) < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: tokens too far apart", who);
-    const int64_t blocks = a.n_slabs * a.n_tiles;
-    DNATOK_REQUIRE(blocks * 64 * (W + 1) < (1ll << 32), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
+    // (eight workgroups of a slab at a time: some find no tile left)
+    const int64_t blocks = a.n_slabs * (a.n_tiles == 1 ? 1 : (a.n_tiles + 7) & ~7ll);
+    const unsigned threads = 64 * ((backward ? kBackwardWaves : kForwardWaves) + 1);
+    DNATOK_REQUIRE(blocks * threads < (1ll << 32), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
     const unsigned grid = (unsigned)blocks;
     if (backward) {
-        if (reverse) gated_scan_backward_kernel<T, V, kSteps, W, true><<<grid, 64 * (W + 1), 0, s>>>(a);
-        else gated_scan_backward_kernel<T, V, kSteps, W, false><<<grid, 64 * (W + 1), 0, s>>>(a);
+        if (reverse) gated_scan_backward_kernel<T, V, kSteps, kBackwardWaves, true><<<grid, threads, 0, s>>>(a);
+        else gated_scan_backward_kernel<T, V, kSteps, kBackwardWaves, false><<<grid, threads, 0, s>>>(a);
     } else {
-        if (reverse) gated_scan_kernel<T, V, kSteps, W, true><<<grid, 64 * (W + 1), 0, s>>>(a);
-        else gated_scan_kernel<T, V, kSteps, W, false><<<grid, 64 * (W + 1), 0, s>>>(a);
+        if (reverse) gated_scan_kernel<T, V, kSteps, kForwardWaves, true><<<grid, threads, 0, s>>>(a);
+        else gated_scan_kernel<T, V, kSteps, kForwardWaves, false><<<grid, threads, 0, s>>>(a);
     }
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
 }
 
 template <typename T>
-int run_scan(const char *who, const ScanArgs<T> &a, int32_t dtype, bool backward, bool reverse, hipStream_t s)
+int run_scan(const char *who, const ScanArgs<T> &a, bool backward, bool reverse, hipStream_t s)
 {
-    const bool wide = waves_of(a.rows.total, a.dim, dtype) == 15;
     if constexpr (sizeof(T) == 2)
-        if (paired(a))
-            return wide ? launch_scan<T, 2, 15>(who, a, backward, reverse, s) : launch_scan<T, 2, 3>(who, a, backward, reverse, s);
-    return wide ? launch_scan<T, 1, 15>(who, a, backward, reverse, s) : launch_scan<T, 1, 3>(who, a, backward, reverse, s);
+        if (paired(a)) return launch_scan<T, 2>(who, a, backward, reverse, s);
+    return launch_scan<T, 1>(who, a, backward, reverse, s);
 }
 
 }  // namespace
@@ -858,9 +855,9 @@ extern "C" size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim)
     return states_bytes(total, dim);
 }
 
-extern "C" size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype)
+extern "C" size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim)
 {
-    return Layout(total, dim, dtype).bytes;
+    return std::max(Layout(total, dim, kForwardWaves).bytes, Layout(total, dim, kBackwardWaves).bytes);
 }
 
 extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
@@ -874,7 +871,7 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(h0, last, n_rows * dim, s);
     SCAN_REQUIRE(x && gate && y, "null buffer");
-    const Layout l(total, dim, dtype);
+    const Layout l(total, dim, kForwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
     int rc = DNATOK_OK;
@@ -886,7 +883,7 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
         a.dim = dim, a.n_tiles = l.tiles, a.h0 = h0, a.states = states;
         a.y = (T *)y, a.last = last;
         if (l.bytes) rc = fill_words(a, l, work, s);
-        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, dtype, false, reverse != 0, s);
+        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, false, reverse != 0, s);
     });
     return rc;
 }
@@ -903,7 +900,7 @@ extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(dlast, dh0, n_rows * dim, s);
     SCAN_REQUIRE(x && gate && states && dx && dgate, "null buffer");
-    const Layout l(total, dim, dtype);
+    const Layout l(total, dim, kBackwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
     int rc = DNATOK_OK;
@@ -916,7 +913,7 @@ extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const
         a.dy = (const T *)dy, a.dy_stride = dy ? dy_stride : 0, a.dlast = dlast;
         a.dx = (T *)dx, a.dgate = (T *)dgate, a.dh0 = dh0;
         if (l.bytes) rc = fill_words(a, l, work, s);
-        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, dtype, true, reverse != 0, s);
+        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, true, reverse != 0, s);
     });
     return rc;
 }

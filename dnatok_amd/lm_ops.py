@@ -77,7 +77,7 @@ class _GatedScan(torch.autograd.Function):
         dgate = torch.empty_like(dx)
         dh0 = torch.empty_like(h0) if h0 is not None and ctx.needs_input_grad[4] else None
         code = _DTYPES[x.dtype]
-        need = L.dnatok_gated_scan_work_bytes(total, dim, code)
+        need = L.dnatok_gated_scan_work_bytes(total, dim)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         with _on(device):
             _lib.check(L.dnatok_gated_scan_backward(
@@ -96,7 +96,7 @@ def _scan_forward(x, gate, offsets, n_rows, h0, reverse, keep_states):
     states = None
     if keep_states:
         states = torch.empty(L.dnatok_gated_scan_states_bytes(total, dim) // 4, dtype=torch.float32, device=device)
-    need = L.dnatok_gated_scan_work_bytes(total, dim, code)
+    need = L.dnatok_gated_scan_work_bytes(total, dim)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     with _on(device):
         _lib.check(L.dnatok_gated_scan(

@@ -435,7 +435,7 @@ int dnatok_normalize_rows(const dnatok_norm_step *steps_h, int32_t n_steps, cons
  * backward pass needs, dnatok_gated_scan_states_bytes(); work is the call's own space,
  * dnatok_gated_scan_work_bytes(), at least 8-byte aligned. */
 size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim);
-size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim, int32_t dtype);
+size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim);
 int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
                       const int64_t *offsets, int64_t n_rows, int64_t total, int64_t dim, int reverse,
                       const float *h0, void *y, float *last, float *states, void *work, size_t work_bytes,
