@@ -12,9 +12,10 @@
 // packed subtraction, there the sum over a group of (128 + q) x is corrected by (128 + zero) times the sum of
 // x (from the matrix cores as well, with ones for W).  Every product is exact in 32 bits, sums are 32-bit sums.
 //
-// A workgroup takes TT x 16 rows of W and its eight waves take the columns in slices of KB x 32; a wave holds its slice of
-// x in registers for all the rows.  A lane loads four words (32 columns of one row); four lanes then exchange words, so
-// that an instruction's 32 columns lie next to each other and in one group.  The waves' sums meet in LDS.
+// A workgroup takes TT x 16 rows of W and its eight waves take the columns in slices of KB x 32.  A lane loads four words (32
+// columns of one row); four lanes then exchange words, so that an instruction's 32 columns lie next to each other and
+// in one group.  The waves' sums meet in LDS.  A wave holds its slice of x in registers (w4_kernel); a single row of x lies in
+// LDS, ready to be multiplied (w4_row_kernel).
 #include "lm_common.hpp"
 
 namespace dnatok {
@@ -51,29 +52,31 @@ struct W4Args {
     int64_t y_stride;
 };
 
-// Eight columns of a row of x, in the order in which the weights come out of a word.
-template <typename T>
-__device__ __forceinline__ typename Frag<T>::type load_x(const W4Args<T> &a, int64_t row, int32_t k)
+// Eight columns of a row of x in the order in which the weights come out of a word.
+__device__ __forceinline__ u32x4 in_order(u32x4 v)
 {
-    u32x4 v = {0, 0, 0, 0};
-    if (row < a.m && k < a.k) {
-        const T *p = a.x + row * a.x_stride + k;
-        if (a.x_aligned && k + 8 <= a.k) {
-            v = *reinterpret_cast<const u32x4 *>(p);
-        } else {
-            uint16_t e[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = k + i < a.k ? __builtin_bit_cast(uint16_t, p[i]) : (uint16_t)0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (uint32_t)e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
-        }
-    }
     u32x4 o;
     o[0] = __builtin_amdgcn_perm(v[2], v[0], 0x05040100);              // columns 0 and 4
     o[1] = __builtin_amdgcn_perm(v[2], v[0], 0x07060302);              // 1 and 5
     o[2] = __builtin_amdgcn_perm(v[3], v[1], 0x05040100);              // 2 and 6
     o[3] = __builtin_amdgcn_perm(v[3], v[1], 0x07060302);              // 3 and 7
-    return __builtin_bit_cast(typename Frag<T>::type, o);
+    return o;
+}
+// Columns k .. k + 7 of a row, zeros behind the last one.
+template <typename T>
+__device__ __forceinline__ u32x4 load_x(const W4Args<T> &a, const T *row, int32_t k)
+{
+    u32x4 v = {0, 0, 0, 0};
+    if (a.x_aligned && k + 8 <= a.k) {
+        v = *reinterpret_cast<const u32x4 *>(row + k);
+    } else {
+        uint16_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = k + i < a.k ? __builtin_bit_cast(uint16_t, row[k + i]) : (uint16_t)0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (uint32_t)e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
+    }
+    return v;
 }
 
 // The weights of a word: 128 + q, or q - zero (`minus`: -1024 - zero, twice).
@@ -82,9 +85,13 @@ __device__ __forceinline__ typename Frag<T>::type unpack(uint32_t q, uint32_t mi
 {
     constexpr bool half = std::is_same<T, _Float16>::value;
     constexpr uint32_t magic = half ? 0x64006400u : 0x43004300u;
+    // (constants in registers: an instruction takes one literal, and `and` with `or` would be two)
+    uint32_t low = 0x000F000Fu, high = magic;
+    asm("" : "+s"(low));
+    asm("" : "+v"(high));
     u32x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (q >> (4 * i) & 0x000F000Fu) | magic;
+    for (int i = 0; i < 4; ++i) o[i] = (q >> (4 * i) & low) | high;
     auto f = __builtin_bit_cast(typename Frag<T>::type, o);
     if constexpr (half) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -113,23 +120,26 @@ struct Slice {
     uint8_t zero[SEGS];
 };
 
-// GB: blocks of a group, if 1, 2 or 4; 1 also for groups of other sizes, whose scale is then looked up for each block.
+// A workgroup's rows of weights: a buffer resource that ends with the matrix (rows and words behind the last one read as
+// zeros; words behind a row's last one are the next row's, and multiplied by zeros of x).
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const W4Args<T> &a, int64_t n0)
+{
+    const int64_t bytes = ((a.n - n0 - 1) * a.w_stride + a.words) * 4;
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(a.w + n0 * a.w_stride), 0, (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF),
+                                             0x00020000);
+}
+
+// Row n0 + local, slice from block b0 on.  GB: blocks with one scale, 1, 2 or 4; groups may be larger.
 template <typename T, int KB, int GB>
-__device__ __forceinline__ void load_slice(const W4Args<T> &a, int64_t row, int32_t b0, int kq, Slice<KB, KB / GB> &s)
+__device__ __forceinline__ void load_slice(const W4Args<T> &a, __amdgpu_buffer_rsrc_t rows, int64_t n0, int local, int32_t b0,
+                                           int kq, Slice<KB, KB / GB> &s)
 {
     constexpr int SEGS = KB / GB;
-    const uint32_t *w = a.w + row * a.w_stride;
-    const bool whole = (b0 + KB) * 4 <= a.words;
+    const int lane_bytes = local * (int)a.w_stride * 4 + kq * 16;      // (a workgroup's rows are less than 2^31 bytes)
 #pragma unroll
-    for (int h = 0; h < KB / 4; ++h) {
-        const int32_t at = b0 * 4 + h * 16 + kq * 4;
-        if (whole) {
-            __builtin_memcpy(&s.q[h], w + at, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s.q[h][j] = at + j < a.words ? w[at + j] : 0;
-        }
-    }
+    for (int h = 0; h < KB / 4; ++h) s.q[h] = __builtin_amdgcn_raw_buffer_load_b128(rows, lane_bytes + h * 64, b0 * 16, 0);
+    const int64_t row = n0 + local < a.n ? n0 + local : a.n - 1;
     const T *scales = a.scales + row * a.n_groups;
     const uint8_t *zeros = a.zeros + row * a.n_groups;
     if (a.per_group == GB && b0 / GB + SEGS <= a.n_groups) {
@@ -148,36 +158,207 @@ __device__ __forceinline__ void load_slice(const W4Args<T> &a, int64_t row, int3
         for (int i = 0; i < SEGS; ++i) s.zero[i] = 8;
 }
 
+// acc += x times a slice of a tile, blocks b0 .. of which a.blocks bounds the last.  x(b, i): columns of block b of the
+// slice, i-th sixteen rows; sum(seg, i): their sum over a segment, where the type needs it.
+template <typename T, int MT, int KB, int GB, typename X, typename Sum>
+__device__ __forceinline__ void multiply(const W4Args<T> &a, const Slice<KB, KB / GB> &s, int32_t b0, X x, Sum sum,
+                                         f32x4 (&acc)[MT])
+{
+    constexpr bool half = std::is_same<T, _Float16>::value;
+    const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 c[MT];
+#pragma unroll
+    for (int h = 0; h < KB / 4; ++h) {
+        const u32x4 q = exchange(s.q[h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = h * 4 + j, seg = b / GB;
+            if (b0 + seg * GB >= a.blocks) break;                      // (uniform: nothing but padding from here on)
+            uint32_t minus = 0;
+            if constexpr (half) {
+                minus = 0xE400u + s.zero[seg];                         // -1024 - zero
+                minus |= minus << 16;
+            }
+            const auto w = unpack<T>(q[j], minus);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) c[i] = mfma(x(b, i), w, b % GB == 0 ? zero4 : c[i]);
+            if ((b + 1) % GB == 0) {
+                const float scale = to_float(__builtin_bit_cast(T, s.scale[seg]));
+                const float off = -128.0f - (float)s.zero[seg];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if constexpr (!half) {
+                        const f32x4 xs = sum(seg, i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[i][e] = fmaf(off, xs[e], c[i][e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(scale, c[i][e], acc[i][e]);
+                }
+            }
+        }
+    }
+}
+
+// The waves' sums meet, RT tiles of sixteen rows of W at a time, and go to y.  `sums`: [kW4Waves][RT][MT][64].
+template <typename T, typename OUT, int MT, int TT, int RT>
+__device__ __forceinline__ void write_out(const W4Args<T> &a, f32x4 *sums, const f32x4 (&acc)[TT][MT], int64_t n0, int64_t m0,
+                                          int wave, int lane)
+{
+    constexpr int kThreads = 64 * kW4Waves, kOuts = RT * MT * 256, kEach = (kOuts + kThreads - 1) / kThreads;
+#pragma unroll
+    for (int t0 = 0; t0 < TT; t0 += RT) {
+        float bias[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {                              // (on its way while the sums are put down)
+            const int64_t n = n0 + (t0 + (e * kThreads + threadIdx.x) / (MT * 256)) * 16 + threadIdx.x % 16;
+            bias[e] = a.bias ? a.bias[n < a.n ? n : a.n - 1] : 0.0f;
+        }
+        if (t0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sums[((wave * RT + t) * MT + i) * 64 + lane] = acc[t0 + t][i];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int o = e * kThreads + threadIdx.x;
+            if (kOuts % kThreads && o >= kOuts) break;
+            const int t = o / (MT * 256), i = o / 256 % MT, col = o % 16, in = o / 16 % 16;     // 16 rows of W next to each other
+            const int64_t n = n0 + (t0 + t) * 16 + col, m = m0 + i * 16 + in;
+            if (n < a.n && m < a.m) {
+                const float *from = reinterpret_cast<const float *>(sums + (t * MT + i) * 64 + in / 4 * 16 + col) + in % 4;
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kW4Waves; ++w) sum += from[w * RT * MT * 256];
+                ((OUT *)a.y)[m * a.y_stride + n] = from_float<OUT>(sum + bias[e]);
+            }
+        }
+    }
+}
+
+// One row of x, in LDS; all sixteen rows of an instruction hold it.  A workgroup takes one tile; its waves request their first
+// two slices of weights before they look at x, and stay two slices ahead.
+template <typename T, typename OUT, int KB, int GB>
+__global__ __launch_bounds__(64 * kW4Waves) void w4_row_kernel(W4Args<T> a)
+{
+    constexpr bool half = std::is_same<T, _Float16>::value;
+    constexpr int SEGS = KB / GB, kThreads = 64 * kW4Waves, kStep = kW4Waves * KB;
+    typedef typename Frag<T>::type frag;
+    __shared__ float sums[kW4Waves][16];
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    const int32_t units = (a.blocks + KB - 1) / KB * KB * 4;           // of eight columns
+    u32x4 *const xs = reinterpret_cast<u32x4 *>(dynamic);              // [units]
+    float *const unit_sums = reinterpret_cast<float *>(xs + units);    // [units]
+    float *const seg_sums = unit_sums + units;                         // [units / 4 / GB]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, kq = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const __amdgpu_buffer_rsrc_t rows = rows_from(a, n0);
+    int32_t b0 = wave * KB;
+    Slice<KB, SEGS> even, odd;
+    const auto load = [&](Slice<KB, SEGS> &s, int32_t at) {
+        if (at < a.blocks) load_slice<T, KB, GB>(a, rows, n0, r, at, kq, s);
+    };
+    load(even, b0);
+    load(odd, b0 + kStep);
+    const int64_t n = n0 + r;
+    const float bias = a.bias && n < a.n ? a.bias[n] : 0.0f;
+
+    for (int32_t unit = threadIdx.x; unit < units; unit += kThreads) {
+        const u32x4 v = load_x<T>(a, a.x, unit * 8);
+        xs[unit] = in_order(v);
+        if constexpr (!half) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xFFFF0000u);
+            unit_sums[unit] = sum;
+        }
+    }
+    __syncthreads();
+    if constexpr (!half) {
+        for (int32_t o = threadIdx.x; o < units / 4 / GB; o += kThreads) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * GB; ++i) sum += unit_sums[o * 4 * GB + i];
+            seg_sums[o] = sum;
+        }
+        __syncthreads();
+    }
+    f32x4 acc[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+    const auto use = [&](const Slice<KB, SEGS> &s, int32_t at) {
+        const u32x4 *const mine = xs + at * 4 + kq;
+        const float *const seg = seg_sums + at / GB;
+        multiply<T, 1, KB, GB>(a, s, at, [&](int b, int) { return __builtin_bit_cast(frag, mine[b * 4]); },
+                               [&](int i, int) {
+                                   const float v = seg[i];
+                                   return f32x4{v, v, v, v};
+                               },
+                               acc);
+    };
+    for (; b0 < a.blocks; b0 += 2 * kStep) {
+        use(even, b0);
+        load(even, b0 + 2 * kStep);
+        if (b0 + kStep >= a.blocks) break;
+        use(odd, b0 + kStep);
+        load(odd, b0 + 3 * kStep);
+    }
+    if (lane < 16) sums[wave][r] = acc[0][0];
+    __syncthreads();
+    if (threadIdx.x < 16 && n < a.n) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kW4Waves; ++w) sum += sums[w][threadIdx.x];
+        ((OUT *)a.y)[n] = from_float<OUT>(sum + bias);
+    }
+}
+
 template <typename T, typename OUT, int MT, int KB, int TT, int GB>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
 {
     constexpr bool half = std::is_same<T, _Float16>::value;
     constexpr int SEGS = KB / GB;
     typedef typename Frag<T>::type frag;
-    __shared__ f32x4 sums[kW4Waves][MT][64];
+    constexpr int RT = TT * MT <= 4 ? TT : TT * MT <= 8 ? TT / 2 : TT / 4;
+    __shared__ f32x4 sums[kW4Waves * RT * MT * 64];
     __shared__ f32x4 x_sums[half ? 1 : kW4Waves][SEGS][MT][4];         // of the slice's segments, four rows of x to an entry
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, kq = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * (16 * TT), m0 = (int64_t)blockIdx.y * (16 * MT);
+    const __amdgpu_buffer_rsrc_t rows = rows_from(a, n0);
     const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 acc[TT][MT];
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[t][i] = zero4;
+    const T *x_row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = m0 + i * 16 + r;
+        x_row[i] = a.x + (m < a.m ? m : a.m - 1) * a.x_stride + kq * 8;
+    }
 
-    const auto row_of = [&](int t) {
-        const int64_t row = n0 + t * 16 + r;
-        return row < a.n ? row : a.n - 1;
-    };
     for (int32_t b0 = wave * KB; b0 < a.blocks; b0 += kW4Waves * KB) {
         Slice<KB, SEGS> next;
-        load_slice<T, KB, GB>(a, row_of(0), b0, kq, next);
+        load_slice<T, KB, GB>(a, rows, n0, r, b0, kq, next);
+        u32x4 raw[KB][MT];
+        if (a.x_aligned && (b0 + KB) * 32 <= a.k) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) raw[b][i] = *reinterpret_cast<const u32x4 *>(x_row[i] + (b0 + b) * 32);
+        } else {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) raw[b][i] = load_x<T>(a, x_row[i] - kq * 8, (b0 + b) * 32 + kq * 8);
+        }
         frag x[KB][MT];
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x[b][i] = load_x<T>(a, m0 + i * 16 + r, (b0 + b) * 32 + kq * 8);
+            for (int i = 0; i < MT; ++i) x[b][i] = __builtin_bit_cast(frag, in_order(raw[b][i]));
         if constexpr (!half) {
             frag ones;
 #pragma unroll
@@ -195,62 +376,14 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
         }
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-            Slice<KB, SEGS> s = next;
-            if (t + 1 < TT) load_slice<T, KB, GB>(a, row_of(t + 1), b0, kq, next);
-            f32x4 c[MT];
-#pragma unroll
-            for (int h = 0; h < KB / 4; ++h) {
-                const u32x4 q = exchange(s.q[h]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int b = h * 4 + j, seg = b / GB;
-                    if (b0 + seg * GB >= a.blocks) break;              // (uniform: nothing but padding from here on)
-                    uint32_t minus = 0;
-                    if constexpr (half) {
-                        minus = 0xE400u + s.zero[seg];                 // -1024 - zero
-                        minus |= minus << 16;
-                    }
-                    const frag w = unpack<T>(q[j], minus);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) c[i] = mfma(x[b][i], w, b % GB == 0 ? zero4 : c[i]);
-                    if ((b + 1) % GB == 0) {
-                        const float scale = to_float(__builtin_bit_cast(T, s.scale[seg]));
-                        const float off = -128.0f - (float)s.zero[seg];
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            if constexpr (!half) {
-                                const f32x4 sum = x_sums[wave][seg][i][kq];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) c[i][e] = fmaf(off, sum[e], c[i][e]);
-                            }
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(scale, c[i][e], acc[t][i][e]);
-                        }
-                    }
-                }
-            }
+            const Slice<KB, SEGS> s = next;
+            if (t + 1 < TT) load_slice<T, KB, GB>(a, rows, n0, (t + 1) * 16 + r, b0, kq, next);
+            multiply<T, MT, KB, GB>(a, s, b0, [&](int b, int i) { return x[b][i]; },
+                                    [&](int seg, int i) { return x_sums[wave][seg][i][kq]; }, acc[t]);
         }
         if constexpr (!half) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        if (t) __syncthreads();
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[t][i];
-        __syncthreads();
-        for (int o = threadIdx.x; o < MT * 256; o += 64 * kW4Waves) {
-            const int i = o >> 8, col = o & 15, in = o >> 4 & 15;      // 16 rows of W next to each other, then rows of x
-            const int64_t n = n0 + t * 16 + col, m = m0 + i * 16 + in;
-            if (n < a.n && m < a.m) {
-                const int from = (in >> 2) * 16 + col;
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kW4Waves; ++w) sum += sums[w][i][from][in & 3];
-                ((OUT *)a.y)[m * a.y_stride + n] = from_float<OUT>(sum + (a.bias ? a.bias[n] : 0.0f));
-            }
-        }
-    }
+    write_out<T, OUT, MT, TT, RT>(a, sums, acc, n0, m0, wave, lane);
 }
 
 }  // namespace dnatok
@@ -263,28 +396,47 @@ template <typename T, typename OUT, int MT, int KB, int TT>
 void launch_w4(const W4Args<T> &a, hipStream_t s)
 {
     const dim3 grid((unsigned)((a.n + 16 * TT - 1) / (16 * TT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-    if (a.per_group == 4) w4_kernel<T, OUT, MT, KB, TT, 4><<<grid, 64 * kW4Waves, 0, s>>>(a);
-    else if (a.per_group == 2) w4_kernel<T, OUT, MT, KB, TT, 2><<<grid, 64 * kW4Waves, 0, s>>>(a);
+    if (a.per_group % 4 == 0) w4_kernel<T, OUT, MT, KB, TT, 4><<<grid, 64 * kW4Waves, 0, s>>>(a);
+    else if (a.per_group % 2 == 0) w4_kernel<T, OUT, MT, KB, TT, 2><<<grid, 64 * kW4Waves, 0, s>>>(a);
     else w4_kernel<T, OUT, MT, KB, TT, 1><<<grid, 64 * kW4Waves, 0, s>>>(a);
 }
 
-// Sixteen-row tiles to a workgroup: as many as leave two workgroups for each of the 256 CUs.
-template <typename T, typename OUT, int MT, int KB>
-void launch_w4_rows(const W4Args<T> &a, hipStream_t s)
+// Tiles to a workgroup, so that x is fetched less often: as many as leave about a workgroup for each of the 256 CUs.  us for
+// 1, 2, 4 tiles: 8 x 4096 x 4096 8.1, 10.4, 15; 8 x 8192 x 4096 11.3, 9.6, -; 32 x 8192 x 4096 (1,024 tiles) -, 17.6, 15.4.
+template <typename T, typename OUT, int KB>
+void launch_w4_tiles(const W4Args<T> &a, hipStream_t s)
 {
-    const int64_t groups = (a.n + 15) / 16 * ((a.m + 16 * MT - 1) / (16 * MT));
-    if (groups >= 2048) launch_w4<T, OUT, MT, KB, 4>(a, s);
-    else if (groups >= 1024) launch_w4<T, OUT, MT, KB, 2>(a, s);
-    else launch_w4<T, OUT, MT, KB, 1>(a, s);
+    const int64_t tiles = (a.n + 15) / 16 * ((a.m + 15) / 16);
+    if (tiles >= 900) launch_w4<T, OUT, 1, KB, 4>(a, s);
+    else if (tiles >= 450) launch_w4<T, OUT, 1, KB, 2>(a, s);
+    else launch_w4<T, OUT, 1, KB, 1>(a, s);
+}
+
+// Bytes of LDS that one row of x takes, and the most that is given to it: three workgroups on a CU, with their registers.
+constexpr int64_t kRowLds = 48 * 1024;
+template <typename T>
+int64_t row_lds(const W4Args<T> &a)
+{
+    return (a.blocks + 7) / 8 * 32 * (std::is_same<T, _Float16>::value ? 16 : 16 + 4 + 1);
 }
 
 template <typename T, typename OUT>
 void run_w4(const W4Args<T> &a, hipStream_t s)
 {
-    if (a.m > 32) launch_w4_rows<T, OUT, 4, 4>(a, s);
-    else if (a.m > 16) launch_w4_rows<T, OUT, 2, 4>(a, s);
-    else if (a.k <= 32 * 4 * kW4Waves) launch_w4_rows<T, OUT, 1, 4>(a, s);
-    else launch_w4_rows<T, OUT, 1, 8>(a, s);
+    if (a.m == 1 && row_lds(a) <= kRowLds) {
+        const unsigned grid = (unsigned)((a.n + 15) / 16), lds = (unsigned)row_lds(a);
+        if (a.per_group % 4 == 0) w4_row_kernel<T, OUT, 8, 4><<<grid, 64 * kW4Waves, lds, s>>>(a);
+        else if (a.per_group % 2 == 0) w4_row_kernel<T, OUT, 8, 2><<<grid, 64 * kW4Waves, lds, s>>>(a);
+        else w4_row_kernel<T, OUT, 8, 1><<<grid, 64 * kW4Waves, lds, s>>>(a);
+    } else if (a.m > 32 && a.n >= 16 * 640) {
+        // weights unpacked once for 64 rows.  61 x 12301 x 2040: 16.2 us, in blocks of 16 rows 20.6; 64 x 32000 x 2048: 45, 63;
+        // with fewer rows of W there are too few workgroups: 64 x 8192 x 8192 58, 46
+        launch_w4<T, OUT, 4, 4, 4>(a, s);
+    } else if (a.k > 1024) {
+        launch_w4_tiles<T, OUT, 8>(a, s);
+    } else {
+        launch_w4_tiles<T, OUT, 4>(a, s);                              // (a slice to a wave at most)
+    }
 }
 
 }  // namespace
@@ -303,8 +455,8 @@ extern "C" int dnatok_w4_matvec(const void *x, int64_t x_stride, int32_t dtype, 
     W4_REQUIRE(weight_stride >= (k + 7) / 8, "weight rows overlap");
     if (m == 0 || n == 0) return DNATOK_OK;
     W4_REQUIRE(x && weights && scales && y, "null buffer");
-    DNATOK_REQUIRE(n < (1ll << 31) && m <= 65535 && k < (1ll << 30), DNATOK_E_TOO_LARGE,
-                   "%s: at most 2^31 outputs of 65535 rows, 2^30 columns", who);
+    DNATOK_REQUIRE(n < (1ll << 31) && m <= 65535 && weight_stride < (1ll << 22), DNATOK_E_TOO_LARGE,
+                   "%s: at most 2^31 outputs of 65535 rows, 2^22 words between rows of weights", who);
     hipStream_t s = (hipStream_t)stream;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
