@@ -86,13 +86,48 @@ static PyObject *pack_strings(PyObject *self, PyObject *args)
     return Py_BuildValue("(nnnn)", n, total, longest, bytes_at);
 }
 
+/* call(address, ...): calls the C function at `address`, whose arguments are all integers or pointers (None: NULL), and
+ * returns its int.  What ctypes does in 2 - 3 us, which is a fifth of a small operator's call, in 0.3: an integer or
+ * pointer argument travels in a 64-bit register or stack slot whatever its width. */
+#define CALL_MAX 24
+typedef int (*int_function)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                            int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                            int64_t, int64_t, int64_t, int64_t);
+
+static PyObject *call(PyObject *self, PyObject *const *args, Py_ssize_t n)
+{
+    (void)self;
+    if (n < 1 || n > CALL_MAX + 1) {
+        PyErr_SetString(PyExc_TypeError, "call() takes an address and at most 24 integers");
+        return NULL;
+    }
+    int64_t a[CALL_MAX + 1] = {0};
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (args[i] == Py_None) continue;
+        a[i] = PyLong_AsLongLong(args[i]);
+        if (a[i] == -1 && PyErr_Occurred()) return NULL;
+    }
+    if (!a[0]) {
+        PyErr_SetString(PyExc_TypeError, "call() needs an address");
+        return NULL;
+    }
+    const int_function f = (int_function)(uintptr_t)a[0];
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = f(a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15], a[16], a[17],
+           a[18], a[19], a[20], a[21], a[22], a[23], a[24]);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
+    {"call", (PyCFunction)(void (*)(void))call, METH_FASTCALL, "call(address, *integers) -> int"},
     {"pack_strings", pack_strings, METH_VARARGS,
      "pack_strings(seqs, address, capacity, utf8) -> (n, total, longest, bytes_at) or -needed"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hostpack",
-                                    "Strings of a batch into one byte buffer + offsets, in C.", -1, methods,
+                                    "Strings of a batch into one byte buffer + offsets, and quick calls of C functions, in C.", -1, methods,
                                     NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__hostpack(void) { return PyModule_Create(&module); }

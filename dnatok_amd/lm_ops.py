@@ -7,7 +7,8 @@ reference has no counterpart.
 """
 from __future__ import annotations
 
-import contextlib
+import ctypes
+import functools
 from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -15,20 +16,35 @@ import torch
 
 from . import _lib
 
+try:                                    # quick calls; without the C module ctypes makes them
+    from ._hostpack import call as _quick_call
+except ImportError:                     # pragma: no cover
+    _quick_call = None
+
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_NO_GUARD = contextlib.nullcontext()
 
 
-def _stream(device: torch.device) -> int:
-    # (see encoders._stream: the raw handle is much cheaper than the Stream object)
-    if _raw_stream is not None:
-        return _raw_stream(device.index)
-    return torch.cuda.current_stream(device).cuda_stream
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    """A C entry point that takes integers and pointers and returns a status."""
+    fn = getattr(_lib.lib(), name)
+    if _quick_call is None:
+        return fn
+    return functools.partial(_quick_call, ctypes.cast(fn, ctypes.c_void_p).value)
 
 
-def _on(device: torch.device):
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _run(name: str, device: torch.device, *args) -> None:
+    """Calls an entry point on the current stream of ``device``, the last argument of all of them."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        stream = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+        rc = _entry(name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = _entry(name)(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -37,13 +53,15 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 def _require_rows(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: torch.device) -> int:
     """A matrix whose rows' elements lie next to each other; returns the elements between rows."""
-    if t.device != device or t.dtype != dtype or t.shape != shape or not (t.stride(-1) == 1 or t.shape[-1] == 1):
-        raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with contiguous rows")
-    return t.stride(0)
+    if t.dtype is dtype and t.shape == shape and t.device == device:
+        stride = t.stride()
+        if stride[1] == 1 or shape[1] == 1:
+            return stride[0]
+    raise ValueError(f"{name} must be a {dtype} tensor {tuple(shape)} on {device} with contiguous rows")
 
 
 def _require(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, device: torch.device) -> None:
-    if t is not None and (t.device != device or t.dtype != dtype or t.shape != shape or not t.is_contiguous()):
+    if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.device == device):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}")
 
 
@@ -79,12 +97,10 @@ class _GatedScan(torch.autograd.Function):
         code = _DTYPES[x.dtype]
         need = L.dnatok_gated_scan_work_bytes(total, dim)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        with _on(device):
-            _lib.check(L.dnatok_gated_scan_backward(
-                x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, _ptr(offsets), ctx.n_rows, total, dim,
-                int(ctx.reverse), _ptr(h0), _ptr(dy), 0 if dy is None else dy.stride(0), _ptr(dlast), states.data_ptr(),
-                dx.data_ptr(), dgate.data_ptr(), _ptr(dh0), _ptr(work), need, _stream(device)),
-                "dnatok_gated_scan_backward")
+        _run("dnatok_gated_scan_backward", device, x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code,
+             _ptr(offsets), ctx.n_rows, total, dim, int(ctx.reverse), _ptr(h0), _ptr(dy),
+             0 if dy is None else dy.stride(0), _ptr(dlast), states.data_ptr(), dx.data_ptr(), dgate.data_ptr(), _ptr(dh0),
+             _ptr(work), need)
         return dx, dgate, None, None, dh0, None
 
 
@@ -98,11 +114,8 @@ def _scan_forward(x, gate, offsets, n_rows, h0, reverse, keep_states):
         states = torch.empty(L.dnatok_gated_scan_states_bytes(total, dim) // 4, dtype=torch.float32, device=device)
     need = L.dnatok_gated_scan_work_bytes(total, dim)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with _on(device):
-        _lib.check(L.dnatok_gated_scan(
-            x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, _ptr(offsets), n_rows, total, dim,
-            int(reverse), _ptr(h0), y.data_ptr(), last.data_ptr(), _ptr(states), _ptr(work), need, _stream(device)),
-            "dnatok_gated_scan")
+    _run("dnatok_gated_scan", device, x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0), code, _ptr(offsets), n_rows,
+         total, dim, int(reverse), _ptr(h0), y.data_ptr(), last.data_ptr(), _ptr(states), _ptr(work), need)
     return y, last, states
 
 
@@ -152,21 +165,19 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
     float32 [B, D] (zero if not given).  Returns ``(y, new_state)``; ``out_state`` receives the new state and may be
     ``state`` itself.  Without gradients."""
     _require_floats(x, "x")
-    if x.dim() != 2 or x.shape[1] == 0:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) != 2 or shape[1] == 0:
         raise ValueError("x must be [B, D]")
-    device = x.device
-    xs = _require_rows(x, "x", x.shape, x.dtype, device)
-    gs = _require_rows(gate, "gate", x.shape, x.dtype, device)
-    _require(state, "state", x.shape, torch.float32, device)
-    _require(out_state, "out_state", x.shape, torch.float32, device)
+    xs = _require_rows(x, "x", shape, dtype, device)
+    gs = _require_rows(gate, "gate", shape, dtype, device)
+    _require(state, "state", shape, torch.float32, device)
+    _require(out_state, "out_state", shape, torch.float32, device)
     _forward_only("gated_step", x, gate, state)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if out_state is None:
-        out_state = torch.empty(x.shape, dtype=torch.float32, device=device)
-    with _on(device):
-        _lib.check(_lib.lib().dnatok_gated_step(x.data_ptr(), xs, gate.data_ptr(), gs, _DTYPES[x.dtype], _ptr(state),
-                                                x.shape[0], x.shape[1], y.data_ptr(), out_state.data_ptr(),
-                                                _stream(device)), "dnatok_gated_step")
+        out_state = torch.empty_like(y, dtype=torch.float32)
+    _run("dnatok_gated_step", device, x.data_ptr(), xs, gate.data_ptr(), gs, _DTYPES[dtype], _ptr(state), shape[0], shape[1],
+         y.data_ptr(), out_state.data_ptr())
     return y, out_state
 
 
@@ -252,15 +263,13 @@ class W4Matrix:
         if out_dtype not in (x.dtype, torch.float32):
             raise ValueError("out_dtype must be x's type or float32")
         if out is None:
-            out = torch.empty((m, n), dtype=out_dtype, device=device)
+            out = x.new_empty((m, n), dtype=out_dtype)
         elif squeeze:
             out = out.unsqueeze(0)
         ys = _require_rows(out, "out", (m, n), out_dtype, device)
-        with _on(device):
-            _lib.check(_lib.lib().dnatok_w4_matvec(
-                x.data_ptr(), xs, _DTYPES[x.dtype], self.q.data_ptr(), self.q.stride(0), self.scales.data_ptr(),
-                _ptr(self.zeros), m, n, k, self.group, _ptr(bias), out.data_ptr(), ys, _DTYPES[out_dtype],
-                _stream(device)), "dnatok_w4_matvec")
+        _run("dnatok_w4_matvec", device, x.data_ptr(), xs, _DTYPES[x.dtype], self.q.data_ptr(), self.q.stride(0),
+             self.scales.data_ptr(), _ptr(self.zeros), m, n, k, self.group, _ptr(bias), out.data_ptr(), ys,
+             _DTYPES[out_dtype])
         return out[0] if squeeze else out
 
 
@@ -328,15 +337,90 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     if out_dtype not in (logits.dtype, torch.float32):
         raise ValueError("out_dtype must be the logits' type or float32")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=out_dtype, device=device)
+        out = torch.empty_like(logits, dtype=out_dtype, memory_format=torch.contiguous_format)
     out_stride = _require_rows(out, "out", (rows, vocab), out_dtype, device)
     repetition = _per_row(repetition, "repetition", rows, device)
     presence = _per_row(presence, "presence", rows, device)
     frequency = _per_row(frequency, "frequency", rows, device)
-    with _on(device):
-        _lib.check(_lib.lib().dnatok_logits_process(
-            logits.data_ptr(), stride, _DTYPES[logits.dtype], rows, vocab, _ptr(history), _ptr(history_offsets),
-            _ptr(prompt_lengths), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias), bias_stride,
-            _ptr(allowed), allowed_stride, n_states, _ptr(state), out.data_ptr(), out_stride, _DTYPES[out_dtype],
-            _stream(device)), "dnatok_logits_process")
+    _run("dnatok_logits_process", device, logits.data_ptr(), stride, _DTYPES[logits.dtype], rows, vocab, _ptr(history),
+         _ptr(history_offsets), _ptr(prompt_lengths), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias),
+         bias_stride, _ptr(allowed), allowed_stride, n_states, _ptr(state), out.data_ptr(), out_stride, _DTYPES[out_dtype])
     return out
+
+
+# the letters of a motif (IUPAC), and the bases that each stands for
+IUPAC = {"A": "A", "C": "C", "G": "G", "T": "T", "R": "AG", "Y": "CT", "S": "CG", "W": "AT", "K": "GT", "M": "AC",
+         "B": "CGT", "D": "AGT", "H": "ACT", "V": "ACG", "N": "ACGT"}
+
+
+def token_bytes(vocab) -> list:
+    """A tokenizer's vocabulary (token -> id) as the bytes of each id; None for ids whose token is not made of
+    bases."""
+    tokens = [None] * (max(vocab.values(), default=-1) + 1)
+    for token, i in vocab.items():
+        if token and not token.strip("ACGTN"):
+            tokens[i] = token.encode("ascii")
+    return tokens
+
+
+class TokenGrammar:
+    """A finite automaton over bytes, as bit masks and next states over a vocabulary's tokens.
+
+    ``transitions`` [S, 256] holds the next state for each state and byte, -1 for none; ``tokens`` the bytes
+    of each id (None: never allowed, see :func:`token_bytes`).  A token is allowed in a state if all its bytes can be
+    followed from there; ``eos_id`` in the states of ``accepting`` only.  ``allowed`` int32 [S, ceil(V / 32)] is what
+    :func:`process_logits` takes; ``advance`` follows the tokens that were chosen.  State S, behind the last one, is
+    that of a row which took a forbidden token: nothing may follow."""
+
+    def __init__(self, transitions, tokens: Sequence[Optional[bytes]], *, accepting: Sequence[int] = (),
+                 eos_id: Optional[int] = None, device="cuda"):
+        trans = np.ascontiguousarray(transitions, dtype=np.int32)
+        if trans.ndim != 2 or trans.shape[1] != 256 or trans.shape[0] == 0:
+            raise ValueError("transitions must be [S, 256]")
+        s, v = trans.shape[0], len(tokens)
+        if v == 0:
+            raise ValueError("no tokens")
+        if trans.min() < -1 or trans.max() >= s:
+            raise ValueError("transitions lead to states that are not there")
+        if eos_id is not None and not 0 <= eos_id < v:
+            raise ValueError("eos_id is not in the vocabulary")
+        lengths = np.array([0 if t is None else len(t) for t in tokens])
+        table = np.zeros((v, max(1, lengths.max())), dtype=np.uint8)
+        for i, t in enumerate(tokens):
+            if t:
+                table[i, :len(t)] = np.frombuffer(t, dtype=np.uint8)
+        dead = np.concatenate([trans, np.full((1, 256), -1, dtype=np.int32)])     # (row -1: dead stays dead)
+        state = np.where(lengths > 0, np.arange(s, dtype=np.int32)[:, None], -1)
+        for at in range(table.shape[1]):
+            state = np.where(lengths > at, dead[state, table[:, at]], state)
+        if eos_id is not None:
+            state[:, eos_id] = -1
+            for a in accepting:
+                state[a, eos_id] = a
+        self.n_states, self.vocab = s, v
+        bits = np.zeros((s, -(-v // 32) * 32), dtype=np.uint8)
+        bits[:, :v] = state >= 0
+        words = np.packbits(bits, axis=1, bitorder="little").view("<u4").view(np.int32)
+        following = np.concatenate([np.where(state < 0, s, state), np.full((1, v), s)]).astype(np.int32)
+        self.allowed = torch.from_numpy(np.ascontiguousarray(words)).to(device)
+        self.next_state = torch.from_numpy(following).to(device)
+
+    @classmethod
+    def from_iupac(cls, pattern: str, tokens: Sequence[Optional[bytes]], *, repeat: bool = False,
+                   eos_id: Optional[int] = None, device="cuda") -> "TokenGrammar":
+        """Sequences that spell ``pattern`` (IUPAC letters), once, or again and again with ``repeat``.  State i: i letters
+        of the pattern are there; the sequence may end where the pattern does."""
+        n = len(pattern)
+        if n == 0 or any(c not in IUPAC for c in pattern.upper()):
+            raise ValueError("pattern must be IUPAC letters")
+        states = n if repeat else n + 1
+        trans = np.full((states, 256), -1, dtype=np.int32)
+        for i, c in enumerate(pattern.upper()):
+            for base in IUPAC[c]:
+                trans[i, ord(base)] = (i + 1) % states
+        return cls(trans, tokens, accepting=[0] if repeat else [n], eos_id=eos_id, device=device)
+
+    def advance(self, state: torch.Tensor, token: torch.Tensor) -> torch.Tensor:
+        """The states of rows in ``state`` int32 [B] that took ``token`` [B]; negative states stay."""
+        at = state.clamp(0, self.n_states).long()
+        return torch.where(state < 0, state, self.next_state[at, token.long()])

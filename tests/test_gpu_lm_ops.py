@@ -583,3 +583,21 @@ def test_nothing_to_do():
     q, scales, z, xh, b = w4_inputs(0, 16, 64, 32, torch.bfloat16, True)
     assert lm_ops.W4Matrix(q, scales, z, in_features=64, group=32).matvec(xh).shape == (0, 16)
     assert lm_ops.process_logits(torch.empty((0, 9), device=DEV)).shape == (0, 9)
+
+
+# ---- all of them together -----------------------------------------------------------------------
+
+def test_example_trains_and_generates_what_the_motif_allows(capsys):
+    import importlib.util
+    import os
+    import re
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "generate_dna.py")
+    spec = importlib.util.spec_from_file_location("generate_dna", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    print("example: 12 training steps, a motif", flush=True)
+    losses, sequences = example.main(["--motif", "ATGNNNRYNNTAA", "--rows", "3", "--train", "12"])
+    assert len(losses) == 12 and losses[-1] < losses[0]
+    assert len(sequences) == 3
+    for s in sequences:
+        assert re.fullmatch("ATG[ACGT]{3}[AG][CT][ACGT]{2}TAA", s), s

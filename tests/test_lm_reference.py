@@ -88,3 +88,61 @@ def test_wrappers_refuse_tensors_that_are_not_on_the_gpu():
         lm_ops.W4Matrix(torch.zeros((4, 1), dtype=torch.int32), torch.ones(4, 1).bfloat16(), in_features=8, group=32)
     with pytest.raises(ValueError, match="GPU"):
         lm_ops.process_logits(x)
+
+
+def test_token_grammar_by_hand():
+    tokens = [b"A", b"C", b"G", b"T", b"AC", b"GT", b"ACG", None, b"TTT"]
+    g = lm_ops.TokenGrammar.from_iupac("ANG", tokens, eos_id=7, device="cpu")
+    assert g.n_states == 4 and g.allowed.shape == (4, 1) and g.next_state.shape == (5, 9)
+    bits = lambda s: [v for v in range(9) if int(g.allowed[s, 0]) >> v & 1]
+    assert bits(0) == [0, 4, 6] and bits(1) == [0, 1, 2, 3] and bits(2) == [2] and bits(3) == [7]
+    # (state 1 allows CG, none of the tokens; GT has T where G must be)
+    assert g.next_state[0].tolist() == [1, 4, 4, 4, 2, 4, 3, 4, 4]
+    assert g.next_state[4].tolist() == [4] * 9                          # a row that took what was forbidden
+    state = g.advance(torch.tensor([0, 0, -1, 4, 3], dtype=torch.int32), torch.tensor([4, 8, 3, 0, 7]))
+    assert state.tolist() == [2, 4, -1, 4, 3]
+    again = lm_ops.TokenGrammar.from_iupac("AY", tokens, repeat=True, device="cpu")
+    assert again.n_states == 2 and again.next_state[0, 4] == 0 and again.next_state[0, 6] == 2
+
+
+@pytest.mark.parametrize("vocab", [31, 32, 33, 200])
+def test_token_grammar_against_following_every_byte(vocab):
+    rng = np.random.default_rng(vocab)
+    tokens = [None if rng.random() < 0.1 else bytes(rng.choice(list(b"ACGT"), rng.integers(1, 6))) for _ in range(vocab)]
+    trans = np.full((6, 256), -1)
+    trans[:, list(b"ACGT")] = rng.integers(-1, 6, (6, 4))
+    g = lm_ops.TokenGrammar(trans, tokens, device="cpu")
+    for s in range(6):
+        for v, t in enumerate(tokens):
+            at = s if t else -1
+            for byte in t or b"":
+                at = trans[at, byte] if at >= 0 else -1
+            assert (int(g.allowed[s, v >> 5]) >> (v & 31) & 1) == (at >= 0)
+            assert g.next_state[s, v] == (at if at >= 0 else 6)
+
+
+def test_token_grammar_refusals():
+    for bad in (lambda: lm_ops.TokenGrammar(np.zeros((2, 255)), [b"A"], device="cpu"),
+                lambda: lm_ops.TokenGrammar(np.full((2, 256), 2), [b"A"], device="cpu"),
+                lambda: lm_ops.TokenGrammar(np.zeros((2, 256)), [], device="cpu"),
+                lambda: lm_ops.TokenGrammar(np.zeros((2, 256)), [b"A"], eos_id=1, device="cpu"),
+                lambda: lm_ops.TokenGrammar.from_iupac("AXG", [b"A"], device="cpu"),
+                lambda: lm_ops.TokenGrammar.from_iupac("", [b"A"], device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_token_bytes():
+    assert lm_ops.token_bytes({"A": 1, "[PAD]": 0, "ACGN": 3, "<unk>": 2}) == [None, b"A", None, b"ACGN"]
+
+
+def test_quick_calls_are_the_calls_of_ctypes():
+    from dnatok_amd import _hostpack
+    L = _lib.lib()
+    address = ctypes.cast(L.dnatok_w4_matvec, ctypes.c_void_p).value
+    args = (4096, 64, 1, 4096, 7, 4096, None, 1, 4, 64, 32, None, 4096, 4, 1, None)
+    assert _hostpack.call(address, *args) == L.dnatok_w4_matvec(*args) == -1
+    assert b"overlap" in L.dnatok_last_error()
+    for bad in ((), (0, 1), (None,), (address, "x"), (address,) + (0,) * 25):
+        with pytest.raises(TypeError):
+            _hostpack.call(*bad)
