@@ -37,9 +37,12 @@ constexpr int kCounterStride = 32;                // (a 128-byte line to a count
 
 __global__ __launch_bounds__(256) void fill_words_kernel(uint64_t *words, int64_t n, int64_t n_counters)
 {
+    typedef uint64_t two __attribute__((ext_vector_type(2)));         // (n is a multiple of 16, a counter 16 words)
     const int64_t all = n + n_counters * kCounterStride / 2;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256)
-        words[i] = i < n ? kNoWord : 0;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 2; i < all; i += (int64_t)gridDim.x * 512) {
+        const uint64_t v = i < n ? kNoWord : 0;
+        *reinterpret_cast<two *>(words + i) = two{v, v};
+    }
 }
 
 template <typename T>
@@ -444,7 +447,9 @@ struct Strip {
         if constexpr (V * sizeof(T) == 4) {
             uint32_t w;
             __builtin_memcpy(&w, &c, 4);
-            __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), 0);
+            // (2: streamed, not kept in the caches.  64 x 8192 x 512 434 -> 400 us, training step's backward 342 -> 322;
+            // only rows of 203 floats, whose ends share lines, lose: 1024 -> 1079.  Loads gain less and lose more.)
+            __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), 2);
         } else {
             uint16_t w;
             __builtin_memcpy(&w, &c, 2);
@@ -789,11 +794,11 @@ int check_rows(const char *who, int32_t dtype, int64_t n_rows, int64_t total, in
 template <typename T>
 int fill_words(ScanArgs<T> &a, const Layout &l, void *at, hipStream_t s)
 {
-    const int64_t blocks = (l.words + 2047) / 2048;
+    const int64_t blocks = (l.words + 1023) / 1024;
     a.tile_words = (uint64_t *)at;
     a.group_words = a.tile_words + l.tiles * a.dim;
     a.counters = (uint32_t *)(a.tile_words + l.words);
-    fill_words_kernel<<<(unsigned)std::min<int64_t>(blocks, 4096), 256, 0, s>>>(a.tile_words, l.words, l.counters);
+    fill_words_kernel<<<(unsigned)std::min<int64_t>(blocks, 2048), 256, 0, s>>>(a.tile_words, l.words, l.counters);
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
 }
@@ -874,6 +879,7 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
     const Layout l(total, dim, kForwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
+    SCAN_REQUIRE(((uintptr_t)work & 15) == 0, "the work space must be 16-byte aligned");
     int rc = DNATOK_OK;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -903,6 +909,7 @@ extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const
     const Layout l(total, dim, kBackwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
+    SCAN_REQUIRE(((uintptr_t)work & 15) == 0, "the work space must be 16-byte aligned");
     int rc = DNATOK_OK;
     with_type(dtype, [&](auto t) {
         using T = decltype(t);

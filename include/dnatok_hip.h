@@ -433,7 +433,7 @@ int dnatok_normalize_rows(const dnatok_norm_step *steps_h, int32_t n_steps, cons
  * is the state in front of a row's first step, last float[n_rows, dim] (NULL allowed) receives the
  * state behind its last one: h0 again for an empty row.  states (NULL allowed) receives what the
  * backward pass needs, dnatok_gated_scan_states_bytes(); work is the call's own space,
- * dnatok_gated_scan_work_bytes(), at least 8-byte aligned. */
+ * dnatok_gated_scan_work_bytes(), 16-byte aligned. */
 size_t dnatok_gated_scan_states_bytes(int64_t total, int64_t dim);
 size_t dnatok_gated_scan_work_bytes(int64_t total, int64_t dim);
 int dnatok_gated_scan(const void *x, int64_t x_stride, const void *gate, int64_t gate_stride, int32_t dtype,
