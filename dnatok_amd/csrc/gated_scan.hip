@@ -447,9 +447,10 @@ struct Strip {
         if constexpr (V * sizeof(T) == 4) {
             uint32_t w;
             __builtin_memcpy(&w, &c, 4);
-            // (2: streamed, not kept in the caches.  64 x 8192 x 512 434 -> 400 us, training step's backward 342 -> 322;
-            // only rows of 203 floats, whose ends share lines, lose: 1024 -> 1079.  Loads gain less and lose more.)
-            __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), 2);
+            // (2: streamed, not kept in the caches.  64 x 8192 x 512 434 -> 400 us, a training step's backward 342 -> 322.  For
+            // 32 bits between 3 % less and, with rows of 203 floats, whose ends share lines, 5 % more: not used.  Loads
+            // gain less.)
+            __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), sizeof(T) == 2 ? 2 : 0);
         } else {
             uint16_t w;
             __builtin_memcpy(&w, &c, 2);
