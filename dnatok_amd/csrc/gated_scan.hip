@@ -15,15 +15,20 @@
 // the state in front of the tile comes from the tiles before it; a second pass over the registers gives the
 // states.  So every value and gate is read from memory once.  The backward pass does the same from the other side
 // with what flows towards earlier tokens, and runs the states of a wave's tokens again from the one in front of them,
-// which the forward pass has left: 4 bytes for 16 tokens instead of a state for each.
+// which the forward pass has left: 4 bytes for 24 tokens instead of a state for each.
 //
 // The state in front of a tile: a 64-bit word per tile and channel holds the tile's (A, H); the sixteenth tile of a group
 // leaves the same for the group, and then the state at the group's end in its place (marked).  A word says by itself
 // whether it is there (a fill kernel has put a pattern that none has), so nothing has to be ordered by a fence.  A tile
 // takes the nearest group in front whose state is there, and runs that state through the groups and then the tiles
 // between, one after the other.  These are the same steps in the same order wherever the state is found and whoever came
-// first, so the result is the same to the last bit.  (With tiles alone, states one by one, a contig's tiles
-// followed each other every 0.2 us: 2.6 times the time that its bytes take.)
+// first, so the result is the same to the last bit.  (With tiles alone, states one by one, a contig's tiles followed each
+// other every 0.16 us and more: 4,000,000 tokens x 64 in 2517 us, in an early form with groups 855, now 534; its bytes take 323.)
+//
+// Bound by memory and by the waits for states.  Measured, bfloat16: 64 rows of 8,192 tokens x 512 forward 394 us with the fill
+// of the words, 4.09 TB/s (a copy 4.76); a contig of 1,000,003 x 256 409; 256 rows of 1,024 x 512 forward and backward 511.
+// Vector issue is busy 0.36 of the time forward and 0.32 backward.  float32, 300 rows x 203: 1649, 2.6 TB/s of the bytes: a
+// slab's piece of a token, 256 bytes, does not begin on a line.
 #include "lm_common.hpp"
 
 #include <algorithm>
@@ -733,6 +738,7 @@ __global__ __launch_bounds__(256) void copy_states_kernel(const float *from, flo
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from ? from[i] : 0.0f;
 }
 
+// One token of every row: a thread to a channel.  1000 x 1024 float16: 4.9 us (its bytes take 3.0); 1 x 512: 2.2 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(256) void gated_step_kernel(
     const T *__restrict__ x, int64_t x_stride, const T *__restrict__ gate, int64_t gate_stride, const float *state,
@@ -757,7 +763,8 @@ namespace {
 
 constexpr int kSteps = 24;                        // tokens that a wave holds in registers
 // Waves to a tile beside the one that looks for the carry.  On 64 rows of 8,192 tokens x 512 (bfloat16), us forward and
-// backward: 24 tokens x 7 waves 411, 691; x 11 432, 632; 16 tokens x 15 476, 651; x 7 506, 724; 32 tokens x 7 472, 691.
+// backward: 24 tokens x 7 waves 411, 691; x 11 432, 632; 16 tokens x 15 476, 651; x 7 506, 724; 32 tokens x 7 472, 691
+// (all before stores were streamed).
 // Small batches differ by 1 us in 15.
 constexpr int kForwardWaves = 7, kBackwardWaves = 11;
 
@@ -828,6 +835,7 @@ template <typename T, int V>
 int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hipStream_t s)
 {
     a.n_slabs = (uint32_t)((a.dim + 64 * V - 1) / (64 * V));
+    // (a wave's tokens in 32 bits)
     const int64_t widest = std::max({a.x_stride, a.gate_stride, a.dy_stride, a.dim});
     DNATOK_REQUIRE(widest * (int64_t)sizeof(T) * (kSteps + 1) < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: tokens too far apart", who);
     // (eight workgroups of a slab at a time: some find no tile left)
@@ -877,6 +885,7 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(h0, last, n_rows * dim, s);
     SCAN_REQUIRE(x && gate && y, "null buffer");
+    SCAN_REQUIRE(x_stride >= 0 && gate_stride >= 0, "negative stride");
     const Layout l(total, dim, kForwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
@@ -907,6 +916,7 @@ extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const
     hipStream_t s = (hipStream_t)stream;
     if (total == 0) return copy_states(dlast, dh0, n_rows * dim, s);
     SCAN_REQUIRE(x && gate && states && dx && dgate, "null buffer");
+    SCAN_REQUIRE(x_stride >= 0 && gate_stride >= 0 && (!dy || dy_stride >= 0), "negative stride");
     const Layout l(total, dim, kBackwardWaves);
     DNATOK_REQUIRE(l.bytes == 0 || (work && work_bytes >= l.bytes), DNATOK_E_SCRATCH, "%s: the work space needs %zu bytes",
                    who, l.bytes);
@@ -933,6 +943,7 @@ extern "C" int dnatok_gated_step(const void *x, int64_t x_stride, const void *ga
     if (int rc = check_rows(who, dtype, n_rows, n_rows, dim, nullptr)) return rc;
     if (n_rows == 0) return DNATOK_OK;
     SCAN_REQUIRE(x && gate && y && new_state, "null buffer");
+    SCAN_REQUIRE(x_stride >= 0 && gate_stride >= 0, "negative stride");
     const int64_t blocks = (n_rows * dim + 255) / 256;
     DNATOK_REQUIRE(blocks < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
     hipStream_t s = (hipStream_t)stream;

@@ -9,7 +9,8 @@
 // A workgroup takes a slice of one row's tokens: it reads the whole history and counts the ids of its slice in LDS (a
 // word a token: whole numbers, so the order of the additions does not matter), then passes over its logits once.  The
 // logits are requested before the counting.  With a history of some thousand ids this is a chain of a few
-// trips to memory: offsets, ids, the atomics, stores.
+// trips to memory: offsets, ids, the atomics, stores.  256 rows of 32,000 tokens, bfloat16: 16.3 us a call with histories of up to
+// 16,000 ids (2.6 TB/s); replayed in a graph 16.8, and 11.4 with histories of at most two.
 #include "lm_common.hpp"
 
 namespace dnatok {
@@ -37,7 +38,8 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // HISTORY: whether there is one; without it nothing is counted.  (Two workgroups to a CU: with 69 registers for 32-bit logits
-// instead of 64 it is one, 256 rows of 32,000 tokens 22.6 instead of 19.9 us.)
+// instead of 64 it is one, 256 rows of 32,000 tokens 22.6 instead of 19.9 us.  That one, from and to 32 bits, then keeps four
+// registers in scratch memory; no other does.)
 template <typename T, typename OUT, bool HISTORY>
 __global__ __launch_bounds__(kLogitsThreads) __attribute__((amdgpu_waves_per_eu(8))) void logits_kernel(const T *in, OUT *out, LogitsArgs a)
 {
@@ -169,6 +171,7 @@ extern "C" int dnatok_logits_process(const void *logits, int64_t logits_stride, 
     LOGITS_REQUIRE(n_rows >= 0 && vocab >= 0, "bad size");
     if (n_rows == 0 || vocab == 0) return DNATOK_OK;
     LOGITS_REQUIRE(logits && out, "null buffer");
+    LOGITS_REQUIRE(logits_stride >= 0 && out_stride >= 0 && bias_stride >= 0, "negative stride");
     LOGITS_REQUIRE(!history == !history_offsets, "a history needs its offsets and the other way round");
     LOGITS_REQUIRE(!allowed || (n_states > 0 && allowed_stride >= (vocab + 31) / 32), "bad mask size");
     LOGITS_REQUIRE(!state || allowed, "states without masks");

@@ -16,6 +16,10 @@
 // columns of one row); four lanes then exchange words, so that an instruction's 32 columns lie next to each other and
 // in one group.  The waves' sums meet in LDS.  A wave holds its slice of x in registers (w4_kernel); a single row of x lies in
 // LDS, ready to be multiplied (w4_row_kernel).
+//
+// Measured, us a call: one row, 32000 x 4096 bfloat16 in groups of 64 18.2 (3.85 TB/s; a copy 4.76); 16 rows, 8192 x 8192
+// float16 in groups of 32 18.0 (2.25 TB/s, waves waiting 0.66 of their time); 61 rows, 12301 x 2040 15.4; one row, 4096 x 1024
+// 3.9 in the kernel and 8.3 with the host.
 #include "lm_common.hpp"
 
 namespace dnatok {
@@ -455,6 +459,7 @@ extern "C" int dnatok_w4_matvec(const void *x, int64_t x_stride, int32_t dtype, 
     W4_REQUIRE(weight_stride >= (k + 7) / 8, "weight rows overlap");
     if (m == 0 || n == 0) return DNATOK_OK;
     W4_REQUIRE(x && weights && scales && y, "null buffer");
+    W4_REQUIRE(x_stride >= 0 && y_stride >= 0, "negative stride");
     DNATOK_REQUIRE(n < (1ll << 31) && m <= 65535 && weight_stride < (1ll << 22), DNATOK_E_TOO_LARGE,
                    "%s: at most 2^31 outputs of 65535 rows, 2^22 words between rows of weights", who);
     hipStream_t s = (hipStream_t)stream;
