@@ -18,7 +18,7 @@
 // LDS, ready to be multiplied (w4_row_kernel).
 //
 // Measured, us a call: one row, 32000 x 4096 bfloat16 in groups of 64 18.2 (3.85 TB/s; a copy 4.76); 16 rows, 8192 x 8192
-// float16 in groups of 32 18.0 (2.25 TB/s, waves waiting 0.66 of their time); 61 rows, 12301 x 2040 15.4; one row, 4096 x 1024
+// float16 in groups of 32 16.2 (2.5 TB/s); 61 rows, 12301 x 2040 15.1; one row, 4096 x 1024
 // 3.9 in the kernel and 8.3 with the host.
 #include "lm_common.hpp"
 
@@ -51,6 +51,7 @@ struct W4Args {
     int64_t m, n;
     int32_t k, blocks, words, per_group, n_groups;     // columns; 32 of them; words of a row; blocks of a group
     bool x_aligned;                                    // rows of x begin on multiples of 16 bytes
+    bool x_in_lines;                                   // and all at the same place of a 128-byte line
     const float *bias;
     void *y;
     int64_t y_stride;
@@ -317,13 +318,20 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_row_kernel(W4Args<T> a)
     }
 }
 
-template <typename T, typename OUT, int MT, int KB, int TT, int GB>
+// LINES: rows of x begin at the same place of their lines.  Then the sixteen rows that a load takes 16 bytes of meet in one
+// part of the cache's lines, so odd rows fetch the other half of the line, and two loads' results are exchanged.  us without,
+// with: 64 x 32000 x 2048 43.5, 38.0; 64 x 8192 x 8192 46.3, 40.1; 16 x 8192 x 8192 20.2, 19.5; 8 x 8192 x 4096 10.1, 9.6.
+// Rows at other strides spread by themselves, there it loses: 61 x 12301 x 2040 16.8, 18.7; 16 x 8192 x 4128 15.3, 17.3.  (bfloat16,
+// 64 rows, groups of 128 and more: six registers in scratch memory with it, and still 61 x 12301 x 2048 18.9, 17.1.)
+template <typename T, typename OUT, int MT, int KB, int TT, int GB, bool LINES>
 __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
 {
     constexpr bool half = std::is_same<T, _Float16>::value;
     constexpr int SEGS = KB / GB;
     typedef typename Frag<T>::type frag;
-    constexpr int RT = TT * MT <= 4 ? TT : TT * MT <= 8 ? TT / 2 : TT / 4;
+    // (64 KB at most.  The 16 tiles by 4 at a time instead of 8: 61 x 12301 x 2040 16.7, 16.4 us; 64 x 32000 x 2048 44.4, 43.4; all at
+    // once 16.3, 43.2, but 128 KB)
+    constexpr int RT = TT * MT <= 8 ? TT : TT / 2;
     __shared__ f32x4 sums[kW4Waves * RT * MT * 64];
     __shared__ f32x4 x_sums[half ? 1 : kW4Waves][SEGS][MT][4];         // of the slice's segments, four rows of x to an entry
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -336,6 +344,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
     for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[t][i] = zero4;
+    const int odd = LINES ? (r & 1) * 32 : 0;
     const T *x_row[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -351,7 +360,20 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) raw[b][i] = *reinterpret_cast<const u32x4 *>(x_row[i] + (b0 + b) * 32);
+                for (int i = 0; i < MT; ++i)
+                    raw[b][i] = *reinterpret_cast<const u32x4 *>(x_row[i] + (b0 + b) * 32 + (b % 2 ? -odd : odd));
+            if constexpr (LINES) {
+#pragma unroll
+                for (int b = 0; b < KB; b += 2)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t one = raw[b][i][e], two = raw[b + 1][i][e];
+                            raw[b][i][e] = odd ? two : one;
+                            raw[b + 1][i][e] = odd ? one : two;
+                        }
+            }
         } else {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
@@ -396,13 +418,20 @@ using namespace dnatok;
 
 namespace {
 
+template <typename T, typename OUT, int MT, int KB, int TT, bool LINES>
+void launch_w4_x(const W4Args<T> &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)((a.n + 16 * TT - 1) / (16 * TT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
+    if (a.per_group % 4 == 0) w4_kernel<T, OUT, MT, KB, TT, 4, LINES><<<grid, 64 * kW4Waves, 0, s>>>(a);
+    else if (a.per_group % 2 == 0) w4_kernel<T, OUT, MT, KB, TT, 2, LINES><<<grid, 64 * kW4Waves, 0, s>>>(a);
+    else w4_kernel<T, OUT, MT, KB, TT, 1, LINES><<<grid, 64 * kW4Waves, 0, s>>>(a);
+}
+
 template <typename T, typename OUT, int MT, int KB, int TT>
 void launch_w4(const W4Args<T> &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)((a.n + 16 * TT - 1) / (16 * TT)), (unsigned)((a.m + 16 * MT - 1) / (16 * MT)));
-    if (a.per_group % 4 == 0) w4_kernel<T, OUT, MT, KB, TT, 4><<<grid, 64 * kW4Waves, 0, s>>>(a);
-    else if (a.per_group % 2 == 0) w4_kernel<T, OUT, MT, KB, TT, 2><<<grid, 64 * kW4Waves, 0, s>>>(a);
-    else w4_kernel<T, OUT, MT, KB, TT, 1><<<grid, 64 * kW4Waves, 0, s>>>(a);
+    if (a.x_in_lines) launch_w4_x<T, OUT, MT, KB, TT, true>(a, s);
+    else launch_w4_x<T, OUT, MT, KB, TT, false>(a, s);
 }
 
 // Tiles to a workgroup, so that x is fetched less often: as many as leave about a workgroup for each of the 256 CUs.  us for
@@ -433,8 +462,9 @@ void run_w4(const W4Args<T> &a, hipStream_t s)
         else if (a.per_group % 2 == 0) w4_row_kernel<T, OUT, 8, 2><<<grid, 64 * kW4Waves, lds, s>>>(a);
         else w4_row_kernel<T, OUT, 8, 1><<<grid, 64 * kW4Waves, lds, s>>>(a);
     } else if (a.m > 32 && a.n >= 16 * 640) {
-        // weights unpacked once for 64 rows.  61 x 12301 x 2040: 16.2 us, in blocks of 16 rows 20.6; 64 x 32000 x 2048: 45, 63;
-        // with fewer rows of W there are too few workgroups: 64 x 8192 x 8192 58, 46
+        // weights unpacked once for 64 rows.  61 x 12301 x 2040: 16.2 us, in blocks of 16 rows 20.6; 64 x 32000 x 2048: 45, 63
+        // (before rows of x were spread); with fewer rows of W there are too few workgroups: 64 x 8192 x 8192 51, 40; 48 x 10000 x
+        // 4096 29.5, 26.8; 33 x 8192 x 4096 28, 21
         launch_w4<T, OUT, 4, 4, 4>(a, s);
     } else if (a.k > 1024) {
         launch_w4_tiles<T, OUT, 8>(a, s);
@@ -472,6 +502,7 @@ extern "C" int dnatok_w4_matvec(const void *x, int64_t x_stride, int32_t dtype, 
             a.blocks = (int32_t)((k + 31) / 32), a.words = (int32_t)((k + 7) / 8);
             a.per_group = group / 32, a.n_groups = (int32_t)((k + group - 1) / group);
             a.x_aligned = ((uintptr_t)x & 15) == 0 && x_stride % 8 == 0;
+            a.x_in_lines = a.x_aligned && x_stride % 64 == 0;
             a.bias = bias, a.y = y, a.y_stride = y_stride;
             if (y_dtype == DNATOK_F32) run_w4<T, float>(a, s);
             else run_w4<T, T>(a, s);

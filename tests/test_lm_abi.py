@@ -54,6 +54,12 @@ def test_no_flat_accesses_and_no_packed_32_bit_arithmetic(src, tmp_path):
     code = [line.split(";")[0].strip() for line in out.read_text().splitlines()]
     bad = [c for c in code if re.search(r"\bflat_(load|store|atomic)|\bv_pk_(add|mul|fma)_f32", c)]
     assert not bad, f"{len(bad)}, e.g. {bad[:3]}"
-    # registers that one variant, logits from and to 32 bits, keeps in scratch memory by choice
-    spilled = [c for c in code if re.search(r"\bscratch_store_dword\b", c)]
-    assert len(spilled) <= (4 if src == "logits.hip" else 0), spilled[:5]
+    # registers that a kernel keeps in scratch memory by choice: logits from and to 32 bits; bfloat16 products of 64 rows
+    spilled, kernel = {}, None
+    for c in code:
+        if m := re.match(r"^(_Z\w+):", c):
+            kernel = m.group(1)
+        if re.search(r"\bscratch_store_dword", c):
+            spilled[kernel] = spilled.get(kernel, 0) + 4 * {"x2": 2, "x3": 3, "x4": 4}.get(c.split()[0][-2:], 1)
+    most = {"gated_scan.hip": 0, "w4_matvec.hip": 24, "logits.hip": 16}[src]
+    assert max(spilled.values(), default=0) <= most, spilled
