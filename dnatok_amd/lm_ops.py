@@ -213,6 +213,7 @@ class W4Matrix:
         _require(scales, "scales", (self.out_features, groups), scales.dtype, scales.device)
         _require(zeros, "zeros", (self.out_features, groups), torch.uint8, scales.device)
         self.q, self.scales, self.zeros = q, scales, zeros
+        self._group = min(self.group, 1 << 30)         # (32 bits at the C entry; more columns than a matrix has)
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group: int = 128, *, symmetric: bool = True,
@@ -269,7 +270,7 @@ class W4Matrix:
             out = out.unsqueeze(0)
         ys = _require_rows(out, "out", (m, n), out_dtype, device)
         _run("dnatok_w4_matvec", device, x.data_ptr(), xs, _DTYPES[x.dtype], self.q.data_ptr(), self.q.stride(0),
-             self.scales.data_ptr(), _ptr(self.zeros), m, n, k, self.group, _ptr(bias), out.data_ptr(), ys,
+             self.scales.data_ptr(), _ptr(self.zeros), m, n, k, self._group, _ptr(bias), out.data_ptr(), ys,
              _DTYPES[out_dtype])
         return out[0] if squeeze else out
 
