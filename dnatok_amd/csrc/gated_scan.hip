@@ -106,20 +106,21 @@ __device__ __forceinline__ void store_floats(float *p, const float (&v)[V])
     for (int j = 0; j < V; ++j) p[j] = v[j];
 }
 
-// The packed rows along the axis in the order of the recurrence: position p is token p, or token total - 1 - p
-// where rows run backwards; row j in this order ends where row j + 1 starts.
+// The packed axis in the order of the recurrence: position p is token p, or token total - 1 - p where rows run
+// backwards; span j in this order ends where span j + 1 starts.
 template <bool REV>
 struct Axis {
     Rows r;
-    __device__ __forceinline__ int64_t at(int64_t j) const { return REV ? r.total - r.at(r.n - j) : r.at(j); }
-    __device__ __forceinline__ int64_t row(int64_t j) const { return REV ? r.n - 1 - j : j; }
+    __device__ __forceinline__ int64_t count() const { return r.count(); }
+    __device__ __forceinline__ int64_t at(int64_t j) const { return REV ? r.total - r.at(r.count() - j) : r.at(j); }
+    __device__ __forceinline__ int64_t row(int64_t j) const { return r.row(REV ? r.count() - 1 - j : j); }
     __device__ __forceinline__ int64_t token(int64_t p) const { return REV ? r.total - 1 - p : p; }
 
     // The first j with at(j) >= p: every lane of the wave looks at one place of the range that is left.
     __device__ __forceinline__ int64_t first_from(int64_t p, int lane) const
     {
         if (!r.offsets) return (p + r.length - 1) / r.length;
-        int64_t lo = 0, hi = r.n;
+        int64_t lo = 0, hi = r.count();
         while (hi > lo) {
             const int64_t step = (hi - lo + 63) >> 6, i = lo + lane * step;
             const int before = __popcll(__ballot(i < hi && at(i) < p));
@@ -131,10 +132,10 @@ struct Axis {
     }
 };
 
-// Where rows start and end among a wave's positions p0 .. p0 + n: rows (in the axis' order), -1 where there is none.
+// Where spans start and end among a wave's positions p0 .. p0 + n: spans (in the axis' order), -1 where there is none.
 template <int S>
 struct Edges {
-    int32_t start[S + 1], end[S + 1];             // [i]: the row whose first position is p0 + i / whose last is p0 + i - 1
+    int32_t start[S + 1], end[S + 1];             // [i]: the span whose first position is p0 + i / whose last is p0 + i - 1
 };
 
 // Fills `e` and returns the bits of e.start and e.end that are set.  empty(row) is called by the whole wave for each row
@@ -151,20 +152,22 @@ __device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, in
             const int64_t j = base + lane;
             int64_t p = INT64_MAX;
             bool is_empty = false;
-            if (j <= axis.r.n) {
+            if (j <= axis.count()) {
                 const int64_t at = axis.at(j);
                 p = at - p0;
                 if (p >= 0 && p <= n) {
                     if (j > 0 && p > 0 && axis.at(j - 1) < at) e.end[p] = (int32_t)(j - 1);
-                    if (j < axis.r.n) {
+                    if (j < axis.count()) {
                         const bool none = axis.at(j + 1) == at;
                         if (!none && p < n) e.start[p] = (int32_t)j;
                         is_empty = none && (p < n || at == axis.r.total);
                     }
                 }
             }
-            for (uint64_t left = __ballot(is_empty); left; left &= left - 1)
-                empty(axis.row(base + __builtin_ctzll(left)));
+            for (uint64_t left = __ballot(is_empty); left; left &= left - 1) {
+                const int64_t row = axis.row(base + __builtin_ctzll(left));
+                if (row >= 0) empty(row);
+            }
             if (__ballot(p <= n) != ~0ull) break;
         }
     }
@@ -172,6 +175,29 @@ __device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, in
     const int i = lane <= S ? lane : S;
     starts = __ballot(lane <= S && e.start[i] >= 0);
     ends = __ballot(lane <= S && e.end[i] >= 0);
+}
+
+// Whether some of a wave's positions are in no row, and which are not: bit i of `outside`.  Such tokens give zeros: their span
+// starts from zero, and their cells become zeros.
+template <int S, bool REV>
+__device__ __forceinline__ uint64_t outside_rows(const Axis<REV> &axis, int64_t p0, int n)
+{
+    if (!axis.r.offsets) return 0;
+    const int64_t lo = axis.at(1) - p0, hi = axis.at(axis.count() - 1) - p0;
+    const uint64_t all = (1ull << n) - 1, front = lo >= n ? all : lo > 0 ? (1ull << lo) - 1 : 0;
+    const uint64_t back = hi >= n ? 0 : hi > 0 ? all & ~((1ull << hi) - 1) : all;
+    return front | back;
+}
+template <typename T, int V, int S>
+__device__ __forceinline__ void clear_cells(Cell<T, V> (&c)[S], uint64_t which)
+{
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        typename std::conditional<V * sizeof(T) == 4, uint32_t, uint16_t>::type w;
+        __builtin_memcpy(&w, &c[i], sizeof(w));
+        w = which >> i & 1 ? 0 : w;
+        __builtin_memcpy(&c[i], &w, sizeof(w));
+    }
 }
 
 // A piece of the axis: c -> (1 - b) c + h in every channel.  (b and not 1 - b is multiplied up: a rounded product of
@@ -494,17 +520,16 @@ __device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanAr
 {
     float carry[V];
     load_floats<V>(carry, nullptr);
-    if (nth > 0 && axis.at(axis.first_from(edge, lane)) != edge) {
+    if (nth > 0 && axis.at(axis.first_from(edge, lane)) != edge)
         find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
-        if (nth % kGroup == kGroup - 1) {
-            const Piece<V> p = own();
-            if (p.b[0] != kReset) {
-                float end[V];
+    if (nth > 0 && nth % kGroup == kGroup - 1) {                       // (whatever the offsets say: later tiles wait for it)
+        const Piece<V> p = own();
+        if (p.b[0] != kReset) {
+            float end[V];
 #pragma unroll
-                for (int v = 0; v < V; ++v) end[v] = carry[v];
-                p.through(end);
-                put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, end);
-            }
+            for (int v = 0; v < V; ++v) end[v] = carry[v];
+            p.through(end);
+            put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, end);
         }
     }
 #pragma unroll
@@ -556,8 +581,15 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
         load_floats<V>(h, a.h0 ? a.h0 + row * a.dim + c : nullptr);
         if (a.last) store_floats<V>(a.last + row * a.dim + c, h);
     });
+    if (const uint64_t outside = outside_rows<S, REV>(axis, span.p0, n)) {
+        clear_cells<T, V, S>(x, outside);
+        clear_cells<T, V, S>(g, outside);
+    }
     const bool plain = n == S && (starts | ends) == 0;                 // no row starts or ends here: no step has to look
-    const auto initial = [&](int i) { return a.h0 ? a.h0 + axis.row(one_row(edges.start[i])) * a.dim + c : nullptr; };
+    const auto initial = [&](int i) {
+        const int64_t row = axis.row(one_row(edges.start[i]));
+        return a.h0 && row >= 0 ? a.h0 + row * a.dim + c : nullptr;
+    };
 
     float k[S][V];
     Piece<V> own;
@@ -602,8 +634,10 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = next_state(k[i][v], h[v], to_float(x[i].v[v]));
             ys.store(i, h);
-            if (with_edges && (ends >> (i + 1) & 1) && a.last)
-                store_floats<V>(a.last + axis.row(one_row(edges.end[i + 1])) * a.dim + c, h);
+            if (with_edges && (ends >> (i + 1) & 1) && a.last) {
+                const int64_t row = axis.row(one_row(edges.end[i + 1]));
+                if (row >= 0) store_floats<V>(a.last + row * a.dim + c, h);
+            }
         }
     };
     if (plain) second_pass(std::false_type{});
@@ -654,10 +688,19 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
         load_floats<V>(d, a.dlast ? a.dlast + row * a.dim + c : nullptr);
         if (a.dh0) store_floats<V>(a.dh0 + row * a.dim + c, d);
     });
+    if (const uint64_t outside = outside_rows<S, REV>(axis, span.p0, n)) {
+        clear_cells<T, V, S>(x, outside);
+        clear_cells<T, V, S>(g, outside);
+        clear_cells<T, V, S>(dy, outside);
+    }
     const bool plain = n == S && (starts | ends) == 0;
-    const auto initial = [&](int i) { return a.h0 ? a.h0 + axis.row(one_row(edges.start[i])) * a.dim + c : nullptr; };
+    const auto initial = [&](int i) {
+        const int64_t row = axis.row(one_row(edges.start[i]));
+        return a.h0 && row >= 0 ? a.h0 + row * a.dim + c : nullptr;
+    };
     const auto final_grad = [&](int i) {
-        return a.dlast ? a.dlast + axis.row(one_row(edges.end[i + 1])) * a.dim + c : nullptr;
+        const int64_t row = axis.row(one_row(edges.end[i + 1]));
+        return a.dlast && row >= 0 ? a.dlast + row * a.dim + c : nullptr;
     };
 
     float k[S][V];
@@ -724,8 +767,10 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
             }
             dxs.store(i, dx);
             dgs.store(i, dg);
-            if (with_edges && (starts >> i & 1) && a.dh0)
-                store_floats<V>(a.dh0 + axis.row(one_row(edges.start[i])) * a.dim + c, carry);
+            if (with_edges && (starts >> i & 1) && a.dh0) {
+                const int64_t row = axis.row(one_row(edges.start[i]));
+                if (row >= 0) store_floats<V>(a.dh0 + row * a.dim + c, carry);
+            }
         }
     };
     if (plain) second_pass(std::false_type{});
@@ -795,7 +840,8 @@ int check_rows(const char *who, int32_t dtype, int64_t n_rows, int64_t total, in
     SCAN_REQUIRE(dtype == DNATOK_F32 || dtype == DNATOK_BF16 || dtype == DNATOK_F16, "unknown element type");
     SCAN_REQUIRE(n_rows >= 0 && total >= 0 && dim > 0 && (n_rows > 0 || total == 0), "bad size");
     SCAN_REQUIRE(offsets || n_rows == 0 || total % n_rows == 0, "rows without offsets must be of one length");
-    DNATOK_REQUIRE(n_rows < (1ll << 31) && dim < (1ll << 30), DNATOK_E_TOO_LARGE, "%s: at most 2^31 rows of 2^30 channels", who);
+    DNATOK_REQUIRE(n_rows < (1ll << 31) - 2 && dim < (1ll << 30), DNATOK_E_TOO_LARGE, "%s: fewer than 2^31 - 2 rows of 2^30 channels",
+                   who);                                               // (two more spans than rows)
     return DNATOK_OK;
 }
 

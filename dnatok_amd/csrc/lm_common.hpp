@@ -21,11 +21,22 @@ inline void with_type(int32_t dtype, Fn fn)
     else fn(_Float16{});
 }
 
-// Row b of a packed batch is the tokens at(b) .. at(b + 1); without offsets all rows have one length.
+// The packed axis as spans b = 0 .. count() - 1, tokens at(b) .. at(b + 1).  Without offsets these are the rows, all of one length.
+// With offsets the tokens in front of the first row and those behind the last one, which are in no row (the buffer may
+// be longer than its rows), are spans too, mostly empty: so a span starts at the axis' first token and one ends at its last,
+// whatever the offsets are.  row(b): the span's row, or -1.
 struct Rows {
     const int64_t *offsets;
     int64_t n, total, length;
-    __device__ __forceinline__ int64_t at(int64_t b) const { return offsets ? offsets[b] : b * length; }
+    __device__ __forceinline__ int64_t count() const { return offsets ? n + 2 : n; }
+    __device__ __forceinline__ int64_t row(int64_t b) const { return !offsets ? b : b > 0 && b <= n ? b - 1 : -1; }
+    __device__ __forceinline__ int64_t at(int64_t b) const
+    {
+        if (!offsets) return b * length;
+        if (b == 0 || b > n + 1) return b == 0 ? 0 : total;
+        const int64_t v = offsets[b - 1];
+        return v < 0 ? 0 : v < total ? v : total;
+    }
 };
 
 // The gate of the recurrence: k = 1 - f = 1 / (1 + exp(g)), to full relative precision however small (1 - f would be what

@@ -126,7 +126,8 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, offsets: Optional[torch.Tens
     step, float32 [B, D].
 
     ``x`` and ``gate`` are packed rows [total, D] with ``offsets`` int64 [B + 1] as the encoders write
-    them (rows may be empty), or dense rows [B, T, D] without offsets (copied where they do not lie like packed
+    them (ascending; rows may be empty, and there may be room behind the last one, as
+    :func:`dnatok_amd.encoders.pack_ragged` leaves it: tokens in no row give zeros, also as gradients), or dense rows [B, T, D] without offsets (copied where they do not lie like packed
     ones); float32, bfloat16 or float16, the elements of
     a token next to each other (halves of one projection's output will do).  ``h0`` float32 [B, D] is the
     state in front of each row, zero if not given; ``reverse`` runs rows from their last token to their

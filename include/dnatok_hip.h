@@ -428,7 +428,8 @@ int dnatok_normalize_rows(const dnatok_norm_step *steps_h, int32_t n_steps, cons
 /* Gated linear recurrence over packed rows, in every channel:
  *   f_t = sigmoid(gate_t),  h_t = f_t h_(t-1) + (1 - f_t) x_t,  y_t = h_t
  * x, gate and y are [total, dim] of `dtype`; y's rows lie back to back.  Row b is the tokens offsets[b] .. offsets[b+1]
- * (offsets[0] = 0, offsets[n_rows] = total); without offsets the n_rows rows have one length.
+ * (ascending; tokens in front of the first row and behind the last one, up to total, are in no row: their y and their
+ * gradients are zeros, whatever x, gate and dy hold there); without offsets the n_rows rows have one length.
  * reverse = 1 runs every row from its last token to its first.  h0 float[n_rows, dim] (NULL: zeros)
  * is the state in front of a row's first step, last float[n_rows, dim] (NULL allowed) receives the
  * state behind its last one: h0 again for an empty row.  states (NULL allowed) receives what the
