@@ -263,9 +263,11 @@ __device__ __forceinline__ float word_b(uint64_t w) { return __uint_as_float((ui
 __device__ __forceinline__ float word_h(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
 __device__ __forceinline__ bool is_there(uint64_t w) { return (uint32_t)w != 0xFFFFFFFFu; }
 
-// One wave: what reaches the tile that is the `at`-th in order from the tiles in front of it.  own() waits for what the tile
-// itself does and returns it; where the tile is the last of its group it is needed for the group's word, which is left
-// here.  NaN should the words never come.
+// One wave: what reaches the tile that is the `at`-th in order, at > 0, from the tiles in front of it.  own() waits for what the
+// tile itself does and returns it; where the tile is the last of its group the group's word and then its state are left here
+// (unless the tile starts a row: then it has left the state).  The state of a group without a row's start is the
+// one in front of it run through the group's piece, as a tile does that finds only the piece: one rounding, whichever it
+// finds.  NaN should the words never come.
 template <int V, typename Own>
 __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], const uint64_t *tile_words,
                                            uint64_t *group_words, int64_t dim, uint32_t at, uint32_t slab0, uint32_t c,
@@ -310,11 +312,14 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         ok = __all(ok) || looks <= 0;
     }
     const bool reset = need > 0 && word_b(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
-    if (pos == kGroup - 1 && !reset) {
-        const Piece<V> last = own();
-        if (last.b[0] != kReset) {                                     // (otherwise the tile has left the group's state)
-            Piece<V> sum;
-            sum.clear();
+    Piece<V> last, sum;
+    last.clear();
+    sum.clear();
+    bool leave_state = false;                                          // (otherwise the tile has left it, or another will)
+    if (pos == kGroup - 1) {
+        last = own();
+        leave_state = last.b[0] != kReset;
+        if (leave_state && !reset) {
 #pragma unroll 3
             for (int e = need - 1; e >= 0; --e) {
                 Piece<V> p;
@@ -356,13 +361,26 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         if (!ok) nearest = -1;
         if (looks <= 0) break;
     }
+    if (looks <= 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = __builtin_nanf("");
+    float end[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) end[v] = carry[v];
+    if (leave_state && !reset) {
+        sum.through(end);
+        put_states<V>(groups + c, end);
+    }
 #pragma unroll 4
     for (int e = need - 1; e >= 0; --e)
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = carry_through(word_b(window[e][v][lane]), word_h(window[e][v][lane]), carry[v]);
-    if (looks <= 0)
+    if (leave_state && reset) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = __builtin_nanf("");
+        for (int v = 0; v < V; ++v) end[v] = carry[v];
+        last.through(end);
+        put_states<V>(groups + c, end);
+    }
 }
 
 // The pieces of a tile's waves, in LDS (array by array: lanes read neighbouring words).
@@ -513,25 +531,15 @@ __device__ __forceinline__ uint32_t take_tile(ScanShared<S, W, V> &sh, uint32_t 
 }
 
 // The last wave of a workgroup looks for the carry while the others, W, compute; `nth`: the tile's place in the order of the
-// launch.  edge: position at which the carry comes in; nothing comes in where a row starts (ends) there.
-template <int S, int W, int V, bool REV, typename T, typename Own>
-__device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanArgs<T> &a, const Axis<REV> &axis,
-                                           uint32_t nth, uint32_t slab0, uint32_t c, int64_t edge, Own own, int lane)
+// launch.  (Also where a row starts, or ends, at the tile's edge and nothing comes in: so it is no matter of the offsets whether a
+// group's word is left.)
+template <int S, int W, int V, typename T, typename Own>
+__device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanArgs<T> &a, uint32_t nth, uint32_t slab0,
+                                           uint32_t c, Own own, int lane)
 {
     float carry[V];
     load_floats<V>(carry, nullptr);
-    if (nth > 0 && axis.at(axis.first_from(edge, lane)) != edge)
-        find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
-    if (nth > 0 && nth % kGroup == kGroup - 1) {                       // (whatever the offsets say: later tiles wait for it)
-        const Piece<V> p = own();
-        if (p.b[0] != kReset) {
-            float end[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) end[v] = carry[v];
-            p.through(end);
-            put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, end);
-        }
-    }
+    if (nth > 0) find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.carry[v][lane] = carry[v];
     __syncthreads();
@@ -562,7 +570,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
             sh.wait_for_all();
             return sh.parts.front(W, lane);
         };
-        carry_wave<S, W, V>(sh, a, axis, tile, span.slab0, c, (int64_t)tile * (W * S), own, lane);
+        carry_wave<S, W, V>(sh, a, tile, span.slab0, c, own, lane);
         return;
     }
     const int n = span.n;
@@ -661,7 +669,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
             sh.wait_for_all();
             return sh.parts.behind(0, lane);
         };
-        carry_wave<S, W, V>(sh, a, axis, nth, span.slab0, c, ((int64_t)tile + 1) * (W * S), own, lane);
+        carry_wave<S, W, V>(sh, a, nth, span.slab0, c, own, lane);
         return;
     }
     const int n = span.n;
