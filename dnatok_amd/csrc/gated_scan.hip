@@ -36,7 +36,6 @@
 namespace dnatok {
 
 constexpr uint64_t kNoWord = ~0ull;
-constexpr int kLooks = 1 << 20;
 constexpr int kGroup = 16;                        // tiles of a group, and groups that a tile looks back
 constexpr int kCounterStride = 32;                // (a 128-byte line to a counter)
 
@@ -267,7 +266,10 @@ __device__ __forceinline__ bool is_there(uint64_t w) { return (uint32_t)w != 0xF
 // tile itself does and returns it; where the tile is the last of its group the group's word and then its state are left here
 // (unless the tile starts a row: then it has left the state).  The state of a group without a row's start is the
 // one in front of it run through the group's piece, as a tile does that finds only the piece: one rounding, whichever it
-// finds.  NaN should the words never come.
+// finds.
+// Every wait ends.  Tiles are taken in order by workgroups that run, and each leaves its word, and its group's piece, before it
+// waits for a state; the first tile of all has its word as a reset, whatever the offsets are, so the first group's state needs
+// no other group's, and each further one only those in front of it.
 template <int V, typename Own>
 __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], const uint64_t *tile_words,
                                            uint64_t *group_words, int64_t dim, uint32_t at, uint32_t slab0, uint32_t c,
@@ -281,7 +283,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
     const int back = (lane & (kGroup - 1)) + 1;
     const bool wanted = group ? lane < 2 * kGroup && back <= n_groups : back <= pos;
     const uint64_t *const mine = (group ? groups : tiles) - back * dim + slab0;
-    int looks = kLooks, need, nearest;                                 // tiles that count; the nearest group with a state, or -1
+    int need, nearest;                                                 // tiles that count; the nearest group with a state, or -1
     const auto look = [&] {
         const uint64_t w = wanted ? get_word(mine) : kNoWord;
         const uint64_t there = __ballot(is_there(w)), resets = __ballot(word_b(w) == kReset);
@@ -293,7 +295,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
     };
     load_floats<V>(carry, nullptr);
     for (bool ok = false; !ok;) {
-        while (!look() && --looks > 0) __builtin_amdgcn_s_sleep(1);
+        while (!look()) __builtin_amdgcn_s_sleep(1);
         ok = true;
         for (int e0 = 0; e0 < need; e0 += 8) {
             uint64_t q[8][V];
@@ -309,7 +311,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
                     if (e0 + k < kGroup) window[e0 + k][v][lane] = q[k][v];
                 }
         }
-        ok = __all(ok) || looks <= 0;
+        ok = __all(ok);
     }
     const bool reset = need > 0 && word_b(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
     Piece<V> last, sum;
@@ -335,7 +337,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         }
     }
     for (bool ok = reset; !ok;) {
-        while (nearest < 0 && --looks > 0) {
+        while (nearest < 0) {
             __builtin_amdgcn_s_sleep(1);
             look();
         }
@@ -359,11 +361,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         }
         ok = __all(ok);
         if (!ok) nearest = -1;
-        if (looks <= 0) break;
     }
-    if (looks <= 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = __builtin_nanf("");
     float end[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) end[v] = carry[v];
@@ -618,7 +616,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
     if (plain) first_pass(std::false_type{});
     else first_pass(std::true_type{});
     keep_raw<T, V, S>(x);
-    own.close(starts != 0);
+    own.close(starts != 0 || span.p0 == 0);                            // (the axis' first token starts a span, were the offsets wrong)
     sh.parts.put(wave, lane, own);
     if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, tile, c, sh.parts.front(W, lane));
     Piece<V> front;                                                    // the tile's waves in front of this one
@@ -731,7 +729,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
     else first_pass(std::true_type{});
     keep_raw<T, V, S>(x);
     keep_raw<T, V, S>(dy);
-    own.close(ends != 0);
+    own.close(ends != 0 || (n > 0 && span.p0 + n == a.rows.total));    // (the axis' last token ends a span)
     sh.parts.put(wave, lane, own);
     if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, nth, c, sh.parts.behind(0, lane));
     Piece<V> behind;                                                   // the tile's waves behind this one
