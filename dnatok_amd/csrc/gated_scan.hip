@@ -115,11 +115,13 @@ struct Axis {
     __device__ __forceinline__ int64_t row(int64_t j) const { return r.row(REV ? r.count() - 1 - j : j); }
     __device__ __forceinline__ int64_t token(int64_t p) const { return REV ? r.total - 1 - p : p; }
 
-    // The first j with at(j) >= p: every lane of the wave looks at one place of the range that is left.
+    // The first j with at(j) >= p, or with offsets the last but one if there is none before: every lane of the wave looks at one
+    // place of the range that is left.
     __device__ __forceinline__ int64_t first_from(int64_t p, int lane) const
     {
         if (!r.offsets) return (p + r.length - 1) / r.length;
-        int64_t lo = 0, hi = r.count();
+        if (p <= 0) return 0;
+        int64_t lo = 1, hi = r.n + 1;                                  // (a place to each row's start, and one round for 64 rows)
         while (hi > lo) {
             const int64_t step = (hi - lo + 63) >> 6, i = lo + lane * step;
             const int before = __popcll(__ballot(i < hi && at(i) < p));
@@ -137,17 +139,20 @@ struct Edges {
     int32_t start[S + 1], end[S + 1];             // [i]: the span whose first position is p0 + i / whose last is p0 + i - 1
 };
 
-// Fills `e` and returns the bits of e.start and e.end that are set.  empty(row) is called by the whole wave for each row
-// without tokens that lies here.
+// Fills `e` and returns the bits of e.start and e.end that are set, and whether the first or the last span may be here.  empty(row)
+// is called by the whole wave for each row without tokens that lies here.
 template <int S, bool REV, typename Fn>
-__device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, int n, int lane, Edges<S> &e,
+__device__ __forceinline__ bool find_edges(const Axis<REV> &axis, int64_t p0, int n, int lane, Edges<S> &e,
                                            uint64_t &starts, uint64_t &ends, Fn empty)
 {
     static_assert(S + 1 <= 64, "a lane to a position");
     if (lane <= S) e.start[lane] = e.end[lane] = -1;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    bool rim = false;
     if (n > 0) {
-        for (int64_t base = axis.first_from(p0, lane);; base += 64) {
+        const int64_t first = axis.first_from(p0, lane);
+        rim = first <= 1;
+        for (int64_t base = first;; base += 64) {
             const int64_t j = base + lane;
             int64_t p = INT64_MAX;
             bool is_empty = false;
@@ -167,6 +172,7 @@ __device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, in
                 const int64_t row = axis.row(base + __builtin_ctzll(left));
                 if (row >= 0) empty(row);
             }
+            rim = rim || __ballot(j + 1 >= axis.count() && p <= n);
             if (__ballot(p <= n) != ~0ull) break;
         }
     }
@@ -174,6 +180,7 @@ __device__ __forceinline__ void find_edges(const Axis<REV> &axis, int64_t p0, in
     const int i = lane <= S ? lane : S;
     starts = __ballot(lane <= S && e.start[i] >= 0);
     ends = __ballot(lane <= S && e.end[i] >= 0);
+    return rim;
 }
 
 // Whether some of a wave's positions are in no row, and which are not: bit i of `outside`.  Such tokens give zeros: their span
@@ -264,14 +271,15 @@ __device__ __forceinline__ bool is_there(uint64_t w) { return (uint32_t)w != 0xF
 
 // One wave: what reaches the tile that is the `at`-th in order, at > 0, from the tiles in front of it.  own() waits for what the
 // tile itself does and returns it; where the tile is the last of its group the group's word and then its state are left here
-// (unless the tile starts a row: then it has left the state).  The state of a group without a row's start is the
+// (unless the tile starts a row: then it has left the state), or true is returned: a row starts in the group, and its state is what
+// the tile makes of the carry.  The state of a group without a row's start is the
 // one in front of it run through the group's piece, as a tile does that finds only the piece: one rounding, whichever it
 // finds.
 // Every wait ends.  Tiles are taken in order by workgroups that run, and each leaves its word, and its group's piece, before it
 // waits for a state; the first tile of all has its word as a reset, whatever the offsets are, so the first group's state needs
 // no other group's, and each further one only those in front of it.
 template <int V, typename Own>
-__device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], const uint64_t *tile_words,
+__device__ __forceinline__ bool find_carry(uint64_t (&window)[kGroup][V][64], const uint64_t *tile_words,
                                            uint64_t *group_words, int64_t dim, uint32_t at, uint32_t slab0, uint32_t c,
                                            Own own, int lane, float (&carry)[V])
 {
@@ -314,14 +322,14 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         ok = __all(ok);
     }
     const bool reset = need > 0 && word_b(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
-    Piece<V> last, sum;
-    last.clear();
+    const bool group_end = pos == kGroup - 1;
+    Piece<V> sum;
     sum.clear();
-    bool leave_state = false;                                          // (otherwise the tile has left it, or another will)
-    if (pos == kGroup - 1) {
-        last = own();
+    bool leave_state = false;                                          // (otherwise the tile has left it)
+    if (group_end && !reset) {
+        const Piece<V> last = own();
         leave_state = last.b[0] != kReset;
-        if (leave_state && !reset) {
+        if (leave_state) {
 #pragma unroll 3
             for (int e = need - 1; e >= 0; --e) {
                 Piece<V> p;
@@ -362,10 +370,10 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
         ok = __all(ok);
         if (!ok) nearest = -1;
     }
-    float end[V];
+    if (leave_state) {
+        float end[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) end[v] = carry[v];
-    if (leave_state && !reset) {
+        for (int v = 0; v < V; ++v) end[v] = carry[v];
         sum.through(end);
         put_states<V>(groups + c, end);
     }
@@ -373,12 +381,7 @@ __device__ __forceinline__ void find_carry(uint64_t (&window)[kGroup][V][64], co
     for (int e = need - 1; e >= 0; --e)
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = carry_through(word_b(window[e][v][lane]), word_h(window[e][v][lane]), carry[v]);
-    if (leave_state && reset) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) end[v] = carry[v];
-        last.through(end);
-        put_states<V>(groups + c, end);
-    }
+    return group_end && reset;
 }
 
 // The pieces of a tile's waves, in LDS (array by array: lanes read neighbouring words).
@@ -537,10 +540,17 @@ __device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanAr
 {
     float carry[V];
     load_floats<V>(carry, nullptr);
-    if (nth > 0) find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
+    const bool leave_state = nth > 0 && find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.carry[v][lane] = carry[v];
     __syncthreads();
+    if (leave_state) {
+        const Piece<V> p = own();
+        if (p.b[0] != kReset) {                                        // (otherwise the tile has left it)
+            p.through(carry);
+            put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, carry);
+        }
+    }
 }
 
 // The word of a tile, and that of its group if the tile is the last of it and a row starts (ends) inside: then the state
@@ -582,12 +592,12 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
     }
     Edges<S> &edges = sh.edges[wave];
     uint64_t starts, ends;
-    find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
+    const bool rim = find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
         float h[V];
         load_floats<V>(h, a.h0 ? a.h0 + row * a.dim + c : nullptr);
         if (a.last) store_floats<V>(a.last + row * a.dim + c, h);
     });
-    if (const uint64_t outside = outside_rows<S, REV>(axis, span.p0, n)) {
+    if (const uint64_t outside = rim ? outside_rows<S, REV>(axis, span.p0, n) : 0) {
         clear_cells<T, V, S>(x, outside);
         clear_cells<T, V, S>(g, outside);
     }
@@ -689,12 +699,12 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
     }
     Edges<S> &edges = sh.edges[wave];
     uint64_t starts, ends;
-    find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
+    const bool rim = find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
         float d[V];
         load_floats<V>(d, a.dlast ? a.dlast + row * a.dim + c : nullptr);
         if (a.dh0) store_floats<V>(a.dh0 + row * a.dim + c, d);
     });
-    if (const uint64_t outside = outside_rows<S, REV>(axis, span.p0, n)) {
+    if (const uint64_t outside = rim ? outside_rows<S, REV>(axis, span.p0, n) : 0) {
         clear_cells<T, V, S>(x, outside);
         clear_cells<T, V, S>(g, outside);
         clear_cells<T, V, S>(dy, outside);

@@ -33,9 +33,8 @@ struct Rows {
     __device__ __forceinline__ int64_t at(int64_t b) const
     {
         if (!offsets) return b * length;
-        if (b == 0 || b > n + 1) return b == 0 ? 0 : total;
-        const int64_t v = offsets[b - 1];
-        return v < 0 ? 0 : v < total ? v : total;
+        const int64_t v = offsets[b <= 0 ? 0 : b > n ? n : b - 1];
+        return b <= 0 ? 0 : b > n + 1 ? total : v;
     }
 };
 
