@@ -73,30 +73,59 @@ struct ScanArgs {
 // V channels of one token as they lie in memory.
 template <typename T, int V> struct Cell { T v[V]; };
 
-// The cells go on as they lie in memory: without this the compiler keeps their 32-bit forms, twice the registers.
-template <typename T, int V, int S>
-__device__ __forceinline__ void keep_raw(Cell<T, V> (&c)[S])
+// A number that was there before, and what was found out about it is not kept with it.
+__device__ __forceinline__ float once_more(float m)
+{
+    asm volatile("" : "+v"(m));
+    return m;
+}
+
+// step(i, look) for the S tokens of a wave, forwards or backwards, four at a time: look is a true_type where one of the four has a bit in
+// `looks`.  (The compiler keeps room for both kinds of a part at once, so parts are short.)
+constexpr int kPart = 4;
+template <int S, typename Fn>
+__device__ __forceinline__ void by_parts(uint64_t looks, Fn step)
+{
+    static_assert(S % kPart == 0, "whole parts");
+#pragma unroll
+    for (int from = 0; from < S; from += kPart) {
+        if (looks >> from & ((1 << kPart) - 1)) {
+#pragma unroll
+            for (int i = from; i < from + kPart; ++i) step(i, std::true_type{});
+        } else {
+#pragma unroll
+            for (int i = from; i < from + kPart; ++i) step(i, std::false_type{});
+        }
+    }
+}
+template <int S, typename Fn>
+__device__ __forceinline__ void by_parts_back(uint64_t looks, Fn step)
 {
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-        if constexpr (V * sizeof(T) == 4) {
-            uint32_t w;
-            __builtin_memcpy(&w, &c[i], 4);
-            asm volatile("" : "+v"(w));
-            __builtin_memcpy(&c[i], &w, 4);
+    for (int from = S - kPart; from >= 0; from -= kPart) {
+        if (looks >> from & ((1 << kPart) - 1)) {
+#pragma unroll
+            for (int i = from + kPart - 1; i >= from; --i) step(i, std::true_type{});
         } else {
-            uint16_t w;
-            __builtin_memcpy(&w, &c[i], 2);
-            asm volatile("" : "+v"(w));
-            __builtin_memcpy(&c[i], &w, 2);
+#pragma unroll
+            for (int i = from + kPart - 1; i >= from; --i) step(i, std::false_type{});
         }
     }
 }
 template <int V>
-__device__ __forceinline__ void load_floats(float (&to)[V], const float *p)       // (zeros without an array)
+__device__ __forceinline__ void clear_floats(float (&to)[V])
 {
 #pragma unroll
-    for (int v = 0; v < V; ++v) to[v] = p ? p[v] : 0.0f;
+    for (int v = 0; v < V; ++v) to[v] = 0.0f;
+}
+// Channels from c on of one row of an array [rows, dim]; zeros without an array, or where there is no row (-1).
+template <int V>
+__device__ __forceinline__ void load_row(float (&to)[V], const float *array, int64_t row, int64_t dim, uint32_t c)
+{
+    clear_floats<V>(to);
+    if (array && row >= 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) to[v] = array[row * dim + c + v];
 }
 template <int V>
 __device__ __forceinline__ void store_floats(float *p, const float (&v)[V])
@@ -206,49 +235,71 @@ __device__ __forceinline__ void clear_cells(Cell<T, V> (&c)[S], uint64_t which)
     }
 }
 
-// A piece of the axis: c -> (1 - b) c + h in every channel.  (b and not 1 - b is multiplied up: a rounded product of
-// factors next to 1 would lose what slow channels forget, always in the same direction where the gate is constant.)
-// Where a row begins inside (or ends, for what flows backwards) the piece is a reset: h comes out, and nothing of what
-// comes in, be it infinite.
-constexpr float kReset = 2.0f;
-
-__device__ __forceinline__ float carry_through(float b, float h, float c) { return b == kReset ? h : fmaf(-b, c, c) + h; }
-
+// What a run of tokens makes of the state in front of it, c -> a c + h, with b = 1 - a beside a: a rounded product of factors next to 1
+// would lose what slow channels forget, always in the same direction where the gate is constant, and what is left of 1 - b would
+// lose a small a.
 template <int V>
-struct Piece {
-    float b[V], h[V];
+struct Run {
+    float a[V], b[V], h[V];
     __device__ __forceinline__ void clear()
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) b[v] = h[v] = 0.0f;
+        for (int v = 0; v < V; ++v) a[v] = 1.0f, b[v] = h[v] = 0.0f;
     }
-    __device__ __forceinline__ void factor(int v, float k) { b[v] = next_state(k, b[v], 1.0f); }
-    __device__ __forceinline__ void close(bool edge)
+    __device__ __forceinline__ void factor(int v, const Gate &g)
+    {
+        b[v] = fmaf(g.k, a[v], b[v]);
+        a[v] *= g.f;
+    }
+    __device__ __forceinline__ void then(const Run &r)
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) b[v] = edge ? kReset : b[v];
-    }
-    __device__ __forceinline__ void through(float (&c)[V]) const
-    {
-#pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = carry_through(b[v], h[v], c[v]);
-    }
-    __device__ __forceinline__ void then(const Piece &p)
-    {
-        p.through(h);
-#pragma unroll
-        for (int v = 0; v < V; ++v) b[v] = b[v] == kReset || p.b[v] == kReset ? kReset : next_state(p.b[v], b[v], 1.0f);
+        for (int v = 0; v < V; ++v) {
+            h[v] = fmaf(r.a[v], h[v], r.h[v]);
+            b[v] = fmaf(a[v], r.b[v], b[v]);
+            a[v] *= r.a[v];
+        }
     }
 };
 
-// A word of the tiles: low b, high h.  (b is never the NaN of an absent word.)
+// The same of a tile or a group in a word: of a and b the one that is at most 1/2, t >= 0 is b, t < 0 (-0 among them) is -a.
+// Where a row begins inside (or ends, for what flows backwards) it is a reset: h comes out, and nothing of what comes in,
+// be it infinite.
+constexpr float kReset = 2.0f;
+
+__device__ __forceinline__ bool is_b(float t) { return !__builtin_signbitf(t); }
+__device__ __forceinline__ float carry_through(float t, float h, float c)
+{
+    return t == kReset ? h : fmaf(-t, c, is_b(t) ? c : 0.0f) + h;
+}
+
+template <int V>
+struct Piece {
+    float t[V], h[V];
+    __device__ __forceinline__ Piece(const Run<V> &r, bool reset)
+    {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            t[v] = reset ? kReset : r.b[v] <= 0.5f ? r.b[v] : -r.a[v];
+            h[v] = r.h[v];
+        }
+    }
+    __device__ __forceinline__ bool is_reset() const { return t[0] == kReset; }        // (of all channels at once)
+    __device__ __forceinline__ void through(float (&c)[V]) const
+    {
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = carry_through(t[v], h[v], c[v]);
+    }
+};
+
+// A word of the tiles: low t, high h.  (t is never the NaN of an absent word.)
 template <int V>
 __device__ __forceinline__ void put_words(uint64_t *to, const Piece<V> &p)
 {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const float b = p.b[v] == p.b[v] ? p.b[v] : __builtin_nanf("");
-        __hip_atomic_store(to + v, (uint64_t)__float_as_uint(p.h[v]) << 32 | __float_as_uint(b), __ATOMIC_RELAXED,
+        const float t = p.t[v] == p.t[v] ? p.t[v] : __builtin_nanf("");
+        __hip_atomic_store(to + v, (uint64_t)__float_as_uint(p.h[v]) << 32 | __float_as_uint(t), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     }
 }
@@ -265,9 +316,32 @@ __device__ __forceinline__ uint64_t get_word(const uint64_t *p)
 {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float word_b(uint64_t w) { return __uint_as_float((uint32_t)w); }
+__device__ __forceinline__ float word_t(uint64_t w) { return __uint_as_float((uint32_t)w); }
 __device__ __forceinline__ float word_h(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
+// The word of a tile that is no reset, as a run again.
+template <int V>
+__device__ __forceinline__ Run<V> run_of(const uint64_t (&words)[V][64], int lane)
+{
+    Run<V> r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const float t = word_t(words[v][lane]);
+        r.a[v] = is_b(t) ? 1.0f - t : -t;
+        r.b[v] = is_b(t) ? t : 1.0f + t;
+        r.h[v] = word_h(words[v][lane]);
+    }
+    return r;
+}
 __device__ __forceinline__ bool is_there(uint64_t w) { return (uint32_t)w != 0xFFFFFFFFu; }
+
+// The first n waves of a tile, in the order of the recurrence, as one run.  reset: a row starts (ends) in one of them, and the
+// run is what follows it.
+template <int V>
+struct Front {
+    Run<V> run;
+    bool reset;
+    __device__ __forceinline__ Piece<V> piece() const { return Piece<V>(run, reset); }
+};
 
 // One wave: what reaches the tile that is the `at`-th in order, at > 0, from the tiles in front of it.  own() waits for what the
 // tile itself does and returns it; where the tile is the last of its group the group's word and then its state are left here
@@ -294,14 +368,14 @@ __device__ __forceinline__ bool find_carry(uint64_t (&window)[kGroup][V][64], co
     int need, nearest;                                                 // tiles that count; the nearest group with a state, or -1
     const auto look = [&] {
         const uint64_t w = wanted ? get_word(mine) : kNoWord;
-        const uint64_t there = __ballot(is_there(w)), resets = __ballot(word_b(w) == kReset);
+        const uint64_t there = __ballot(is_there(w)), resets = __ballot(word_t(w) == kReset);
         const uint32_t t = (uint32_t)resets & ((1u << kGroup) - 1), g = (uint32_t)(resets >> kGroup);
         need = t ? __builtin_ctz(t) + 1 : pos;
         nearest = g ? __builtin_ctz(g) : -1;
         if (g && (~(uint32_t)(there >> kGroup) & ((1u << nearest) - 1))) nearest = -1;
         return (~(uint32_t)there & ((1u << need) - 1)) == 0;
     };
-    load_floats<V>(carry, nullptr);
+    clear_floats<V>(carry);
     for (bool ok = false; !ok;) {
         while (!look()) __builtin_amdgcn_s_sleep(1);
         ok = true;
@@ -321,27 +395,19 @@ __device__ __forceinline__ bool find_carry(uint64_t (&window)[kGroup][V][64], co
         }
         ok = __all(ok);
     }
-    const bool reset = need > 0 && word_b(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
+    const bool reset = need > 0 && word_t(window[need > 0 ? need - 1 : 0][0][lane]) == kReset;     // (of all channels at once)
     const bool group_end = pos == kGroup - 1;
-    Piece<V> sum;
+    Run<V> sum;
     sum.clear();
     bool leave_state = false;                                          // (otherwise the tile has left it)
     if (group_end && !reset) {
-        const Piece<V> last = own();
-        leave_state = last.b[0] != kReset;
+        const Front<V> last = own();
+        leave_state = !last.reset;
         if (leave_state) {
 #pragma unroll 3
-            for (int e = need - 1; e >= 0; --e) {
-                Piece<V> p;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    p.b[v] = word_b(window[e][v][lane]);
-                    p.h[v] = word_h(window[e][v][lane]);
-                }
-                sum.then(p);
-            }
-            sum.then(last);
-            put_words<V>(groups + c, sum);
+            for (int e = need - 1; e >= 0; --e) sum.then(run_of<V>(window[e], lane));
+            sum.then(last.run);
+            put_words<V>(groups + c, Piece<V>(sum, false));
         }
     }
     for (bool ok = reset; !ok;) {
@@ -361,9 +427,9 @@ __device__ __forceinline__ bool find_carry(uint64_t (&window)[kGroup][V][64], co
                 if (far < k) continue;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float b = word_b(q[k][v]);
-                    ok = ok && is_there(q[k][v]) && (b == kReset || far - k < nearest);
-                    carry[v] = carry_through(b, word_h(q[k][v]), carry[v]);
+                    const float t = word_t(q[k][v]);
+                    ok = ok && is_there(q[k][v]) && (t == kReset || far - k < nearest);
+                    carry[v] = carry_through(t, word_h(q[k][v]), carry[v]);
                 }
             }
         }
@@ -374,68 +440,60 @@ __device__ __forceinline__ bool find_carry(uint64_t (&window)[kGroup][V][64], co
         float end[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) end[v] = carry[v];
-        sum.through(end);
+        Piece<V>(sum, false).through(end);
         put_states<V>(groups + c, end);
     }
-#pragma unroll 4
-    for (int e = need - 1; e >= 0; --e)
+    // (for this tile alone: what each of at most fifteen tiles keeps may be rounded)
+    if (reset)
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = carry_through(word_b(window[e][v][lane]), word_h(window[e][v][lane]), carry[v]);
+        for (int v = 0; v < V; ++v) carry[v] = word_h(window[need - 1][v][lane]);
+#pragma unroll 4
+    for (int e = need - 1 - reset; e >= 0; --e) {
+        const Run<V> r = run_of<V>(window[e], lane);
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = fmaf(r.a[v], carry[v], r.h[v]);
+    }
     return group_end && reset;
 }
 
-// The pieces of a tile's waves, in LDS (array by array: lanes read neighbouring words).
-template <int W, int V>
-struct Pieces {
-    float b[W][V][64], h[W][V][64];
-    __device__ __forceinline__ void put(int wave, int lane, const Piece<V> &p)
-    {
-#pragma unroll
-        for (int v = 0; v < V; ++v) b[wave][v][lane] = p.b[v], h[wave][v][lane] = p.h[v];
-    }
-    __device__ __forceinline__ Piece<V> get(int wave, int lane) const
-    {
-        Piece<V> p;
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.b[v] = b[wave][v][lane], p.h[v] = h[wave][v][lane];
-        return p;
-    }
-    // waves 0 .. n - 1 one after the other, n > 0
-    __device__ __forceinline__ Piece<V> front(int n, int lane) const
-    {
-        Piece<V> p = get(0, lane);
-#pragma unroll 3
-        for (int w = 1; w < n; ++w) p.then(get(w, lane));
-        return p;
-    }
-    // waves W - 1 .. first one after the other, first < W
-    __device__ __forceinline__ Piece<V> behind(int first, int lane) const
-    {
-        Piece<V> p = get(W - 1, lane);
-#pragma unroll 3
-        for (int w = W - 2; w >= first; --w) p.then(get(w, lane));
-        return p;
-    }
-};
-
 template <int S, int W, int V>
 struct ScanShared {
-    Pieces<W, V> parts;                           // of what the tile hands on: states forwards, gradients backwards
+    float a[W][V][64], b[W][V][64], h[W][V][64];  // the waves' runs, in order: of states forwards, gradients backwards
     uint64_t window[kGroup][V][64];
     float carry[V][64];
     uint32_t tile;
-    int arrived;                                  // waves whose pieces are there
+    uint32_t arrived;                             // how many waves' runs are there, and from bit 8 on which hold a reset
     Edges<S> edges[W];
-    // A wave's pieces are there.  True for the last of the waves.
-    __device__ __forceinline__ bool arrive(int lane)
+    static_assert(W <= 24, "a bit to a wave");
+
+    // A wave's run is there.  True for the last of the waves.
+    __device__ __forceinline__ bool arrive(int nth, int lane, const Run<V> &r, bool reset)
     {
-        int before = 0;
-        if (lane == 0) before = __hip_atomic_fetch_add(&arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
-        return __builtin_amdgcn_readfirstlane(before) == W - 1;
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[nth][v][lane] = r.a[v], b[nth][v][lane] = r.b[v], h[nth][v][lane] = r.h[v];
+        uint32_t before = 0;
+        if (lane == 0)
+            before = __hip_atomic_fetch_add(&arrived, 1u + (reset ? 256u << nth : 0u), __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
+        return (__builtin_amdgcn_readfirstlane(before) & 255) == W - 1;
     }
-    __device__ __forceinline__ void wait_for_all() const
+    // The first n of the waves, n > 0, once all are there.
+    __device__ __forceinline__ Front<V> front(int n, int lane) const
     {
-        while (__hip_atomic_load(&arrived, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) < W) __builtin_amdgcn_s_sleep(1);
+        uint32_t now;
+        while (((now = __hip_atomic_load(&arrived, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP)) & 255) < W)
+            __builtin_amdgcn_s_sleep(1);
+        const uint32_t resets = __builtin_amdgcn_readfirstlane(now) >> 8 & ((1u << n) - 1);
+        const int first = resets ? 31 - __builtin_clz(resets) : 0;
+        const auto get = [&](int w) {
+            Run<V> r;
+#pragma unroll
+            for (int v = 0; v < V; ++v) r.a[v] = a[w][v][lane], r.b[v] = b[w][v][lane], r.h[v] = h[w][v][lane];
+            return r;
+        };
+        Front<V> f{get(first), resets != 0};
+#pragma unroll 3
+        for (int w = first + 1; w < n; ++w) f.run.then(get(w));
+        return f;
     }
 };
 
@@ -471,6 +529,13 @@ struct Strip {
         token_bytes = (int)(stride * sizeof(T));
         rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(base + span.lowest * stride), 0,
                                                  (n - 1) * token_bytes + (int)(dim * sizeof(T)), 0x00020000);
+    }
+    // No array: loads give zeros, since they lie behind the end of a buffer of no bytes (at its first token, so that no offset
+    // of a token is taken off those none).
+    __device__ __forceinline__ void empty()
+    {
+        n = 1;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(nullptr, 0, 0, 0x00020000);
     }
     __device__ __forceinline__ int offset(int i) const                 // (positions behind the last one: the last one)
     {
@@ -539,15 +604,15 @@ __device__ __forceinline__ void carry_wave(ScanShared<S, W, V> &sh, const ScanAr
                                            uint32_t c, Own own, int lane)
 {
     float carry[V];
-    load_floats<V>(carry, nullptr);
+    clear_floats<V>(carry);
     const bool leave_state = nth > 0 && find_carry<V>(sh.window, a.tile_words, a.group_words, a.dim, nth, slab0, c, own, lane, carry);
 #pragma unroll
     for (int v = 0; v < V; ++v) sh.carry[v][lane] = carry[v];
     __syncthreads();
     if (leave_state) {
-        const Piece<V> p = own();
-        if (p.b[0] != kReset) {                                        // (otherwise the tile has left it)
-            p.through(carry);
+        const Front<V> f = own();
+        if (!f.reset) {                                                // (otherwise the tile has left it)
+            f.piece().through(carry);
             put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, carry);
         }
     }
@@ -559,12 +624,14 @@ template <int V, typename T>
 __device__ __forceinline__ void put_tile(const ScanArgs<T> &a, uint32_t nth, uint32_t c, const Piece<V> &p)
 {
     put_words<V>(a.tile_words + (int64_t)nth * a.dim + c, p);
-    if (nth % kGroup == kGroup - 1 && p.b[0] == kReset)
+    if (nth % kGroup == kGroup - 1 && p.is_reset())
         put_states<V>(a.group_words + (int64_t)(nth / kGroup) * a.dim + c, p.h);
 }
 
+// (Two workgroups on a CU, three with one channel to a lane: with two registers more than the 128 of that it was one, 568 us
+// instead of 410 for 64 x 8192 x 512.)
 template <typename T, int V, int S, int W, bool REV>
-__global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
+__global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V == 1 ? 6 : 4))) void gated_scan_kernel(ScanArgs<T> a)
 {
     __shared__ ScanShared<S, W, V> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -574,11 +641,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
     const uint32_t c = span.c;
     if (wave == W) {
-        const auto own = [&] {
-            sh.wait_for_all();
-            return sh.parts.front(W, lane);
-        };
-        carry_wave<S, W, V>(sh, a, tile, span.slab0, c, own, lane);
+        carry_wave<S, W, V>(sh, a, tile, span.slab0, c, [&] { return sh.front(W, lane); }, lane);
         return;
     }
     const int n = span.n;
@@ -594,70 +657,58 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_kernel(ScanArgs<T> a)
     uint64_t starts, ends;
     const bool rim = find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
         float h[V];
-        load_floats<V>(h, a.h0 ? a.h0 + row * a.dim + c : nullptr);
+        load_row<V>(h, a.h0, row, a.dim, c);
         if (a.last) store_floats<V>(a.last + row * a.dim + c, h);
     });
     if (const uint64_t outside = rim ? outside_rows<S, REV>(axis, span.p0, n) : 0) {
         clear_cells<T, V, S>(x, outside);
         clear_cells<T, V, S>(g, outside);
     }
-    const bool plain = n == S && (starts | ends) == 0;                 // no row starts or ends here: no step has to look
-    const auto initial = [&](int i) {
-        const int64_t row = axis.row(one_row(edges.start[i]));
-        return a.h0 && row >= 0 ? a.h0 + row * a.dim + c : nullptr;
-    };
+    const uint64_t looks = starts | ends >> 1 | ~0ull << n;            // positions at which a step has to look
 
-    float k[S][V];
-    Piece<V> own;
+    // What the tokens up to each make of zero, and the factor of what comes in: state = A c + H.  (24 roundings of f at most: it is
+    // between the tiles that an f next to 1 must not be rounded, and there its b is at hand.)
+    float A[S][V], H[S][V];
+    Run<V> own;
     own.clear();
-    const auto first_pass = [&](auto with_edges) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (with_edges && i >= n) break;
-            if (with_edges && (starts >> i & 1)) load_floats<V>(own.h, initial(i));
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                k[i][v] = gate_taken(to_float(g[i].v[v]));
-                own.h[v] = next_state(k[i][v], own.h[v], to_float(x[i].v[v]));
-                own.factor(v, k[i][v]);
-            }
+    by_parts<S>(looks, [&](int i, auto look) {
+        if (look && i >= n) return;
+        if (look && (starts >> i & 1)) {
+            own.clear();
+            load_row<V>(own.h, a.h0, axis.row(one_row(edges.start[i])), a.dim, c);
         }
-    };
-    if (plain) first_pass(std::false_type{});
-    else first_pass(std::true_type{});
-    keep_raw<T, V, S>(x);
-    own.close(starts != 0 || span.p0 == 0);                            // (the axis' first token starts a span, were the offsets wrong)
-    sh.parts.put(wave, lane, own);
-    if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, tile, c, sh.parts.front(W, lane));
-    Piece<V> front;                                                    // the tile's waves in front of this one
-    front.clear();
-    if (wave > 0) {
-        sh.wait_for_all();
-        front = sh.parts.front(wave, lane);
-    }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Gate gate = gate_of(to_float(g[i].v[v]));
+            own.h[v] = fmaf(gate.f, own.h[v], gate.k * to_float(x[i].v[v]));
+            own.factor(v, gate);
+            A[i][v] = own.a[v];
+            H[i][v] = own.h[v];
+        }
+    });
+    // (the axis' first token starts a span, were the offsets wrong)
+    if (sh.arrive(wave, lane, own, starts != 0 || span.p0 == 0) && a.n_tiles > 1) put_tile<V>(a, tile, c, sh.front(W, lane).piece());
+    Front<V> front;                                                    // the tile's waves in front of this one
+    if (wave > 0) front = sh.front(wave, lane);
     __syncthreads();
-    float h[V];
+    float c0[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = sh.carry[v][lane];
-    if (wave > 0) front.through(h);
-    if (a.states && n > 0) store_floats<V>(a.states + span.p0 / S * a.dim + c, h);
+    for (int v = 0; v < V; ++v) c0[v] = sh.carry[v][lane];
+    if (wave > 0) front.piece().through(c0);
+    if (a.states && n > 0) store_floats<V>(a.states + span.p0 / S * a.dim + c, c0);
     const strip ys(a.y, a.dim, span, a.dim);
-    const auto second_pass = [&](auto with_edges) {
+    by_parts<S>(looks, [&](int i, auto look) {
+        if (look && i >= n) return;
+        if (look && (starts >> i & 1)) clear_floats<V>(c0);
+        float h[V];
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (with_edges && i >= n) break;
-            if (with_edges && (starts >> i & 1)) load_floats<V>(h, initial(i));
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = next_state(k[i][v], h[v], to_float(x[i].v[v]));
-            ys.store(i, h);
-            if (with_edges && (ends >> (i + 1) & 1) && a.last) {
-                const int64_t row = axis.row(one_row(edges.end[i + 1]));
-                if (row >= 0) store_floats<V>(a.last + row * a.dim + c, h);
-            }
+        for (int v = 0; v < V; ++v) h[v] = fmaf(A[i][v], c0[v], H[i][v]);
+        ys.store(i, h);
+        if (look && (ends >> (i + 1) & 1) && a.last) {
+            const int64_t row = axis.row(one_row(edges.end[i + 1]));
+            if (row >= 0) store_floats<V>(a.last + row * a.dim + c, h);
         }
-    };
-    if (plain) second_pass(std::false_type{});
-    else second_pass(std::true_type{});
+    });
 }
 
 //   dh_t = dy_t + f_(t+1) dh_(t+1),  dx_t = (1 - f_t) dh_t,  dgate_t = dh_t (h_(t-1) - x_t) f_t (1 - f_t)
@@ -673,14 +724,10 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
     const Span<V, S, W, REV> span(a.rows, a.dim, tile, slab, wave, lane);
     const uint32_t c = span.c;
     if (wave == W) {
-        const auto own = [&] {
-            sh.wait_for_all();
-            return sh.parts.behind(0, lane);
-        };
-        carry_wave<S, W, V>(sh, a, nth, span.slab0, c, own, lane);
+        carry_wave<S, W, V>(sh, a, nth, span.slab0, c, [&] { return sh.front(W, lane); }, lane);
         return;
     }
-    const int n = span.n;
+    const int n = span.n, order = W - 1 - wave;
     typedef Strip<T, V, S, REV> strip;
     const strip xs(a.x, a.x_stride, span, a.dim), gs(a.gate, a.gate_stride, span, a.dim);
     Cell<T, V> x[S], g[S], dy[S];
@@ -689,19 +736,15 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
         x[i] = xs.load(i);
         g[i] = gs.load(i);
     }
-    if (a.dy) {
-        const strip ds(a.dy, a.dy_stride, span, a.dim);
+    strip ds(a.dy, a.dy_stride, span, a.dim);
+    if (!a.dy) ds.empty();
 #pragma unroll
-        for (int i = 0; i < S; ++i) dy[i] = ds.load(i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < S; ++i) dy[i] = Cell<T, V>{};
-    }
+    for (int i = 0; i < S; ++i) dy[i] = ds.load(i);
     Edges<S> &edges = sh.edges[wave];
     uint64_t starts, ends;
     const bool rim = find_edges<S, REV>(axis, span.p0, n, lane, edges, starts, ends, [&](int64_t row) {
         float d[V];
-        load_floats<V>(d, a.dlast ? a.dlast + row * a.dim + c : nullptr);
+        load_row<V>(d, a.dlast, row, a.dim, c);
         if (a.dh0) store_floats<V>(a.dh0 + row * a.dim + c, d);
     });
     if (const uint64_t outside = rim ? outside_rows<S, REV>(axis, span.p0, n) : 0) {
@@ -709,88 +752,72 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
         clear_cells<T, V, S>(g, outside);
         clear_cells<T, V, S>(dy, outside);
     }
-    const bool plain = n == S && (starts | ends) == 0;
-    const auto initial = [&](int i) {
-        const int64_t row = axis.row(one_row(edges.start[i]));
-        return a.h0 && row >= 0 ? a.h0 + row * a.dim + c : nullptr;
-    };
-    const auto final_grad = [&](int i) {
-        const int64_t row = axis.row(one_row(edges.end[i + 1]));
-        return a.dlast && row >= 0 ? a.dlast + row * a.dim + c : nullptr;
+    const uint64_t looks = starts | ends >> 1 | ~0ull << n;            // positions at which a step has to look
+    const auto final_grad = [&](int i, float (&to)[V]) {
+        load_row<V>(to, a.dlast, axis.row(one_row(edges.end[i + 1])), a.dim, c);
     };
 
-    float k[S][V];
-    Piece<V> own;
+    float m[S][V];                                                     // the gates
+    Run<V> own;
     own.clear();
-    const auto first_pass = [&](auto with_edges) {
-#pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-            if (with_edges && i >= n) continue;
-            if (with_edges && (ends >> (i + 1) & 1)) load_floats<V>(own.h, final_grad(i));
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                k[i][v] = gate_taken(to_float(g[i].v[v]));
-                own.h[v] = forget(k[i][v], own.h[v] + to_float(dy[i].v[v]));
-                own.factor(v, k[i][v]);
-            }
+    by_parts_back<S>(looks, [&](int i, auto look) {
+        if (look && i >= n) return;
+        if (look && (ends >> (i + 1) & 1)) {
+            own.clear();
+            final_grad(i, own.h);
         }
-    };
-    if (plain) first_pass(std::false_type{});
-    else first_pass(std::true_type{});
-    keep_raw<T, V, S>(x);
-    keep_raw<T, V, S>(dy);
-    own.close(ends != 0 || (n > 0 && span.p0 + n == a.rows.total));    // (the axis' last token ends a span)
-    sh.parts.put(wave, lane, own);
-    if (sh.arrive(lane) && a.n_tiles > 1) put_tile<V>(a, nth, c, sh.parts.behind(0, lane));
-    Piece<V> behind;                                                   // the tile's waves behind this one
-    behind.clear();
-    if (wave < W - 1) {
-        sh.wait_for_all();
-        behind = sh.parts.behind(wave + 1, lane);
-    }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Gate gate = gate_of(to_float(g[i].v[v]));
+            m[i][v] = one_number(gate);
+            own.h[v] = gate.f * (own.h[v] + to_float(dy[i].v[v]));
+            own.factor(v, gate);
+        }
+    });
+    // (the axis' last token ends a span, were the offsets wrong)
+    const bool reset = ends != 0 || (n > 0 && span.p0 + n == a.rows.total);
+    if (sh.arrive(order, lane, own, reset) && a.n_tiles > 1) put_tile<V>(a, nth, c, sh.front(W, lane).piece());
+    Front<V> behind;                                                   // the tile's waves behind this one
+    if (order > 0) behind = sh.front(order, lane);
     float h[V];                                                        // the state in front of the wave's first token
-    load_floats<V>(h, n > 0 ? a.states + span.p0 / S * a.dim + c : nullptr);
+    load_row<V>(h, a.states, n > 0 ? span.p0 / S : -1, a.dim, c);
     __syncthreads();
     float carry[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = sh.carry[v][lane];
-    if (wave < W - 1) behind.through(carry);
+    if (order > 0) behind.piece().through(carry);
     const strip dxs(a.dx, a.dim, span, a.dim), dgs(a.dgate, a.dim, span, a.dim);
-    const auto second_pass = [&](auto with_edges) {
-        float from_x[S][V];                                            // h_(t-1) - x_t
+    float from_x[S][V];                                                // h_(t-1) - x_t
+    by_parts<S>(looks, [&](int i, auto look) {
+        if (look && i >= n) return;
+        if (look && (starts >> i & 1)) load_row<V>(h, a.h0, axis.row(one_row(edges.start[i])), a.dim, c);
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            if (with_edges && i >= n) break;
-            if (with_edges && (starts >> i & 1)) load_floats<V>(h, initial(i));
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float xv = to_float(x[i].v[v]);
-                from_x[i][v] = h[v] - xv;
-                h[v] = fmaf(-k[i][v], from_x[i][v], h[v]);
-            }
+        for (int v = 0; v < V; ++v) {
+            const Gate gate = gate_from(m[i][v]);
+            const float xv = to_float(x[i].v[v]);
+            from_x[i][v] = h[v] - xv;
+            h[v] = fmaf(gate.f, h[v], gate.k * xv);
         }
+    });
+    by_parts_back<S>(looks, [&](int i, auto look) {
+        if (look && i >= n) return;
+        if (look && (ends >> (i + 1) & 1)) final_grad(i, carry);
+        float dx[V], dg[V];
 #pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-            if (with_edges && i >= n) continue;
-            if (with_edges && (ends >> (i + 1) & 1)) load_floats<V>(carry, final_grad(i));
-            float dx[V], dg[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float dh = to_float(dy[i].v[v]) + carry[v];
-                dx[v] = k[i][v] * dh;
-                dg[v] = dh * from_x[i][v] * slope(k[i][v]);
-                carry[v] = forget(k[i][v], dh);
-            }
-            dxs.store(i, dx);
-            dgs.store(i, dg);
-            if (with_edges && (starts >> i & 1) && a.dh0) {
-                const int64_t row = axis.row(one_row(edges.start[i]));
-                if (row >= 0) store_floats<V>(a.dh0 + row * a.dim + c, carry);
-            }
+        for (int v = 0; v < V; ++v) {
+            const Gate gate = gate_from(once_more(m[i][v]));
+            const float dh = to_float(dy[i].v[v]) + carry[v];
+            dx[v] = gate.k * dh;
+            dg[v] = dh * from_x[i][v] * (gate.f * gate.k);
+            carry[v] = gate.f * dh;
         }
-    };
-    if (plain) second_pass(std::false_type{});
-    else second_pass(std::true_type{});
+        dxs.store(i, dx);
+        dgs.store(i, dg);
+        if (look && (starts >> i & 1) && a.dh0) {
+            const int64_t row = axis.row(one_row(edges.start[i]));
+            if (row >= 0) store_floats<V>(a.dh0 + row * a.dim + c, carry);
+        }
+    });
 }
 
 // Rows that are all empty have no tile: their states go straight through.
@@ -808,8 +835,8 @@ __global__ __launch_bounds__(256) void gated_step_kernel(
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n_rows * dim) return;
     const int64_t b = i / dim, c = i - b * dim;
-    const float k = gate_taken(to_float(gate[b * gate_stride + c]));
-    const float h = next_state(k, state ? state[i] : 0.0f, to_float(x[b * x_stride + c]));
+    const Gate g = gate_of(to_float(gate[b * gate_stride + c]));
+    const float h = next_state(g, state ? state[i] : 0.0f, to_float(x[b * x_stride + c]));
     y[i] = from_float<T>(h);
     new_state[i] = h;
 }

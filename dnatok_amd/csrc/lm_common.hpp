@@ -38,15 +38,33 @@ struct Rows {
     }
 };
 
-// The gate of the recurrence: k = 1 - f = 1 / (1 + exp(g)), to full relative precision however small (1 - f would be what
-// is left of a rounded f).  The steps below use k alone, so that a channel that forgets once in a million tokens
-// keeps its rate; each rounds once, by at most half a unit of the larger of what goes in.
-__device__ __forceinline__ float gate_taken(float g)
+// The gate of the recurrence: f = 1 / (1 + E) and k = 1 - f = E f with E = exp(-g), each to a part in 2^24 / (|g| + 4) of itself however
+// small it is (what is left of a rounded 1 - k or 1 - f would not be), so that a channel that forgets once in a million
+// tokens keeps its rate, and one that keeps a millionth of a state keeps that much, and passes that much of a gradient on.
+// (E is at most 2^126, beyond that its reciprocal would be 0 and E f with it: f is 2^-126 where it should be less.  `minimum` keeps a NaN.)
+struct Gate {
+    float f, k;
+};
+__device__ __forceinline__ Gate gate_of(float g)
 {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(1.44269504f * g));
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(-1.44269504f * g, 126.0f));
+    const float f = __builtin_amdgcn_rcpf(1.0f + e);
+    return Gate{f, e * f};
 }
-__device__ __forceinline__ float next_state(float k, float h, float x) { return fmaf(k, x - h, h); }     // f h + (1 - f) x
-__device__ __forceinline__ float forget(float k, float v) { return fmaf(-k, v, v); }                     // f v
-__device__ __forceinline__ float slope(float k) { return fmaf(-k, k, k); }                               // f (1 - f)
+// Both in one number: k where it is the smaller, otherwise -f.  The larger is 1 - the smaller, to half a unit.
+__device__ __forceinline__ float one_number(const Gate &g) { return g.k <= 0.5f ? g.k : -g.f; }
+__device__ __forceinline__ Gate gate_from(float m)
+{
+    const float large = 1.0f - __builtin_fabsf(m);
+    return m >= 0.0f ? Gate{large, m} : Gate{-m, large};
+}
+// f h + k x without the rounding of an f (or k) next to 1, which over many steps would be a wrong rate: the larger one's part with
+// the smaller's share taken off it, and the smaller one's added.
+__device__ __forceinline__ float next_state(const Gate &g, float h, float x)
+{
+    const bool keeps = g.k <= 0.5f;
+    const float p = keeps ? h : x, q = keeps ? x : h, s = keeps ? g.k : g.f;
+    return fmaf(s, q, fmaf(-s, p, p));
+}
 
 }  // namespace dnatok
