@@ -237,7 +237,9 @@ __device__ __forceinline__ void clear_cells(Cell<T, V> (&c)[S], uint64_t which)
 
 // What a run of tokens makes of the state in front of it, c -> a c + h, with b = 1 - a beside a: a rounded product of factors next to 1
 // would lose what slow channels forget, always in the same direction where the gate is constant, and what is left of 1 - b would
-// lose a small a.
+// lose a small a.  An infinite state stays one whatever is forgotten: no a is 0.
+__device__ __forceinline__ float not_zero(float a) { return fmaxf(a, FLT_MIN); }      // (of a NaN as well: then h is one)
+
 template <int V>
 struct Run {
     float a[V], b[V], h[V];
@@ -257,20 +259,20 @@ struct Run {
         for (int v = 0; v < V; ++v) {
             h[v] = fmaf(r.a[v], h[v], r.h[v]);
             b[v] = fmaf(a[v], r.b[v], b[v]);
-            a[v] *= r.a[v];
+            a[v] = not_zero(a[v] * r.a[v]);
         }
     }
 };
 
-// The same of a tile or a group in a word: of a and b the one that is at most 1/2, t >= 0 is b, t < 0 (-0 among them) is -a.
+// The same of a tile or a group in a word: of a and b the one that is at most 1/2, t >= 0 is b, t < 0 is -a.
 // Where a row begins inside (or ends, for what flows backwards) it is a reset: h comes out, and nothing of what comes in,
 // be it infinite.
 constexpr float kReset = 2.0f;
 
-__device__ __forceinline__ bool is_b(float t) { return !__builtin_signbitf(t); }
+__device__ __forceinline__ bool is_b(float t) { return t >= 0.0f; }
 __device__ __forceinline__ float carry_through(float t, float h, float c)
 {
-    return t == kReset ? h : fmaf(-t, c, is_b(t) ? c : 0.0f) + h;
+    return t == kReset ? h : (__builtin_isinf(c) ? c : fmaf(-t, c, is_b(t) ? c : 0.0f)) + h;
 }
 
 template <int V>
@@ -470,7 +472,7 @@ struct ScanShared {
     __device__ __forceinline__ bool arrive(int nth, int lane, const Run<V> &r, bool reset)
     {
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[nth][v][lane] = r.a[v], b[nth][v][lane] = r.b[v], h[nth][v][lane] = r.h[v];
+        for (int v = 0; v < V; ++v) a[nth][v][lane] = not_zero(r.a[v]), b[nth][v][lane] = r.b[v], h[nth][v][lane] = r.h[v];
         uint32_t before = 0;
         if (lane == 0)
             before = __hip_atomic_fetch_add(&arrived, 1u + (reset ? 256u << nth : 0u), __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -629,7 +631,7 @@ __device__ __forceinline__ void put_tile(const ScanArgs<T> &a, uint32_t nth, uin
 }
 
 // (Two workgroups on a CU, three with one channel to a lane: with two registers more than the 128 of that it was one, 568 us
-// instead of 410 for 64 x 8192 x 512.)
+// instead of 413 for 64 x 8192 x 512.)
 template <typename T, int V, int S, int W, bool REV>
 __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V == 1 ? 6 : 4))) void gated_scan_kernel(ScanArgs<T> a)
 {
@@ -682,7 +684,7 @@ __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V 
             const Gate gate = gate_of(to_float(g[i].v[v]));
             own.h[v] = fmaf(gate.f, own.h[v], gate.k * to_float(x[i].v[v]));
             own.factor(v, gate);
-            A[i][v] = own.a[v];
+            A[i][v] = own.a[v] = not_zero(own.a[v]);
             H[i][v] = own.h[v];
         }
     });

@@ -3,6 +3,7 @@
 
 #include "common.hpp"
 
+#include <cfloat>
 #include <type_traits>
 
 namespace dnatok {
@@ -58,13 +59,15 @@ __device__ __forceinline__ Gate gate_from(float m)
     const float large = 1.0f - __builtin_fabsf(m);
     return m >= 0.0f ? Gate{large, m} : Gate{-m, large};
 }
+// v, or the largest number of its sign for an infinity: what is taken off v in proportion, so that an infinity stays one.
+__device__ __forceinline__ float finite(float v) { return __builtin_amdgcn_fmed3f(v, -FLT_MAX, FLT_MAX); }
 // f h + k x without the rounding of an f (or k) next to 1, which over many steps would be a wrong rate: the larger one's part with
 // the smaller's share taken off it, and the smaller one's added.
 __device__ __forceinline__ float next_state(const Gate &g, float h, float x)
 {
     const bool keeps = g.k <= 0.5f;
     const float p = keeps ? h : x, q = keeps ? x : h, s = keeps ? g.k : g.f;
-    return fmaf(s, q, fmaf(-s, p, p));
+    return fmaf(s, q, fmaf(-s, finite(p), p));
 }
 
 }  // namespace dnatok
