@@ -922,18 +922,21 @@ bool paired(const ScanArgs<T> &a)
            ((a.dim | a.x_stride | a.gate_stride | a.dy_stride) & 1) == 0;
 }
 
+// (everything that is refused is refused before the first launch, that of the words)
 template <typename T, int V>
-int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hipStream_t s)
+int launch_scan(const char *who, ScanArgs<T> a, const Layout &l, void *work, bool backward, bool reverse, hipStream_t s)
 {
     a.n_slabs = (uint32_t)((a.dim + 64 * V - 1) / (64 * V));
     // (a wave's tokens in 32 bits)
     const int64_t widest = std::max({a.x_stride, a.gate_stride, a.dy_stride, a.dim});
-    DNATOK_REQUIRE(widest * (int64_t)sizeof(T) * (kSteps + 1) < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: tokens too far apart", who);
+    DNATOK_REQUIRE(widest <= ((1ll << 31) - 1) / (int64_t)(sizeof(T) * (kSteps + 1)), DNATOK_E_TOO_LARGE, "%s: tokens too far apart", who);
     // (eight workgroups of a slab at a time: some find no tile left)
     const int64_t blocks = a.n_slabs * (a.n_tiles == 1 ? 1 : (a.n_tiles + 7) & ~7ll);
     const unsigned threads = 64 * ((backward ? kBackwardWaves : kForwardWaves) + 1);
     DNATOK_REQUIRE(blocks * threads < (1ll << 32), DNATOK_E_TOO_LARGE, "%s: more cells than one launch takes", who);
     const unsigned grid = (unsigned)blocks;
+    if (l.bytes)
+        if (int rc = fill_words(a, l, work, s)) return rc;
     if (backward) {
         if (reverse) gated_scan_backward_kernel<T, V, kSteps, kBackwardWaves, true><<<grid, threads, 0, s>>>(a);
         else gated_scan_backward_kernel<T, V, kSteps, kBackwardWaves, false><<<grid, threads, 0, s>>>(a);
@@ -946,11 +949,11 @@ int launch_scan(const char *who, ScanArgs<T> a, bool backward, bool reverse, hip
 }
 
 template <typename T>
-int run_scan(const char *who, const ScanArgs<T> &a, bool backward, bool reverse, hipStream_t s)
+int run_scan(const char *who, const ScanArgs<T> &a, const Layout &l, void *work, bool backward, bool reverse, hipStream_t s)
 {
     if constexpr (sizeof(T) == 2)
-        if (paired(a)) return launch_scan<T, 2>(who, a, backward, reverse, s);
-    return launch_scan<T, 1>(who, a, backward, reverse, s);
+        if (paired(a)) return launch_scan<T, 2>(who, a, l, work, backward, reverse, s);
+    return launch_scan<T, 1>(who, a, l, work, backward, reverse, s);
 }
 
 }  // namespace
@@ -989,8 +992,7 @@ extern "C" int dnatok_gated_scan(const void *x, int64_t x_stride, const void *ga
         a.rows = Rows{offsets, n_rows, total, total / n_rows};
         a.dim = dim, a.n_tiles = l.tiles, a.h0 = h0, a.states = states;
         a.y = (T *)y, a.last = last;
-        if (l.bytes) rc = fill_words(a, l, work, s);
-        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, false, reverse != 0, s);
+        rc = run_scan<T>(who, a, l, work, false, reverse != 0, s);
     });
     return rc;
 }
@@ -1021,8 +1023,7 @@ extern "C" int dnatok_gated_scan_backward(const void *x, int64_t x_stride, const
         a.dim = dim, a.n_tiles = l.tiles, a.h0 = h0, a.states = const_cast<float *>(states);
         a.dy = (const T *)dy, a.dy_stride = dy ? dy_stride : 0, a.dlast = dlast;
         a.dx = (T *)dx, a.dgate = (T *)dgate, a.dh0 = dh0;
-        if (l.bytes) rc = fill_words(a, l, work, s);
-        if (rc == DNATOK_OK) rc = run_scan<T>(who, a, true, reverse != 0, s);
+        rc = run_scan<T>(who, a, l, work, true, reverse != 0, s);
     });
     return rc;
 }
