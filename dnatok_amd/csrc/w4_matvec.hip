@@ -106,6 +106,19 @@ __device__ __forceinline__ typename Frag<T>::type unpack(uint32_t q, uint32_t mi
     return f;
 }
 
+// The same for bfloat16 as q - zero, exactly, by way of 32 bits: three times the instructions.
+__device__ __forceinline__ Frag<__bf16>::type unpack_exact(uint32_t q, float zero)
+{
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                                      // (whole numbers below 2^8: the low halves are zeros)
+        const uint32_t low = __float_as_uint((float)(q >> (4 * i) & 15) - zero);
+        const uint32_t high = __float_as_uint((float)(q >> (4 * i + 16) & 15) - zero);
+        o[i] = __builtin_amdgcn_perm(high, low, 0x07060302);
+    }
+    return __builtin_bit_cast(Frag<__bf16>::type, o);
+}
+
 // Words j of four lanes sixteen apart, which hold blocks 0 .. 3 of the columns: to word j of block i in register i of
 // lane j.
 __device__ __forceinline__ u32x4 exchange(u32x4 q)
@@ -164,8 +177,8 @@ __device__ __forceinline__ void load_slice(const W4Args<T> &a, __amdgpu_buffer_r
 }
 
 // acc += x times a slice of a tile, blocks b0 .. of which a.blocks bounds the last.  x(b, i): columns of block b of the
-// slice, i-th sixteen rows; sum(seg, i): their sum over a segment, where the type needs it.
-template <typename T, int MT, int KB, int GB, typename X, typename Sum>
+// slice, i-th sixteen rows; sum(seg, i): their sum over a segment, where the type needs it.  EXACT: with q - zero in bfloat16 too.
+template <typename T, int MT, int KB, int GB, bool EXACT, typename X, typename Sum>
 __device__ __forceinline__ void multiply(const W4Args<T> &a, const Slice<KB, KB / GB> &s, int32_t b0, X x, Sum sum,
                                          f32x4 (&acc)[MT])
 {
@@ -184,7 +197,9 @@ __device__ __forceinline__ void multiply(const W4Args<T> &a, const Slice<KB, KB 
                 minus = 0xE400u + s.zero[seg];                         // -1024 - zero
                 minus |= minus << 16;
             }
-            const auto w = unpack<T>(q[j], minus);
+            typename Frag<T>::type w;
+            if constexpr (EXACT && !half) w = unpack_exact(q[j], (float)s.zero[seg]);
+            else w = unpack<T>(q[j], minus);
 #pragma unroll
             for (int i = 0; i < MT; ++i) c[i] = mfma(x(b, i), w, b % GB == 0 ? zero4 : c[i]);
             if ((b + 1) % GB == 0) {
@@ -192,7 +207,7 @@ __device__ __forceinline__ void multiply(const W4Args<T> &a, const Slice<KB, KB 
                 const float off = -128.0f - (float)s.zero[seg];
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    if constexpr (!half) {
+                    if constexpr (!half && !EXACT) {
                         const f32x4 xs = sum(seg, i);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) c[i][e] = fmaf(off, xs[e], c[i][e]);
@@ -203,6 +218,23 @@ __device__ __forceinline__ void multiply(const W4Args<T> &a, const Slice<KB, KB 
             }
         }
     }
+}
+
+// bfloat16: (128 + q) x and the sum of x are infinities, and their difference no number, where x holds one or is so large that
+// 2^8 times it passes the largest number.  A wave whose sums are not all finite therefore does its slices once more with q - zero,
+// and takes those for the sums that are not: an infinity where the formula has one, and no other row is touched.  The first
+// pass pays one comparison at its end for that.
+__device__ __forceinline__ bool all_finite(f32x4 acc)
+{
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ok = ok && __builtin_isfinite(acc[e]);
+    return __all(ok);
+}
+__device__ __forceinline__ void take_where_not_finite(f32x4 &acc, f32x4 exact)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = __builtin_isfinite(acc[e]) ? acc[e] : exact[e];
 }
 
 // The waves' sums meet, RT tiles of sixteen rows of W at a time, and go to y.  `sums`: [kW4Waves][RT][MT][64].
@@ -291,22 +323,32 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_row_kernel(W4Args<T> a)
         __syncthreads();
     }
     f32x4 acc[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-    const auto use = [&](const Slice<KB, SEGS> &s, int32_t at) {
+    const auto use = [&](const Slice<KB, SEGS> &s, int32_t at, f32x4 (&to)[1], auto exact) {
         const u32x4 *const mine = xs + at * 4 + kq;
         const float *const seg = seg_sums + at / GB;
-        multiply<T, 1, KB, GB>(a, s, at, [&](int b, int) { return __builtin_bit_cast(frag, mine[b * 4]); },
-                               [&](int i, int) {
-                                   const float v = seg[i];
-                                   return f32x4{v, v, v, v};
-                               },
-                               acc);
+        multiply<T, 1, KB, GB, exact.value>(a, s, at, [&](int b, int) { return __builtin_bit_cast(frag, mine[b * 4]); },
+                                            [&](int i, int) {
+                                                const float v = seg[i];
+                                                return f32x4{v, v, v, v};
+                                            },
+                                            to);
     };
     for (; b0 < a.blocks; b0 += 2 * kStep) {
-        use(even, b0);
+        use(even, b0, acc, std::false_type{});
         load(even, b0 + 2 * kStep);
         if (b0 + kStep >= a.blocks) break;
-        use(odd, b0 + kStep);
+        use(odd, b0 + kStep, acc, std::false_type{});
         load(odd, b0 + 3 * kStep);
+    }
+    if constexpr (!half) {
+        if (!all_finite(acc[0])) {
+            f32x4 exact[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+            for (int32_t at = wave * KB; at < a.blocks; at += kStep) {
+                load(even, at);
+                use(even, at, exact, std::true_type{});
+            }
+            take_where_not_finite(acc[0], exact[0]);
+        }
     }
     if (lane < 16) sums[wave][r] = acc[0][0];
     __syncthreads();
@@ -404,10 +446,44 @@ __global__ __launch_bounds__(64 * kW4Waves) void w4_kernel(W4Args<T> a)
         for (int t = 0; t < TT; ++t) {
             const Slice<KB, SEGS> s = next;
             if (t + 1 < TT) load_slice<T, KB, GB>(a, rows, n0, (t + 1) * 16 + r, b0, kq, next);
-            multiply<T, MT, KB, GB>(a, s, b0, [&](int b, int i) { return x[b][i]; },
-                                    [&](int seg, int i) { return x_sums[wave][seg][i][kq]; }, acc[t]);
+            multiply<T, MT, KB, GB, false>(a, s, b0, [&](int b, int i) { return x[b][i]; },
+                                           [&](int seg, int i) { return x_sums[wave][seg][i][kq]; }, acc[t]);
         }
         if constexpr (!half) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if constexpr (!half) {
+        float none = 0.0f;                                             // (0 times a sum that is not finite is NaN)
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) none = fmaf(acc[t][i][e], 0.0f, none);
+        if (!__all(none == 0.0f)) {
+            // sixteen rows of x at a time, and their addresses again, which the loop above would otherwise keep in registers
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if (all_finite(acc[t][i])) continue;
+                    int row = threadIdx.x & 15, part = threadIdx.x >> 4 & 3;
+                    asm volatile("" : "+v"(row), "+v"(part));
+                    const int64_t m = m0 + i * 16 + row;
+                    const T *const from = a.x + (m < a.m ? m : a.m - 1) * a.x_stride;
+                    f32x4 exact[1] = {zero4};
+                    for (int32_t b0 = wave * KB; b0 < a.blocks; b0 += kW4Waves * KB) {
+                        Slice<KB, SEGS> s;
+                        load_slice<T, KB, GB>(a, rows, n0, t * 16 + row, b0, part, s);
+                        multiply<T, 1, KB, GB, true>(
+                            a, s, b0,
+                            [&](int b, int) {
+                                return __builtin_bit_cast(frag, in_order(load_x<T>(a, from, (b0 + b) * 32 + part * 8)));
+                            },
+                            [&](int, int) { return zero4; }, exact);
+                    }
+                    take_where_not_finite(acc[t][i], exact[0]);
+                }
+        }
     }
     write_out<T, OUT, MT, TT, RT>(a, sums, acc, n0, m0, wave, lane);
 }
