@@ -13,6 +13,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -45,6 +46,14 @@ def _run(name: str, device: torch.device, *args) -> None:
             rc = _entry(name)(*args, torch.cuda.current_stream().cuda_stream)
     if rc:
         _lib.check(rc, name)
+
+
+def _no_tangent(name: str, *tensors) -> None:
+    """Forward-mode derivatives are refused: a kernel would drop them."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -156,6 +165,7 @@ def _gated_scan(x, gate, offsets, n_rows, h0, reverse):
     _require_rows(x, "x", x.shape, x.dtype, x.device)
     _require_rows(gate, "gate", x.shape, x.dtype, x.device)
     _require(h0, "h0", (n_rows, dim), torch.float32, x.device)
+    _no_tangent("gated_scan", x, gate, h0)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedScan.apply(x, gate, offsets, n_rows, h0, reverse)
     return _scan_forward(x, gate, offsets, n_rows, h0, reverse, False)[:2]
@@ -184,6 +194,7 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
 
 
 def _forward_only(name: str, *tensors) -> None:
+    _no_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -260,7 +271,7 @@ class W4Matrix:
         m, n, k = x.shape[0], self.out_features, self.in_features
         xs = _require_rows(x, "x", (m, k), self.scales.dtype, device)
         _require(bias, "bias", (n,), torch.float32, device)
-        _forward_only("W4Matrix.matvec", x, bias)
+        _forward_only("W4Matrix.matvec", x, bias, self.scales)
         if out_dtype is None:
             out_dtype = x.dtype if out is None else out.dtype
         if out_dtype not in (x.dtype, torch.float32):
@@ -334,7 +345,8 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     elif state is not None:
         raise ValueError("state needs allowed")
     _require(state, "state", (rows,), torch.int32, device)
-    _forward_only("process_logits", logits, bias)
+    _forward_only("process_logits", logits, bias,
+                  *(v for v in (repetition, presence, frequency) if isinstance(v, torch.Tensor)))
     if out_dtype is None:
         out_dtype = logits.dtype if out is None else out.dtype
     if out_dtype not in (logits.dtype, torch.float32):
