@@ -74,6 +74,35 @@ def _require(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, de
         raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {device}")
 
 
+def _require_out(name: str, out: torch.Tensor, *inputs: Optional[torch.Tensor], in_place: bool = True) -> None:
+    """``out``, a matrix, has a place of its own for each element and shares none with an input, unless the two are one
+    and the operator reads each element before it writes it (``in_place``).  What autograd kept of ``out`` is out of date from
+    here on."""
+    rows, cols = out.shape
+    pitch, size = out.stride(0), out.element_size()
+    if rows > 1 and pitch < cols:
+        raise ValueError(f"{name}: rows of the output overlap")
+    first, width = out.data_ptr(), cols * size
+    end = first + (max(rows - 1, 0) * pitch + cols) * size
+    for t in inputs:
+        if t is None or t.numel() == 0 or out.numel() == 0:
+            continue
+        own = t.stride(0) if t.dim() == 2 and t.size(0) > 1 else 0
+        wide = t.size(-1) * t.element_size()
+        at = t.data_ptr()
+        if at >= end or at + ((t.size(0) - 1) * own * t.element_size() if t.dim() == 2 else 0) + wide <= first:
+            continue
+        if in_place and t.dtype is out.dtype and t.shape == out.shape and at == first and (rows <= 1 or own == pitch):
+            continue
+        if rows > 1 and own * t.element_size() == pitch * size:       # columns of one matrix next to each other
+            apart = (at - first) % (pitch * size)
+            if apart >= width and apart + wide <= pitch * size:
+                continue
+        raise ValueError(f"{name}: the output overlaps an input")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _require_floats(t: torch.Tensor, name: str, types=tuple(_DTYPES)) -> None:
     if not t.is_cuda or t.dtype not in types:
         raise ValueError(f"{name} must be on the GPU, of " + ", ".join(str(d) for d in types))
@@ -184,10 +213,12 @@ def gated_step(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
     gs = _require_rows(gate, "gate", shape, dtype, device)
     _require(state, "state", shape, torch.float32, device)
     _require(out_state, "out_state", shape, torch.float32, device)
-    _forward_only("gated_step", x, gate, state)
+    _forward_only("gated_step", x, gate, state, out_state)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if out_state is None:
         out_state = torch.empty_like(y, dtype=torch.float32)
+    else:
+        _require_out("gated_step", out_state, x, gate, state)
     _run("dnatok_gated_step", device, x.data_ptr(), xs, gate.data_ptr(), gs, _DTYPES[dtype], _ptr(state), shape[0], shape[1],
          y.data_ptr(), out_state.data_ptr())
     return y, out_state
@@ -261,7 +292,7 @@ class W4Matrix:
                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``x W^T + bias`` for the few rows of ``x`` [M, K] (or one vector [K]), which has the scales' type:
         one token of each sequence.  ``bias`` is float32 [N]; the result has x's type or ``out_dtype`` =
-        float32.  Without gradients."""
+        float32, and goes to ``out``, which shares no memory with them, if given.  Without gradients."""
         squeeze = x.dim() == 1
         if squeeze:
             x = x.unsqueeze(0)
@@ -271,16 +302,19 @@ class W4Matrix:
         m, n, k = x.shape[0], self.out_features, self.in_features
         xs = _require_rows(x, "x", (m, k), self.scales.dtype, device)
         _require(bias, "bias", (n,), torch.float32, device)
-        _forward_only("W4Matrix.matvec", x, bias, self.scales)
+        _forward_only("W4Matrix.matvec", x, bias, self.scales, out)
         if out_dtype is None:
             out_dtype = x.dtype if out is None else out.dtype
         if out_dtype not in (x.dtype, torch.float32):
             raise ValueError("out_dtype must be x's type or float32")
-        if out is None:
+        given = out is not None
+        if not given:
             out = x.new_empty((m, n), dtype=out_dtype)
         elif squeeze:
             out = out.unsqueeze(0)
         ys = _require_rows(out, "out", (m, n), out_dtype, device)
+        if given:
+            _require_out("W4Matrix.matvec", out, x, bias, in_place=False)
         _run("dnatok_w4_matvec", device, x.data_ptr(), xs, _DTYPES[x.dtype], self.q.data_ptr(), self.q.stride(0),
              self.scales.data_ptr(), _ptr(self.zeros), m, n, k, self._group, _ptr(bias), out.data_ptr(), ys,
              _DTYPES[out_dtype])
@@ -345,15 +379,18 @@ def process_logits(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     elif state is not None:
         raise ValueError("state needs allowed")
     _require(state, "state", (rows,), torch.int32, device)
-    _forward_only("process_logits", logits, bias,
+    _forward_only("process_logits", logits, bias, out,
                   *(v for v in (repetition, presence, frequency) if isinstance(v, torch.Tensor)))
     if out_dtype is None:
         out_dtype = logits.dtype if out is None else out.dtype
     if out_dtype not in (logits.dtype, torch.float32):
         raise ValueError("out_dtype must be the logits' type or float32")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(logits, dtype=out_dtype, memory_format=torch.contiguous_format)
     out_stride = _require_rows(out, "out", (rows, vocab), out_dtype, device)
+    if given:
+        _require_out("process_logits", out, logits, bias)
     repetition = _per_row(repetition, "repetition", rows, device)
     presence = _per_row(presence, "presence", rows, device)
     frequency = _per_row(frequency, "frequency", rows, device)
