@@ -426,14 +426,18 @@ class TokenGrammar:
 
     def __init__(self, transitions, tokens: Sequence[Optional[bytes]], *, accepting: Sequence[int] = (),
                  eos_id: Optional[int] = None, device="cuda"):
-        trans = np.ascontiguousarray(transitions, dtype=np.int32)
+        trans = np.asarray(transitions)
         if trans.ndim != 2 or trans.shape[1] != 256 or trans.shape[0] == 0:
             raise ValueError("transitions must be [S, 256]")
         s, v = trans.shape[0], len(tokens)
         if v == 0:
             raise ValueError("no tokens")
-        if trans.min() < -1 or trans.max() >= s:
-            raise ValueError("transitions lead to states that are not there")
+        if not np.array_equal(trans, np.trunc(trans)) or trans.min() < -1 or trans.max() >= s:
+            raise ValueError("transitions must be whole numbers, and lead to states that are there")
+        trans = trans.astype(np.int32)
+        accepting = list(accepting)
+        if any(not 0 <= a < s for a in accepting):
+            raise ValueError("accepting names states that are not there")
         if eos_id is not None and not 0 <= eos_id < v:
             raise ValueError("eos_id is not in the vocabulary")
         lengths = np.array([0 if t is None else len(t) for t in tokens])
@@ -453,9 +457,12 @@ class TokenGrammar:
         bits = np.zeros((s, -(-v // 32) * 32), dtype=np.uint8)
         bits[:, :v] = state >= 0
         words = np.packbits(bits, axis=1, bitorder="little").view("<u4").view(np.int32)
-        following = np.concatenate([np.where(state < 0, s, state), np.full((1, v), s)]).astype(np.int32)
+        # (a column behind the last token, for what is no token)
+        following = np.full((s + 1, v + 1), s, dtype=np.int32)
+        following[:s, :v] = np.where(state < 0, s, state)
         self.allowed = torch.from_numpy(np.ascontiguousarray(words)).to(device)
-        self.next_state = torch.from_numpy(following).to(device)
+        self._following = torch.from_numpy(following).to(device)
+        self.next_state = self._following[:, :v]
 
     @classmethod
     def from_iupac(cls, pattern: str, tokens: Sequence[Optional[bytes]], *, repeat: bool = False,
@@ -473,6 +480,7 @@ class TokenGrammar:
         return cls(trans, tokens, accepting=[0] if repeat else [n], eos_id=eos_id, device=device)
 
     def advance(self, state: torch.Tensor, token: torch.Tensor) -> torch.Tensor:
-        """The states of rows in ``state`` int32 [B] that took ``token`` [B]; negative states stay."""
+        """The states of rows in ``state`` int32 [B] that took ``token`` [B]; negative states stay.  A token that is not in the
+        vocabulary (-1 for none) is a forbidden one."""
         at = state.clamp(0, self.n_states).long()
-        return torch.where(state < 0, state, self.next_state[at, token.long()])
+        return torch.where(state < 0, state, self._following[at, token.clamp(-1, self.vocab).long()])
