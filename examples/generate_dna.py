@@ -96,7 +96,8 @@ class Generator:
         room = torch.arange(rows + 1, device=ids.device) * width
         penalties = [torch.full((rows,), v, device=ids.device) for v in (repetition, presence, frequency)]
         x, states = model(ids, offsets)
-        x = x[(offsets[1:] - 1).clamp(min=0)].contiguous()
+        # the last token's features of each row; zeros for an empty one
+        x = torch.cat([x.new_zeros((1, self.dim)), x])[torch.where(lengths > 0, offsets[1:], 0)]
         state = torch.zeros(rows, dtype=torch.int32, device=ids.device) if grammar else None
         out = []
         for i in range(steps):
