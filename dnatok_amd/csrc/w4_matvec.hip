@@ -537,10 +537,13 @@ void run_w4(const W4Args<T> &a, hipStream_t s)
         if (a.per_group % 4 == 0) w4_row_kernel<T, OUT, 8, 4><<<grid, 64 * kW4Waves, lds, s>>>(a);
         else if (a.per_group % 2 == 0) w4_row_kernel<T, OUT, 8, 2><<<grid, 64 * kW4Waves, lds, s>>>(a);
         else w4_row_kernel<T, OUT, 8, 1><<<grid, 64 * kW4Waves, lds, s>>>(a);
-    } else if (a.m > 32 && a.n >= 16 * 640) {
-        // weights unpacked once for 64 rows.  61 x 12301 x 2040: 16.2 us, in blocks of 16 rows 20.6; 64 x 32000 x 2048: 45, 63
-        // (before rows of x were spread); with fewer rows of W there are too few workgroups: 64 x 8192 x 8192 51, 40; 48 x 10000 x
-        // 4096 29.5, 26.8; 33 x 8192 x 4096 28, 21
+    } else if (a.m > 32 && (a.n + 63) / 64 * ((a.m + 15) / 16) > 512) {
+        // weights unpacked once for 64 rows, where blocks of 16 rows are more workgroups than run at once, two on each of the 256 CUs.
+        // us in blocks of 16 rows and of 64, bfloat16 in groups of 128: with one round of the former 33 x 10240 x 2048 11.8, 13.9;
+        // 48 x 10240 x 8192 40.6, 43.2; 64 x 8192 x 1024 7.4, 9.7; 64 x 8192 x 8192 40.3, 43.4; with more 33 x 12301 x 1024 10.8,
+        // 9.7; 48 x 12301 x 4096 34.9, 24.1; 64 x 10240 x 512 7.3, 7.4; 64 x 10240 x 2048 16.9, 15.0; 64 x 16384 x 8192 76, 49.
+        // The depth decides nothing but at its ends: 33 x 32000 x 512 12.7, 14.1.  (Rows of x that begin off a multiple of 16
+        // bytes are read number by number, 64 of them as well: 33 x 12301 x 5500 73, 91, but 64 x 12301 x 5500 135, 128.)
         launch_w4<T, OUT, 4, 4, 4>(a, s);
     } else if (a.k > 1024) {
         launch_w4_tiles<T, OUT, 8>(a, s);
