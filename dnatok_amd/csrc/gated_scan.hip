@@ -21,13 +21,21 @@
 // leaves the same for the group, and then the state at the group's end in its place (marked).  A word says by itself
 // whether it is there (a fill kernel has put a pattern that none has), so nothing has to be ordered by a fence.  A tile
 // takes the nearest group in front whose state is there, and runs that state through the groups and then the tiles
-// between, one after the other.  These are the same steps in the same order wherever the state is found and whoever came
-// first, so the result is the same to the last bit.  (With tiles alone, states one by one, a contig's tiles followed each
-// other every 0.16 us and more: 4,000,000 tokens x 64 in 2517 us, in an early form with groups 855, now 534; its bytes take 323.)
+// between, one after the other.  A group's state is the one in front of it run through the group's word in the same one step, so
+// the result is the same to the last bit wherever the state is found and whoever came first.  (With tiles alone, states
+// one by one, a contig's tiles followed each other every 0.16 us and more: 4,000,000 tokens x 64 in 2517 us, in an early form with
+// groups 855, now 523; its bytes take 323.)
 //
-// Bound by memory and by the waits for states.  Measured, bfloat16: 64 rows of 8,192 tokens x 512 forward 394 us with the fill
-// of the words, 4.09 TB/s (a copy 4.76); a contig of 1,000,003 x 256 409; 256 rows of 1,024 x 512 forward and backward 511.
-// Vector issue is busy 0.36 of the time forward and 0.32 backward.  float32, 300 rows x 203: 1649, 2.6 TB/s of the bytes: a
+// Tokens in no row, in front of the first or behind the last one, are spans of their own that give zeros.
+//
+// Rounding: f and k = 1 - f are each right to a few units of themselves (more by the gate's size), so what is small stays right: what a closed gate
+// leaves, what an open one takes.  A wave's tokens and a tile's waves are joined by rounded products of f, 168 tokens at most (264
+// backwards); tile by tile and group by group, where such roundings would become a wrong rate, the smaller of a piece's factor
+// and its complement is carried.  An infinite state stays infinite, and NaN comes only where the formula has it.
+//
+// Bound by memory and by the waits for states.  Measured, bfloat16: 64 rows of 8,192 tokens x 512 forward 413 us with the fill
+// of the words, 3.90 TB/s (a copy 4.76); a contig of 1,000,003 x 256 430; 256 rows of 1,024 x 512 forward and backward 543.
+// Vector issue is busy 0.41 of the time forward and 0.43 backward.  float32, 300 rows x 203: 1794, 2.4 TB/s of the bytes: a
 // slab's piece of a token, 256 bytes, does not begin on a line.
 #include "lm_common.hpp"
 
@@ -564,8 +572,8 @@ struct Strip {
         if constexpr (V * sizeof(T) == 4) {
             uint32_t w;
             __builtin_memcpy(&w, &c, 4);
-            // (2: streamed, not kept in the caches.  64 x 8192 x 512 434 -> 400 us, a training step's backward 342 -> 322.  For
-            // 32 bits between 3 % less and, with rows of 203 floats, whose ends share lines, 5 % more: not used.  Loads
+            // (2: streamed, not kept in the caches.  64 x 8192 x 512 434 -> 400 us, a training step's backward 342 -> 322, both in
+            // an earlier form.  For 32 bits between 3 % less and, with rows of 203 floats, whose ends share lines, 5 % more: not used.  Loads
             // gain less.)
             __builtin_amdgcn_raw_buffer_store_b32(w, rsrc, lane_bytes, offset(i), sizeof(T) == 2 ? 2 : 0);
         } else {
@@ -854,7 +862,7 @@ namespace {
 constexpr int kSteps = 24;                        // tokens that a wave holds in registers
 // Waves to a tile beside the one that looks for the carry.  On 64 rows of 8,192 tokens x 512 (bfloat16), us forward and
 // backward: 24 tokens x 7 waves 411, 691; x 11 432, 632; 16 tokens x 15 476, 651; x 7 506, 724; 32 tokens x 7 472, 691
-// (all before stores were streamed).
+// (all in an earlier form).
 // Small batches differ by 1 us in 15.
 constexpr int kForwardWaves = 7, kBackwardWaves = 11;
 

@@ -461,8 +461,10 @@ int dnatok_gated_step(const void *x, int64_t x_stride, const void *gate, int64_t
  * W[n, k] = (q[n, k] - zero[n, k / group]) scale[n, k / group].  q is uint32[n, weight_stride], eight
  * values to a word, the lowest bits first (what lies behind the k-th is not used); scales
  * [n, ceil(k / group)] are of x's type (bfloat16 or float16); zeros uint8[n, ceil(k / group)] hold
- * 0 .. 15 (NULL: 8 everywhere); group is a multiple of 32; bias float[n] or NULL; y is of x's type or
- * float32.  Sums are held in 32 bits and rounded once. */
+ * 0 .. 15 (NULL: 8 everywhere); group is a multiple of 32, and may be larger than k; bias float[n] or NULL; y is of x's type or
+ * float32.  Sums are held in 32 bits and rounded once at their end (bfloat16: sums of (128 + q) x, from which a multiple of
+ * the sum of x is taken off, so some ten times the rounding of sums of (q - zero) x).  An infinite x gives infinities as the formula
+ * has them.  y must not overlap x or bias. */
 int dnatok_w4_matvec(const void *x, int64_t x_stride, int32_t dtype, const uint32_t *weights, int64_t weight_stride,
                      const void *scales, const uint8_t *zeros, int64_t m, int64_t n, int64_t k, int32_t group,
                      const float *bias, void *y, int64_t y_stride, int32_t y_dtype, void *stream);
