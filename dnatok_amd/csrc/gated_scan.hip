@@ -88,35 +88,36 @@ __device__ __forceinline__ float once_more(float m)
     return m;
 }
 
-// step(i, look) for the S tokens of a wave, forwards or backwards, four at a time: look is a true_type where one of the four has a bit in
-// `looks`.  (The compiler keeps room for both kinds of a part at once, so parts are short.)
-constexpr int kPart = 4;
-template <int S, typename Fn>
+// step(i, look) for the S tokens of a wave, forwards or backwards, PART at a time: look is a true_type where one of a part has a bit in
+// `looks`.  (The compiler keeps room for both kinds of a part at once, so parts are as long as the registers allow: states 4 tokens
+// with two channels to a lane, 8 with one; gradients 12.  300 rows x 203 in float32 1730 us, with parts of 4 throughout 1770;
+// 256 x 1024 x 512 526, 541.)
+template <int S, int PART, typename Fn>
 __device__ __forceinline__ void by_parts(uint64_t looks, Fn step)
 {
-    static_assert(S % kPart == 0, "whole parts");
+    static_assert(S % PART == 0, "whole parts");
 #pragma unroll
-    for (int from = 0; from < S; from += kPart) {
-        if (looks >> from & ((1 << kPart) - 1)) {
+    for (int from = 0; from < S; from += PART) {
+        if (looks >> from & ((1 << PART) - 1)) {
 #pragma unroll
-            for (int i = from; i < from + kPart; ++i) step(i, std::true_type{});
+            for (int i = from; i < from + PART; ++i) step(i, std::true_type{});
         } else {
 #pragma unroll
-            for (int i = from; i < from + kPart; ++i) step(i, std::false_type{});
+            for (int i = from; i < from + PART; ++i) step(i, std::false_type{});
         }
     }
 }
-template <int S, typename Fn>
+template <int S, int PART, typename Fn>
 __device__ __forceinline__ void by_parts_back(uint64_t looks, Fn step)
 {
 #pragma unroll
-    for (int from = S - kPart; from >= 0; from -= kPart) {
-        if (looks >> from & ((1 << kPart) - 1)) {
+    for (int from = S - PART; from >= 0; from -= PART) {
+        if (looks >> from & ((1 << PART) - 1)) {
 #pragma unroll
-            for (int i = from + kPart - 1; i >= from; --i) step(i, std::true_type{});
+            for (int i = from + PART - 1; i >= from; --i) step(i, std::true_type{});
         } else {
 #pragma unroll
-            for (int i = from + kPart - 1; i >= from; --i) step(i, std::false_type{});
+            for (int i = from + PART - 1; i >= from; --i) step(i, std::false_type{});
         }
     }
 }
@@ -170,10 +171,12 @@ struct Axis {
     }
 };
 
-// Where spans start and end among a wave's positions p0 .. p0 + n: spans (in the axis' order), -1 where there is none.
+// Where spans start and end among a wave's positions p0 .. p0 + n: the spans' rows, -1 for tokens in no row, kNoEdge where there is no
+// edge.
+constexpr int32_t kNoEdge = -2;
 template <int S>
 struct Edges {
-    int32_t start[S + 1], end[S + 1];             // [i]: the span whose first position is p0 + i / whose last is p0 + i - 1
+    int32_t start[S + 1], end[S + 1];             // [i]: that whose first position is p0 + i / whose last is p0 + i - 1
 };
 
 // Fills `e` and returns the bits of e.start and e.end that are set, and whether the first or the last span may be here.  empty(row)
@@ -183,7 +186,7 @@ __device__ __forceinline__ bool find_edges(const Axis<REV> &axis, int64_t p0, in
                                            uint64_t &starts, uint64_t &ends, Fn empty)
 {
     static_assert(S + 1 <= 64, "a lane to a position");
-    if (lane <= S) e.start[lane] = e.end[lane] = -1;
+    if (lane <= S) e.start[lane] = e.end[lane] = kNoEdge;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     bool rim = false;
     if (n > 0) {
@@ -197,10 +200,10 @@ __device__ __forceinline__ bool find_edges(const Axis<REV> &axis, int64_t p0, in
                 const int64_t at = axis.at(j);
                 p = at - p0;
                 if (p >= 0 && p <= n) {
-                    if (j > 0 && p > 0 && axis.at(j - 1) < at) e.end[p] = (int32_t)(j - 1);
+                    if (j > 0 && p > 0 && axis.at(j - 1) < at) e.end[p] = (int32_t)axis.row(j - 1);
                     if (j < axis.count()) {
                         const bool none = axis.at(j + 1) == at;
-                        if (!none && p < n) e.start[p] = (int32_t)j;
+                        if (!none && p < n) e.start[p] = (int32_t)axis.row(j);
                         is_empty = none && (p < n || at == axis.r.total);
                     }
                 }
@@ -215,8 +218,8 @@ __device__ __forceinline__ bool find_edges(const Axis<REV> &axis, int64_t p0, in
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int i = lane <= S ? lane : S;
-    starts = __ballot(lane <= S && e.start[i] >= 0);
-    ends = __ballot(lane <= S && e.end[i] >= 0);
+    starts = __ballot(lane <= S && e.start[i] != kNoEdge);
+    ends = __ballot(lane <= S && e.end[i] != kNoEdge);
     return rim;
 }
 
@@ -681,11 +684,11 @@ __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V 
     float A[S][V], H[S][V];
     Run<V> own;
     own.clear();
-    by_parts<S>(looks, [&](int i, auto look) {
+    by_parts<S, V == 1 ? 8 : 4>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
         if (look && (starts >> i & 1)) {
             own.clear();
-            load_row<V>(own.h, a.h0, axis.row(one_row(edges.start[i])), a.dim, c);
+            load_row<V>(own.h, a.h0, one_row(edges.start[i]), a.dim, c);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -707,7 +710,7 @@ __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V 
     if (wave > 0) front.piece().through(c0);
     if (a.states && n > 0) store_floats<V>(a.states + span.p0 / S * a.dim + c, c0);
     const strip ys(a.y, a.dim, span, a.dim);
-    by_parts<S>(looks, [&](int i, auto look) {
+    by_parts<S, V == 1 ? 8 : 4>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
         if (look && (starts >> i & 1)) clear_floats<V>(c0);
         float h[V];
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V 
         for (int v = 0; v < V; ++v) h[v] = fmaf(A[i][v], c0[v], H[i][v]);
         ys.store(i, h);
         if (look && (ends >> (i + 1) & 1) && a.last) {
-            const int64_t row = axis.row(one_row(edges.end[i + 1]));
+            const int32_t row = one_row(edges.end[i + 1]);
             if (row >= 0) store_floats<V>(a.last + row * a.dim + c, h);
         }
     });
@@ -764,13 +767,16 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
     }
     const uint64_t looks = starts | ends >> 1 | ~0ull << n;            // positions at which a step has to look
     const auto final_grad = [&](int i, float (&to)[V]) {
-        load_row<V>(to, a.dlast, axis.row(one_row(edges.end[i + 1])), a.dim, c);
+        load_row<V>(to, a.dlast, one_row(edges.end[i + 1]), a.dim, c);
     };
 
-    float m[S][V];                                                     // the gates
+    // The gates, both numbers of each where there are registers for them: with one channel to a lane.
+    constexpr bool kBoth = V == 1;
+    float m[S][V], fs[kBoth ? S : 1][V];
+    const auto gate_at = [&](int i, int v) { return kBoth ? Gate{fs[kBoth ? i : 0][v], m[i][v]} : gate_from(once_more(m[i][v])); };
     Run<V> own;
     own.clear();
-    by_parts_back<S>(looks, [&](int i, auto look) {
+    by_parts_back<S, 12>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
         if (look && (ends >> (i + 1) & 1)) {
             own.clear();
@@ -779,7 +785,8 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const Gate gate = gate_of(to_float(g[i].v[v]));
-            m[i][v] = one_number(gate);
+            m[i][v] = kBoth ? gate.k : one_number(gate);
+            if (kBoth) fs[kBoth ? i : 0][v] = gate.f;
             own.h[v] = gate.f * (own.h[v] + to_float(dy[i].v[v]));
             own.factor(v, gate);
         }
@@ -798,24 +805,24 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
     if (order > 0) behind.piece().through(carry);
     const strip dxs(a.dx, a.dim, span, a.dim), dgs(a.dgate, a.dim, span, a.dim);
     float from_x[S][V];                                                // h_(t-1) - x_t
-    by_parts<S>(looks, [&](int i, auto look) {
+    by_parts<S, V == 1 ? 8 : 4>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
-        if (look && (starts >> i & 1)) load_row<V>(h, a.h0, axis.row(one_row(edges.start[i])), a.dim, c);
+        if (look && (starts >> i & 1)) load_row<V>(h, a.h0, one_row(edges.start[i]), a.dim, c);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Gate gate = gate_from(m[i][v]);
+            const Gate gate = gate_at(i, v);
             const float xv = to_float(x[i].v[v]);
             from_x[i][v] = h[v] - xv;
             h[v] = fmaf(gate.f, h[v], gate.k * xv);
         }
     });
-    by_parts_back<S>(looks, [&](int i, auto look) {
+    by_parts_back<S, 12>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
         if (look && (ends >> (i + 1) & 1)) final_grad(i, carry);
         float dx[V], dg[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Gate gate = gate_from(once_more(m[i][v]));
+            const Gate gate = gate_at(i, v);
             const float dh = to_float(dy[i].v[v]) + carry[v];
             dx[v] = gate.k * dh;
             dg[v] = dh * from_x[i][v] * (gate.f * gate.k);
@@ -824,7 +831,7 @@ __global__ __launch_bounds__(64 * (W + 1)) void gated_scan_backward_kernel(ScanA
         dxs.store(i, dx);
         dgs.store(i, dg);
         if (look && (starts >> i & 1) && a.dh0) {
-            const int64_t row = axis.row(one_row(edges.start[i]));
+            const int32_t row = one_row(edges.start[i]);
             if (row >= 0) store_floats<V>(a.dh0 + row * a.dim + c, carry);
         }
     });
