@@ -90,7 +90,7 @@ __device__ __forceinline__ float once_more(float m)
 
 // step(i, look) for the S tokens of a wave, forwards or backwards, PART at a time: look is a true_type where one of a part has a bit in
 // `looks`.  (The compiler keeps room for both kinds of a part at once, so parts are as long as the registers allow: states 4 tokens
-// with two channels to a lane, 8 with one; gradients 12.  300 rows x 203 in float32 1730 us, with parts of 4 throughout 1770;
+// with two channels to a lane, 8 with one; gradients and outputs 12.  300 rows x 203 in float32 1730 us, with parts of 4 throughout 1770;
 // 256 x 1024 x 512 526, 541.)
 template <int S, int PART, typename Fn>
 __device__ __forceinline__ void by_parts(uint64_t looks, Fn step)
@@ -710,7 +710,7 @@ __global__ __launch_bounds__(64 * (W + 1)) __attribute__((amdgpu_waves_per_eu(V 
     if (wave > 0) front.piece().through(c0);
     if (a.states && n > 0) store_floats<V>(a.states + span.p0 / S * a.dim + c, c0);
     const strip ys(a.y, a.dim, span, a.dim);
-    by_parts<S, V == 1 ? 8 : 4>(looks, [&](int i, auto look) {
+    by_parts<S, 12>(looks, [&](int i, auto look) {
         if (look && i >= n) return;
         if (look && (starts >> i & 1)) clear_floats<V>(c0);
         float h[V];
