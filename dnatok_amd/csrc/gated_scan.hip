@@ -33,9 +33,9 @@
 // backwards); tile by tile and group by group, where such roundings would become a wrong rate, the smaller of a piece's factor
 // and its complement is carried.  An infinite state stays infinite, and NaN comes only where the formula has it.
 //
-// Bound by memory and by the waits for states.  Measured, bfloat16: 64 rows of 8,192 tokens x 512 forward 413 us with the fill
-// of the words, 3.90 TB/s (a copy 4.76); a contig of 1,000,003 x 256 430; 256 rows of 1,024 x 512 forward and backward 543.
-// Vector issue is busy 0.41 of the time forward and 0.43 backward.  float32, 300 rows x 203: 1794, 2.4 TB/s of the bytes: a
+// Bound by memory and by the waits for states.  Measured, bfloat16: 64 rows of 8,192 tokens x 512 forward 412 us with the fill
+// of the words, 3.91 TB/s (a copy 4.76); a contig of 1,000,003 x 256 428; 256 rows of 1,024 x 512 forward and backward 524.
+// Vector issue is busy 0.41 of the time forward and 0.44 backward.  float32, 300 rows x 203: 1723, 2.5 TB/s of the bytes: a
 // slab's piece of a token, 256 bytes, does not begin on a line.
 #include "lm_common.hpp"
 

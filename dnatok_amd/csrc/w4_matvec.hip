@@ -11,7 +11,7 @@
 // i and i + 4; the columns of x are put into the same order once.  float16 takes 1024 + zero off again, exactly; bfloat16 has no
 // packed subtraction, there the sum over a group of (128 + q) x is corrected by (128 + zero) times the sum of
 // x (from the matrix cores as well, with ones for W).  Every product is exact in 32 bits, sums are 32-bit sums; those of
-// bfloat16 hold numbers some ten times as large as what the correction leaves, so their rounding weighs as much more: 5e-7 of the
+// bfloat16 hold numbers some ten times as large as what the correction leaves, so their rounding weighs as much more: 6e-7 of the
 // result at 4096 x 1024 instead of 6e-8, seen where the result has 32 bits.  Sums that are not finite are done again with q - zero.
 //
 // A workgroup takes TT x 16 rows of W and its eight waves take the columns in slices of KB x 32.  A lane loads four words (32
@@ -19,9 +19,9 @@
 // in one group.  The waves' sums meet in LDS.  A wave holds its slice of x in registers (w4_kernel); a single row of x lies in
 // LDS, ready to be multiplied (w4_row_kernel).
 //
-// Measured, us a call: one row, 32000 x 4096 bfloat16 in groups of 64 18.6 (3.75 TB/s; a copy 4.76); 16 rows, 8192 x 8192
+// Measured, us a call: one row, 32000 x 4096 bfloat16 in groups of 64 18.6 (3.77 TB/s; a copy 4.76); 16 rows, 8192 x 8192
 // float16 in groups of 32 16.2 (2.5 TB/s); 61 rows, 12301 x 2040 15.4; one row, 4096 x 1024
-// 3.9 in the kernel and 8.5 with the host.
+// 3.9 in the kernel and 8.9 with the host.
 #include "lm_common.hpp"
 
 namespace dnatok {
