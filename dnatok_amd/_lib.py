@@ -29,7 +29,25 @@ EXPORTS = [
     "dnatok_normalize_bounds", "dnatok_normalize_rows",
     "dnatok_gated_scan_states_bytes", "dnatok_gated_scan_work_bytes", "dnatok_gated_scan",
     "dnatok_gated_scan_backward", "dnatok_gated_step", "dnatok_w4_matvec", "dnatok_logits_process",
+    "dnatok_linear_attention_states_bytes", "dnatok_linear_attention_work_bytes", "dnatok_linear_attention",
+    "dnatok_linear_attention_backward", "dnatok_linear_attention_step",
+    "dnatok_embedding", "dnatok_embedding_work_bytes", "dnatok_embedding_backward",
+    "dnatok_beam_work_bytes", "dnatok_beam_select", "dnatok_reorder_rows",
 ]
+
+
+class LinearShape(ctypes.Structure):
+    """dnatok_linear_shape of include/dnatok_hip.h."""
+    _fields_ = [("dtype", c_int32), ("reverse", c_int32), ("n_rows", c_int64), ("total", c_int64),
+                ("heads", c_int32), ("kv_heads", c_int32), ("dim_k", c_int32), ("dim_v", c_int32),
+                ("q_token", c_int64), ("q_head", c_int64), ("k_token", c_int64), ("k_head", c_int64),
+                ("v_token", c_int64), ("v_head", c_int64), ("dy_token", c_int64), ("dy_head", c_int64),
+                ("scale", ctypes.c_float), ("with_offsets", c_int32)]
+
+
+class Rows(ctypes.Structure):
+    """dnatok_rows of include/dnatok_hip.h."""
+    _fields_ = [("input", c_void_p), ("out", c_void_p), ("bytes", c_int64), ("in_stride", c_int64), ("out_stride", c_int64)]
 
 
 class NormStep(ctypes.Structure):
@@ -152,6 +170,24 @@ def lib() -> ctypes.CDLL:
     L.dnatok_logits_process.argtypes = [c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                         c_void_p, c_void_p, c_int64, c_int32, c_void_p]
+    L.dnatok_linear_attention_states_bytes.argtypes = [c_void_p]
+    L.dnatok_linear_attention_states_bytes.restype = c_size_t
+    L.dnatok_linear_attention_work_bytes.argtypes = [c_void_p, c_int]
+    L.dnatok_linear_attention_work_bytes.restype = c_size_t
+    L.dnatok_linear_attention.argtypes = [c_void_p] * 11 + [c_size_t, c_void_p]
+    L.dnatok_linear_attention_backward.argtypes = [c_void_p] * 15 + [c_size_t, c_void_p]
+    L.dnatok_linear_attention_step.argtypes = [c_void_p] * 9
+    L.dnatok_embedding.argtypes = [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p, c_void_p,
+                                   c_void_p]
+    L.dnatok_embedding_work_bytes.argtypes = [c_int64, c_int64, c_int64]
+    L.dnatok_embedding_work_bytes.restype = c_size_t
+    L.dnatok_embedding_backward.argtypes = [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p,
+                                            c_void_p, c_void_p, c_size_t, c_void_p]
+    L.dnatok_beam_work_bytes.argtypes = [c_int64, c_int32, c_int64, c_int32]
+    L.dnatok_beam_work_bytes.restype = c_size_t
+    L.dnatok_beam_select.argtypes = [c_void_p, c_int64, c_int32, c_int64, c_int32, c_int64, c_void_p, c_void_p, c_int32, c_int32,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    L.dnatok_reorder_rows.argtypes = [c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p]
     for name in EXPORTS:
         getattr(L, name)          # AttributeError here means the library is stale
     _lib = L

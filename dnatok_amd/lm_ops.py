@@ -1,5 +1,6 @@
-"""Model operators on the rows that the encoders write: a gated linear recurrence (training and
-single steps), products with 4-bit weights, and logits on their way to the choice of a token.
+"""Model operators on the rows that the encoders write: embeddings, a gated linear recurrence and linear attention
+(training and single steps), products with 4-bit weights, logits on their way to the choice of a token, and beam
+search.
 
 Thin torch-tensor wrappers over the C ABI like :mod:`dnatok_amd.encoders`: every call runs HIP kernels of
 libdnatok_hip.so on the current stream of its tensors' device, and none of them synchronises.  The
@@ -230,6 +231,238 @@ def _forward_only(name: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
+
+
+# ---- linear attention -------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=1024)
+def _linear_shape(*fields) -> Tuple["_lib.LinearShape", int]:
+    """A call's sizes, and their address, kept for the next call of the same sizes."""
+    shape = _lib.LinearShape(*fields)
+    return shape, ctypes.addressof(shape)
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, offsets, n_rows, h0, scale, reverse):
+        y, last, states = _linear_forward(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse, True)
+        ctx.save_for_backward(q, k, v, log_decay, offsets, h0, states)
+        ctx.n_rows, ctx.scale, ctx.reverse = n_rows, scale, reverse
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast):
+        q, k, v, log_decay, offsets, h0, states = ctx.saved_tensors
+        device, L = q.device, _lib.lib()
+        total, heads, dim_k = q.shape
+        dim_v = v.shape[2]
+        if dy is None:
+            dy = torch.zeros((1, 1, 1), dtype=q.dtype, device=device).expand(total, heads, dim_v)
+        if dim_v > 1 and dy.stride(2) != 1:
+            dy = dy.contiguous()
+        if dlast is not None:
+            dlast = dlast.contiguous()
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+        dh0 = torch.empty_like(h0) if h0 is not None and ctx.needs_input_grad[6] else None
+        _, shape = _shape_of(q, k, v, ctx.n_rows, ctx.scale, ctx.reverse, offsets, dy)
+        need = L.dnatok_linear_attention_work_bytes(shape, 1)
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _run("dnatok_linear_attention_backward", device, shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+             _ptr(offsets), _ptr(h0), dy.data_ptr(), _ptr(dlast), _ptr(states), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+             _ptr(dh0), _ptr(work), need)
+        return dq, dk, dv, None, None, None, dh0, None, None
+
+
+def _shape_of(q, k, v, n_rows, scale, reverse, offsets, dy=None):
+    a, b, c, d = q.stride(), k.stride(), v.stride(), (0, 0) if dy is None else dy.stride()
+    total, heads, dim_k = q.shape
+    return _linear_shape(_DTYPES[q.dtype], int(reverse), n_rows, total, heads, k.shape[1], dim_k, v.shape[2], a[0], a[1], b[0], b[1],
+                         c[0], c[1], d[0], d[1], scale, int(offsets is not None))
+
+
+def _linear_forward(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse, keep_states):
+    total, heads, dim_k = q.shape
+    device, L, dim_v = q.device, _lib.lib(), v.shape[2]
+    _, shape = _shape_of(q, k, v, n_rows, scale, reverse, offsets)
+    y = torch.empty((total, heads, dim_v), dtype=q.dtype, device=device)
+    last = torch.empty((n_rows, heads, dim_k, dim_v), dtype=torch.float32, device=device)
+    states = None
+    if keep_states:
+        states = torch.empty(L.dnatok_linear_attention_states_bytes(shape) // 4, dtype=torch.float32, device=device)
+    need = L.dnatok_linear_attention_work_bytes(shape, 0)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _run("dnatok_linear_attention", device, shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(offsets),
+         _ptr(h0), y.data_ptr(), last.data_ptr(), _ptr(states), _ptr(work), need)
+    return y, last, states
+
+
+def _require_heads(name: str, q, k, v, log_decay, scale) -> float:
+    """Checks what linear attention takes for each token: q [N, H, Dk], k [N, G, Dk], v [N, G, Dv].  Returns the scale."""
+    if k.dim() != 3 or v.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or v.shape[:2] != k.shape[:2]:
+        raise ValueError("q, k and v must be [.., H, Dk], [.., G, Dk] and [.., G, Dv] of the same tokens")
+    (_, heads, dim_k), (_, kv_heads, dim_v) = q.shape, v.shape
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise ValueError("q's heads must be a multiple of k's and v's")
+    if not 1 <= dim_k <= 128 or not 1 <= dim_v <= 128:
+        raise ValueError("heads have 1 to 128 elements")
+    for what, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype is not q.dtype or t.device != q.device or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{what} must be a {q.dtype} tensor on {q.device} with a head's elements next to each other")
+    _require(log_decay, "log_decay", (heads,), torch.float32, q.device)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no gradient for log_decay")
+    scale = dim_k ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < 3.4e38 or abs(scale) < 1e-37:
+        raise ValueError("scale must be a finite number other than 0")
+    return scale
+
+
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                     offsets: Optional[torch.Tensor] = None, *, h0: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, reverse: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Linear attention with a decay for each head: ``S_t = exp(log_decay) S_(t-1) + k_t v_t^T`` and ``y_t = scale q_t S_t`` in
+    every head of every row.  Returns ``(y, last)``: y [total, H, Dv] in q's type, and the states behind each row's last
+    step, float32 [B, H, Dk, Dv].
+
+    ``q`` [total, H, Dk], ``k`` [total, G, Dk] and ``v`` [total, G, Dv] are packed rows with ``offsets`` int64 [B + 1] as for
+    :func:`gated_scan` (rows may be empty; tokens in no row give zeros, also as gradients), or dense rows [B, T, .., ..]
+    without offsets (copied where they do not lie like packed ones); float32, bfloat16 or float16, the elements of a head
+    next to each other (parts of one projection's output will do).  H is a multiple of G: neighbouring heads share keys and
+    values.  Dk and Dv go up to 128.  ``log_decay`` float32 [H] is at most 0 (-inf: nothing is kept); ``scale`` is
+    Dk ** -0.5 if not given.  ``h0`` float32 [B, H, Dk, Dv] is the state in front of each row, zero if not given; ``reverse``
+    runs rows from their last token to their first.  States and sums are held in 32 bits.  Differentiable (once) with
+    respect to q, k, v and h0."""
+    _require_floats(q, "q")
+    if q.dim() == 4 and offsets is None:
+        if k.dim() != 4 or v.dim() != 4 or k.shape[:2] != q.shape[:2] or v.shape[:2] != q.shape[:2]:
+            raise ValueError("q, k and v must be [.., H, Dk], [.., G, Dk] and [.., G, Dv] of the same tokens")
+        b, t = q.shape[:2]
+        y, last = _linear_attention(*(x.reshape(b * t, x.shape[2], x.shape[3]) for x in (q, k, v)), log_decay, None, b, h0, scale,
+                                    reverse)
+        return y.view(b, t, *y.shape[1:]), last
+    if q.dim() != 3 or offsets is None:
+        raise ValueError("q must be [total, H, Dk] with offsets, or [B, T, H, Dk] without")
+    if offsets.dim() != 1 or offsets.numel() < 1:
+        raise ValueError("offsets must be int64 [B + 1]")
+    _require(offsets, "offsets", offsets.shape, torch.int64, q.device)
+    return _linear_attention(q, k, v, log_decay, offsets, offsets.numel() - 1, h0, scale, reverse)
+
+
+def _linear_attention(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse):
+    scale = _require_heads("linear_attention", q, k, v, log_decay, scale)
+    if n_rows == 0 and q.shape[0]:
+        raise ValueError("tokens without rows")
+    _require(h0, "h0", (n_rows, q.shape[1], q.shape[2], v.shape[2]), torch.float32, q.device)
+    _no_tangent("linear_attention", q, k, v, log_decay, h0)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (h0 is not None and h0.requires_grad)):
+        return _LinearAttention.apply(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse)
+    return _linear_forward(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse, False)[:2]
+
+
+def _extent(t: torch.Tensor) -> Tuple[int, int]:
+    """The first byte of a tensor and the one behind its last."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else first
+
+
+def _require_apart(name: str, out: torch.Tensor, *inputs: Optional[torch.Tensor], same: Optional[torch.Tensor] = None) -> None:
+    """``out``, which is contiguous, shares no memory with the inputs; ``same`` may be all of it, but no part."""
+    first, end = _extent(out)
+    for t in inputs:
+        lo, hi = (0, 0) if t is None else _extent(t)
+        if lo < end and first < hi and not (t is same and lo == first and hi == end and t.is_contiguous()):
+            raise ValueError(f"{name}: the output overlaps an input")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                          state: Optional[torch.Tensor] = None, *, scale: Optional[float] = None,
+                          out_state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One step of :func:`linear_attention` for one token of each row: ``q`` [B, H, Dk], ``k`` [B, G, Dk], ``v`` [B, G, Dv],
+    ``state`` float32 [B, H, Dk, Dv] (zero if not given).  Returns ``(y, new_state)``; ``out_state`` receives the new state
+    and may be ``state`` itself.  Without gradients."""
+    _require_floats(q, "q")
+    if q.dim() != 3:
+        raise ValueError("q must be [B, H, Dk]")
+    device = q.device
+    scale = _require_heads("linear_attention_step", q, k, v, log_decay, scale)
+    shape = (q.shape[0], q.shape[1], q.shape[2], v.shape[2])
+    _require(state, "state", shape, torch.float32, device)
+    _require(out_state, "out_state", shape, torch.float32, device)
+    _forward_only("linear_attention_step", q, k, v, log_decay, state, out_state)
+    y = q.new_empty((shape[0], shape[1], shape[3]))
+    if out_state is None:
+        out_state = torch.empty(shape, dtype=torch.float32, device=device)
+    else:
+        _require_apart("linear_attention_step", out_state, q, k, v, log_decay, state, same=state)
+    _run("dnatok_linear_attention_step", device, _shape_of(q, k, v, shape[0], scale, False, None)[1], q.data_ptr(), k.data_ptr(),
+         v.data_ptr(), log_decay.data_ptr(), _ptr(state), y.data_ptr(), out_state.data_ptr())
+    return y, out_state
+
+
+# ---- embeddings -------------------------------------------------------------------------------
+
+@functools.lru_cache(maxsize=256)
+def _host_float(value: float) -> Tuple[ctypes.c_float, int]:
+    """A number in host memory, and its address."""
+    held = ctypes.c_float(value)
+    return held, ctypes.addressof(held)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.shape, ctx.dtype = scale, weight.shape, weight.dtype
+        return _embed(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (ids,), (vocab, dim), device, L = ctx.saved_tensors, ctx.shape, dy.device, _lib.lib()
+        n = ids.numel()
+        dy = dy.reshape(n, dim)
+        if dim > 1 and dy.stride(1) != 1:
+            dy = dy.contiguous()
+        grad = torch.empty((vocab, dim), dtype=ctx.dtype, device=device)
+        need = L.dnatok_embedding_work_bytes(n, vocab, dim)
+        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _run("dnatok_embedding_backward", device, ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), dy.stride(0),
+             _DTYPES[ctx.dtype], vocab, dim, _host_float(ctx.scale)[1], grad.data_ptr(), _ptr(work), need)
+        return None, grad, None
+
+
+def _embed(ids, weight, scale):
+    vocab, dim = weight.shape
+    y = torch.empty((*ids.shape, dim), dtype=weight.dtype, device=weight.device)
+    _run("dnatok_embedding", weight.device, ids.data_ptr(), ids.element_size(), ids.numel(), weight.data_ptr(), weight.stride(0),
+         _DTYPES[weight.dtype], vocab, dim, _host_float(scale)[1], y.data_ptr())
+    return y
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
+    """``scale weight[ids]``: the rows of ``weight`` [V, D] (float32, bfloat16 or float16) for ``ids`` int32 or int64 of any
+    shape, as the encoders pack or pad them.  An id outside 0 .. V - 1 (-1 for none) gives a row of zeros, and has no part in
+    the gradient.  Differentiable (once) with respect to the weight: its gradient is a 32-bit sum over each id's tokens,
+    rounded once, the same to the last bit from call to call."""
+    _require_floats(weight, "weight")
+    if weight.dim() != 2:
+        raise ValueError("weight must be [V, D]")
+    _require_rows(weight, "weight", weight.shape, weight.dtype, weight.device)
+    if ids.dtype not in (torch.int32, torch.int64) or ids.device != weight.device:
+        raise ValueError(f"ids must be int32 or int64 on {weight.device}")
+    scale = float(scale)
+    if not abs(scale) < 3.4e38:
+        raise ValueError("scale must be a finite number")
+    _no_tangent("embedding", weight)
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(ids, weight, scale)
+    return _embed(ids, weight, scale)
 
 
 # ---- products with 4-bit weights --------------------------------------------------------------
@@ -484,3 +717,89 @@ class TokenGrammar:
         vocabulary (-1 for none) is a forbidden one."""
         at = state.clamp(0, self.n_states).long()
         return torch.where(state < 0, state, self._following[at, token.clamp(-1, self.vocab).long()])
+
+
+# ---- beam search ------------------------------------------------------------------------------
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: Optional[int] = None, *,
+                finished: Optional[torch.Tensor] = None, eos_id: Optional[int] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """One step of a beam search: of all continuations of each group's beams, valued ``score + log_softmax(logits)``, the
+    ``width`` best (as many as there are beams if not given).  Returns ``(scores, tokens, parents)``, float32 and int32
+    [B, width], the best first: ``parents`` are the beams within the group that were continued.
+
+    ``logits`` [B * K, V] are float32, bfloat16 or float16, a group's beams next to each other; ``scores`` float32 [B, K] are
+    the beams' values so far (-inf for a beam that is none).  Equal ones are taken by beam, then by token; values are compared in
+    64 bits, those of one beam by their logits.  ``finished`` bool [B, K] marks beams that have ended: their only
+    continuation is ``eos_id``, at no cost.  Forbidden tokens (-inf, see :func:`process_logits`) and what is NaN are no continuations;
+    where fewer than ``width`` are left, the score is -inf, the token -1 (as :meth:`TokenGrammar.advance` takes it) and the
+    parent the place modulo K.  Up to 128 beams, before and after.  :func:`reorder_rows` moves the beams' states.  Without
+    gradients."""
+    _require_floats(logits, "logits")
+    if logits.dim() != 2 or scores.dim() != 2 or scores.shape[1] == 0 or logits.shape[1] == 0:
+        raise ValueError("logits must be [B * K, V] and scores [B, K]")
+    device, (groups, beams), vocab = logits.device, scores.shape, logits.shape[1]
+    width = beams if width is None else int(width)
+    if not 1 <= width <= 128 or beams > 128:
+        raise ValueError("1 to 128 beams, before and after")
+    stride = _require_rows(logits, "logits", (groups * beams, vocab), logits.dtype, device)
+    _require(scores, "scores", (groups, beams), torch.float32, device)
+    _require(finished, "finished", (groups, beams), torch.bool, device)
+    if finished is not None and (eos_id is None or not 0 <= eos_id < vocab):
+        raise ValueError("finished needs an eos_id in the vocabulary")
+    _forward_only("beam_select", logits, scores)
+    new = torch.empty((groups, width), dtype=torch.float32, device=device)
+    tokens, parents = (torch.empty((groups, width), dtype=torch.int32, device=device) for _ in range(2))
+    need = _lib.lib().dnatok_beam_work_bytes(groups, beams, vocab, width)
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _run("dnatok_beam_select", device, logits.data_ptr(), stride, _DTYPES[logits.dtype], groups, beams, vocab, scores.data_ptr(),
+         _ptr(finished), eos_id if finished is not None else 0, width, new.data_ptr(), tokens.data_ptr(), parents.data_ptr(), _ptr(work),
+         need)
+    return new, tokens, parents
+
+
+def reorder_rows(tensors: Sequence[torch.Tensor], parents: torch.Tensor, *,
+                 out: Optional[Sequence[torch.Tensor]] = None) -> list:
+    """The rows of ``tensors``, each [B * K, ..] of any type (states of the recurrences, histories), in the order of the beams
+    that :func:`beam_select` chose: row ``b * W + j`` of a result is row ``b * K + parents[b, j]``; ``parents`` int32 [B, W].
+    A parent that is no beam gives zeros.  Rows are contiguous; ``out`` receives the results and shares no memory with
+    the tensors, or with itself.  Without gradients."""
+    tensors = list(tensors)
+    if parents.dim() != 2 or not parents.is_cuda:
+        raise ValueError("parents must be int32 [B, W] on the GPU")
+    device, (groups, width) = parents.device, parents.shape
+    _require(parents, "parents", (groups, width), torch.int32, device)
+    given = out is not None
+    out = list(out) if given else []
+    if given and len(out) != len(tensors):
+        raise ValueError("out must have as many tensors")
+    if not tensors:
+        return out
+    beams = None
+    for t in tensors:
+        if t.dim() < 1 or t.device != device or t.is_complex() or not t[:1].is_contiguous():
+            raise ValueError(f"tensors must be [B * K, ..] on {device} with contiguous rows")
+        here = t.shape[0] // groups if groups else 1
+        if (beams is not None and here != beams) or here * groups != t.shape[0]:
+            raise ValueError("tensors must have as many rows as there are beams")
+        beams = here
+    if groups * width and not beams:
+        raise ValueError("no beams to choose from")
+    _forward_only("reorder_rows", *tensors, *out)
+    if given:
+        for t, o in zip(tensors, out):
+            _require(o, "out", (groups * width, *t.shape[1:]), t.dtype, device)
+        for i, o in enumerate(out):
+            _require_apart("reorder_rows", o, parents, *tensors, *out[:i])
+    else:
+        out = [torch.empty((groups * width, *t.shape[1:]), dtype=t.dtype, device=device) for t in tensors]
+    if groups * width == 0:
+        return out
+    rows = (_lib.Rows * len(tensors))()
+    for r, t, o in zip(rows, tensors, out):
+        size = t.element_size()
+        r.input, r.out = t.data_ptr(), o.data_ptr()
+        r.bytes = r.out_stride = t.numel() // t.shape[0] * size
+        r.in_stride = t.stride(0) * size
+    _run("dnatok_reorder_rows", device, ctypes.addressof(rows), len(tensors), parents.data_ptr(), groups, beams, width)
+    return out

@@ -487,6 +487,80 @@ int dnatok_logits_process(const void *logits, int64_t logits_stride, int32_t dty
                           int64_t n_states, const int32_t *state, void *out, int64_t out_stride, int32_t out_dtype,
                           void *stream);
 
+/* Linear attention with a decay for each head, over packed rows:
+ *   T_t = g T_(t-1) + k_t v_t^T,  y_t = scale q_t T_t,  g = exp(log_decay)
+ * q is [total, heads, dim_k], k [total, kv_heads, dim_k] and v [total, kv_heads, dim_v] (heads a multiple of kv_heads: so many
+ * neighbouring heads share keys and values); y is [total, heads, dim_v], back to back; all of `dtype`, dims up to 128, a head's
+ * elements next to each other, strides in elements between tokens and between heads.  log_decay float[heads] is at most 0
+ * (-inf: nothing is kept).  Rows, offsets and reverse are those of dnatok_gated_scan; so is what happens to tokens in no row.  h0
+ * float[n_rows, heads, dim_k, dim_v] (NULL: zeros) is T in front of a row's first step, last (NULL allowed) receives T behind its last
+ * one.  A row's y depends on no token behind it, also where that holds infinities or NaN.  states (NULL allowed) receives what the
+ * backward pass needs, dnatok_linear_attention_states_bytes(); work is the call's own space,
+ * dnatok_linear_attention_work_bytes(), 16-byte aligned. */
+typedef struct dnatok_linear_shape {
+    int32_t dtype, reverse;
+    int64_t n_rows, total;
+    int32_t heads, kv_heads, dim_k, dim_v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int64_t dy_token, dy_head;         /* backward pass only */
+    float scale;                       /* finite and not 0 */
+    int32_t with_offsets;              /* whether the call will have offsets (for the sizes of states and work) */
+} dnatok_linear_shape;
+
+size_t dnatok_linear_attention_states_bytes(const dnatok_linear_shape *shape_h);
+size_t dnatok_linear_attention_work_bytes(const dnatok_linear_shape *shape_h, int backward);
+int dnatok_linear_attention(const dnatok_linear_shape *shape_h, const void *q, const void *k, const void *v, const float *log_decay,
+                            const int64_t *offsets, const float *h0, void *y, float *last, float *states, void *work,
+                            size_t work_bytes, void *stream);
+
+/* Gradients of the same call: dy [total, heads, dim_v] of `dtype` and dlast float[n_rows, heads, dim_k, dim_v] (NULL: zeros) are
+ * those of y and last; dq, dk and dv, back to back in q's, k's and v's shapes, and dh0 (NULL allowed) are
+ * written.  The decays have no gradient. */
+int dnatok_linear_attention_backward(const dnatok_linear_shape *shape_h, const void *q, const void *k, const void *v,
+                                     const float *log_decay, const int64_t *offsets, const float *h0, const void *dy,
+                                     const float *dlast, const float *states, void *dq, void *dk, void *dv, float *dh0, void *work,
+                                     size_t work_bytes, void *stream);
+
+/* One step for one token of each row: q, k, v and y as above with n_rows in total's place; state (NULL: zeros) and new_state
+ * float[n_rows, heads, dim_k, dim_v], which may be the same buffer. */
+int dnatok_linear_attention_step(const dnatok_linear_shape *shape_h, const void *q, const void *k, const void *v,
+                                 const float *log_decay, const float *state, void *y, float *new_state, void *stream);
+
+/* Rows of an embedding: y[t] = scale weight[ids[t]], [n, dim] of `dtype`, back to back; ids of 4 or 8 bytes; an id outside 0 ..
+ * vocab - 1 gives a row of zeros.  scale_h points to host memory. */
+int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, const void *weight, int64_t weight_stride, int32_t dtype,
+                     int64_t vocab, int64_t dim, const float *scale_h, void *y, void *stream);
+
+/* Its gradient: grad[v] = scale (sum of dy[t] over the tokens t of id v), [vocab, dim] of `dtype`, zeros for ids that do not
+ * occur.  Sums are 32-bit sums in an order that depends on the ids alone, so equal calls give equal bits.  work:
+ * dnatok_embedding_work_bytes(), 16-byte aligned. */
+size_t dnatok_embedding_work_bytes(int64_t n, int64_t vocab, int64_t dim);
+int dnatok_embedding_backward(const void *ids, int32_t id_bytes, int64_t n, const void *dy, int64_t dy_stride, int32_t dtype,
+                              int64_t vocab, int64_t dim, const float *scale_h, void *grad, void *work, size_t work_bytes,
+                              void *stream);
+
+/* One step of a beam search: of the beams * vocab continuations of each group, valued score + log softmax(logits), the `width`
+ * best in falling order.  logits [groups * beams, vocab]; scores float[groups, beams]; out_scores float, tokens and parents (the beam
+ * within the group) int32 [groups, width].  A beam's continuations are in the order of their logits, equal ones by token; between
+ * beams the value in 64 bits decides, then the lower beam.  finished uint8[groups, beams] (NULL: none) marks beams whose only
+ * continuation is `eos`, at no cost.  Continuations of value -inf or NaN, and beams whose logits have no finite log-sum, give none;
+ * where fewer than `width` are left, the score is -inf, the token -1 and the parent the place modulo beams.  At most 128
+ * beams, before and after.  work: dnatok_beam_work_bytes(), 16-byte aligned. */
+size_t dnatok_beam_work_bytes(int64_t groups, int32_t beams, int64_t vocab, int32_t width);
+int dnatok_beam_select(const void *logits, int64_t logits_stride, int32_t dtype, int64_t groups, int32_t beams, int64_t vocab,
+                       const float *scores, const uint8_t *finished, int32_t eos, int32_t width, float *out_scores,
+                       int32_t *tokens, int32_t *parents, void *work, size_t work_bytes, void *stream);
+
+/* Rows of state in the order of a step's beams, for n tensors of any type at once (tensors_h: host memory): row g * width + j of
+ * `out` is row g * beams + parents[g, j] of `in`, zeros for a parent that is no beam.  Sizes and strides in bytes. */
+typedef struct dnatok_rows {
+    const void *in;
+    void *out;
+    int64_t bytes, in_stride, out_stride;
+} dnatok_rows;
+int dnatok_reorder_rows(const dnatok_rows *tensors_h, int32_t n, const int32_t *parents, int64_t groups, int32_t beams,
+                        int32_t width, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
