@@ -2,48 +2,415 @@
 // t of id v.  An id outside the table stands for no row: zeros, and no part of a gradient.
 #include "lm_common.hpp"
 
+#include <utility>
+
 namespace dnatok {
 
-template <typename T, typename ID>
-__global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, const T *weight, int64_t w_stride, int64_t vocab,
-                                                    int64_t dim, float scale, T *y)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Sixteen bytes of a row of `dim` elements from element `at` on, at any alignment; zeros behind the row's end.
+template <typename T> struct Words {
+    static constexpr int kCount = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(kCount)));
+    typedef float floats __attribute__((ext_vector_type(kCount)));
+};
+template <typename T> __device__ __forceinline__ typename Words<T>::type load_words(const T *row, int64_t at, int64_t dim)
 {
-    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
-        const int64_t id = ids[t];
-        const bool known = id >= 0 && id < vocab;
-        for (int64_t c = threadIdx.x; c < dim; c += 256)
-            y[t * dim + c] = from_float<T>(known ? scale * to_float(weight[id * w_stride + c]) : 0.0f);
+    typename Words<T>::type v{};
+    if (at + Words<T>::kCount <= dim) {
+        __builtin_memcpy(&v, row + at, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Words<T>::kCount; ++i)
+            if (at + i < dim) v[i] = row[at + i];
+    }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store_words(T *row, int64_t at, int64_t dim, typename Words<T>::type v)
+{
+    if (at + Words<T>::kCount <= dim) {
+        __builtin_memcpy(row + at, &v, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Words<T>::kCount; ++i)
+            if (at + i < dim) row[at + i] = v[i];
     }
 }
 
-// A workgroup to a row of the gradient: it looks through all ids.
+// ---- rows for ids --------------------------------------------------------------------------------------
+
+constexpr int kEmbedAhead = 8;                     // rows that a wave has under way
+
+// A wave copies a run of tokens' rows, sixteen bytes to a lane.
 template <typename T, typename ID>
-__global__ __launch_bounds__(256) void embed_grad_kernel(const ID *ids, int64_t n, const T *dy, int64_t dy_stride, int64_t dim,
-                                                         float scale, T *grad)
+__global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, int32_t run, const T *weight, int64_t w_stride,
+                                                    int64_t vocab, int64_t dim, float scale, T *y)
 {
-    __shared__ int found[4], list[256];
-    const int64_t id = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t c0 = 0; c0 < dim; c0 += 256) {
-        const int64_t c = c0 + threadIdx.x;
-        float sum = 0.0f;
-        for (int64_t t0 = 0; t0 < n; t0 += 256) {
-            const bool here = t0 + threadIdx.x < n && (int64_t)ids[t0 + threadIdx.x] == id;
-            const uint64_t mask = __ballot(here);
-            if (lane == 0) found[wave] = __popcll(mask);
-            __syncthreads();
-            int at = 0, all = 0;
-            for (int w = 0; w < 4; ++w) {
-                at += w < wave ? found[w] : 0;
-                all += found[w];
-            }
-            if (here) list[at + __popcll(mask & ((1ull << lane) - 1))] = threadIdx.x;
-            __syncthreads();
-            if (c < dim)
-                for (int i = 0; i < all; ++i) sum += to_float(dy[(t0 + list[i]) * dy_stride + c]);
-            __syncthreads();
+    typedef Words<T> W;
+    const int lane = threadIdx.x & 63;
+    const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * run;
+    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    for (int64_t t0 = first; t0 < first + run && t0 < n; t0 += kEmbedAhead) {
+        const int here = n - t0 < kEmbedAhead ? (int)(n - t0) : kEmbedAhead;
+        int64_t mine = lane < here ? (int64_t)ids[t0 + lane] : -1;
+        if (mine < 0 || mine >= vocab) mine = -1;
+        const int32_t low = (int32_t)mine;         // (below 2^31, or -1)
+        typename W::type v[kEmbedAhead];
+#pragma unroll
+        for (int i = 0; i < kEmbedAhead; ++i) {
+            const int32_t id = __builtin_amdgcn_readlane(low, i);
+            v[i] = typename W::type{};
+            if (id >= 0 && at < dim) v[i] = load_words(weight + id * w_stride, at, dim);
         }
-        if (c < dim) grad[id * dim + c] = from_float<T>(scale * sum);
+#pragma unroll
+        for (int i = 0; i < kEmbedAhead; ++i) {
+            if (i >= here || at >= dim) break;
+            // (a row of no id is zeros whatever the scale is)
+            store_words(y + (t0 + i) * dim, at, dim,
+                        __builtin_convertvector(__builtin_convertvector(v[i], typename W::floats) * scale, typename W::type));
+        }
     }
+}
+
+// ---- tokens sorted by id -----------------------------------------------------------------------------
+
+// Keys are ids, those outside the table the number behind its last row.  A pass sorts by up to eight of their bits: a workgroup
+// counts its tile's digits, a scan gives each tile its place for each digit, and a workgroup writes its tile there, the tokens of one
+// digit in their order.  So tokens of one id stay in their order, and a sum over them is the same in every call.
+constexpr int kSortTile = 4096, kSortThreads = 256, kSortWaves = kSortThreads / 64, kDigits = 256;
+constexpr int kSmallSort = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+
+struct Token {
+    uint32_t key, at;
+};
+
+template <typename ID> __device__ __forceinline__ uint32_t key_of(ID id, uint32_t vocab)
+{
+    return id >= 0 && (uint64_t)id < vocab ? (uint32_t)id : vocab;
+}
+// The lanes with this lane's digit.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool here)
+{
+    uint64_t same = __ballot(here);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t one = __ballot(digit >> b & 1);
+        same &= digit >> b & 1 ? one : ~one;
+    }
+    return same;
+}
+
+template <typename ID>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
+                                                                  int shift, int bits, uint32_t *counts)
+{
+    __shared__ uint32_t count[kDigits];
+    for (int i = threadIdx.x; i < kDigits; i += kSortThreads) count[i] = 0;
+    __syncthreads();
+    const uint32_t first = blockIdx.x * kSortTile, mask = (1u << bits) - 1;
+    const int lane = threadIdx.x & 63;
+    for (uint32_t i = first + threadIdx.x; i - threadIdx.x < first + kSortTile && i - threadIdx.x < n; i += kSortThreads) {
+        const bool here = i < n;
+        const uint32_t digit = here ? (ids ? key_of(ids[i], vocab) : tokens[i].key) >> shift & mask : 0;
+        const uint64_t same = same_digit(digit, bits, here);
+        if (here && (same & ((1ull << lane) - 1)) == 0) atomicAdd(&count[digit], (uint32_t)__popcll(same));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= (int)mask; i += kSortThreads) counts[(size_t)i * gridDim.x + blockIdx.x] = count[i];
+}
+
+// A workgroup to a digit: its tiles' counts become what lies in front of them, and their sum is left in totals.
+__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t *counts, uint32_t tiles, uint32_t *totals)
+{
+    __shared__ uint32_t part[4];
+    uint32_t *mine = counts + (size_t)blockIdx.x * tiles;
+    uint32_t before = 0;
+    for (uint32_t t0 = 0; t0 < tiles; t0 += 256) {
+        const uint32_t t = t0 + threadIdx.x, v = t < tiles ? mine[t] : 0;
+        const uint32_t upto = wave_inclusive_sum_u32(v);
+        if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = upto;
+        __syncthreads();
+        uint32_t front = before;
+        for (unsigned w = 0; w < threadIdx.x >> 6; ++w) front += part[w];
+        if (t < tiles) mine[t] = front + upto - v;
+        before += part[0] + part[1] + part[2] + part[3];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) totals[blockIdx.x] = before;
+}
+
+template <typename ID>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
+                                                                  int shift, int bits, const uint32_t *counts, const uint32_t *totals,
+                                                                  Token *out)
+{
+    __shared__ uint32_t place[kSortWaves][kDigits], part[4];
+    constexpr int kPerLane = kSortTile / kSortThreads;
+    const uint32_t mask = (1u << bits) - 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) place[0][i] = 0;
+    __syncthreads();
+    // a wave has neighbouring tokens, 64 at a time
+    const uint32_t first = blockIdx.x * kSortTile + wave * (kSortTile / kSortWaves);
+    uint32_t key[kPerLane], at[kPerLane];
+    uint64_t same[kPerLane];
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+        const uint32_t i = first + j * 64 + lane;
+        at[j] = i;
+        key[j] = 0;
+        if (i < n) {
+            if (ids) {
+                key[j] = key_of(ids[i], vocab);
+            } else {
+                const Token t = tokens[i];
+                key[j] = t.key;
+                at[j] = t.at;
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+        const bool here = first + j * 64 + lane < n;
+        const uint32_t digit = key[j] >> shift & mask;
+        same[j] = same_digit(digit, bits, here);
+        if (here && (same[j] & ((1ull << lane) - 1)) == 0) atomicAdd(&place[wave][digit], (uint32_t)__popcll(same[j]));
+    }
+    __syncthreads();
+    {   // the digits' places: in front of all of them, of the tile, of the waves
+        const uint32_t d = threadIdx.x, all = d <= mask ? totals[d] : 0;
+        const uint32_t upto = wave_inclusive_sum_u32(all);
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        uint32_t from = upto - all;
+        for (int w = 0; w < wave; ++w) from += part[w];
+        if (d <= mask) {
+            from += counts[(size_t)d * gridDim.x + blockIdx.x];
+            for (int w = 0; w < kSortWaves; ++w) {
+                const uint32_t here = place[w][d];
+                place[w][d] = from;
+                from += here;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+        const bool here = first + j * 64 + lane < n;
+        const uint32_t digit = key[j] >> shift & mask;
+        const uint64_t before = same[j] & ((1ull << lane) - 1);
+        const uint32_t from = here ? place[wave][digit] : 0;
+        __builtin_amdgcn_wave_barrier();
+        if (here) {
+            out[from + __popcll(before)] = Token{key[j], at[j]};
+            if (before == 0) place[wave][digit] = from + __popcll(same[j]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Up to kSmallSort tokens in one workgroup: the same passes in LDS.
+template <typename ID>
+__global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(const ID *ids, uint32_t n, uint32_t vocab, int passes, int bits,
+                                                                   Token *out)
+{
+    __shared__ uint32_t place[kSmallWaves][kDigits], part[kSmallWaves];
+    __shared__ Token token[kSmallSort];
+    constexpr int kPerLane = kSmallSort / kSmallThreads;
+    const uint32_t mask = (1u << bits) - 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t each = ((n + kSmallThreads - 1) / kSmallThreads) * 64, first = wave * each;
+    for (uint32_t i = threadIdx.x; i < n; i += kSmallThreads) token[i] = Token{key_of(ids[i], vocab), i};
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        for (int i = threadIdx.x; i < kSmallWaves * kDigits; i += kSmallThreads) place[0][i] = 0;
+        __syncthreads();
+        Token mine[kPerLane];
+        uint64_t same[kPerLane];
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) {
+            const uint32_t i = first + j * 64 + lane;
+            const bool here = (uint32_t)j * 64 < each && i < n;
+            mine[j] = here ? token[i] : Token{0, 0};
+            const uint32_t digit = mine[j].key >> shift & mask;
+            same[j] = same_digit(digit, bits, here);
+            if (here && (same[j] & ((1ull << lane) - 1)) == 0) atomicAdd(&place[wave][digit], (uint32_t)__popcll(same[j]));
+        }
+        __syncthreads();
+        uint32_t all = 0;
+        if (threadIdx.x < kDigits)
+            for (int w = 0; w < kSmallWaves; ++w) all += place[w][threadIdx.x];
+        const uint32_t upto = wave_inclusive_sum_u32(all);
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        if (threadIdx.x < kDigits) {
+            uint32_t from = upto - all;
+            for (int w = 0; w < wave; ++w) from += part[w];
+            for (int w = 0; w < kSmallWaves; ++w) {
+                const uint32_t here = place[w][threadIdx.x];
+                place[w][threadIdx.x] = from;
+                from += here;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) {
+            const bool here = (uint32_t)j * 64 < each && first + j * 64 + lane < n;
+            const uint32_t digit = mine[j].key >> shift & mask;
+            const uint64_t before = same[j] & ((1ull << lane) - 1);
+            const uint32_t from = here ? place[wave][digit] : 0;
+            __builtin_amdgcn_wave_barrier();
+            if (here) {
+                token[from + __popcll(before)] = mine[j];
+                if (before == 0) place[wave][digit] = from + __popcll(same[j]);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += kSmallThreads) out[i] = token[i];
+}
+
+// ---- sums over the tokens of an id -------------------------------------------------------------------
+
+constexpr int kGradAhead = 8;                      // rows of dy that a wave has under way
+constexpr int kZeroRows = 64;                      // rows of the gradient that a wave looks at for ids that do not occur
+
+struct GradArgs {
+    const Token *tokens;
+    uint32_t n, vocab, tiles;
+    int32_t run;                                   // tokens of a tile, a power of two
+    const void *dy;
+    int64_t dy_stride, dim;
+    float scale;
+    void *grad;
+    float *parts;                                  // [tiles, 2, dim]: of the runs at a tile's begin and end that go on elsewhere
+};
+
+// The first token whose key is not below `key`.
+__device__ __forceinline__ uint32_t first_of(const Token *tokens, uint32_t n, uint32_t key)
+{
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (tokens[mid].key < key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// A wave to a tile of the sorted tokens and 64 x 16 bytes of their rows: it adds up runs of one id.  A run inside the tile is a
+// row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts.  Further waves clear the
+// rows of ids that do not occur.
+template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a)
+{
+    typedef Words<T> W;
+    const int lane = threadIdx.x & 63;
+    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6);
+    T *grad = (T *)a.grad;
+    if (tile >= (a.tiles + 3) / 4 * 4) {
+        const uint32_t row = (tile - (a.tiles + 3) / 4 * 4) * kZeroRows + lane;
+        bool empty = row < a.vocab;
+        if (empty) {
+            const uint32_t i = first_of(a.tokens, a.n, row);
+            empty = i == a.n || a.tokens[i].key != row;
+        }
+        uint64_t rows = __ballot(empty);
+        while (rows) {
+            const int i = __builtin_ctzll(rows);
+            rows &= rows - 1;
+            if (at < a.dim) store_words(grad + (int64_t)(row - lane + i) * a.dim, at, a.dim, typename W::type{});
+        }
+        return;
+    }
+    if (tile >= a.tiles) return;
+    const uint32_t begin = tile * a.run, end = a.n - begin < (uint32_t)a.run ? a.n : begin + a.run;
+    const uint32_t front = begin ? a.tokens[begin - 1].key : ~0u, back = end < a.n ? a.tokens[end].key : ~0u;
+    typename W::floats sum{};
+    uint32_t key = a.tokens[begin].key;
+    bool from_front = key == front;
+    const auto finish = [&](bool goes_on) {
+        if (key >= a.vocab || at >= a.dim) return;
+        if (from_front || goes_on) {
+            float *part = a.parts + ((int64_t)tile * 2 + !from_front) * a.dim;
+#pragma unroll
+            for (int i = 0; i < W::kCount; ++i)
+                if (at + i < a.dim) part[at + i] = sum[i];
+        } else {
+            store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
+        }
+    };
+    for (uint32_t t0 = begin; t0 < end; t0 += 64) {
+        const uint32_t mine_at = t0 + lane < end ? t0 + lane : end - 1;
+        const Token mine = a.tokens[mine_at];
+        for (int j0 = 0; j0 < 64 && t0 + j0 < end; j0 += kGradAhead) {
+            typename W::type v[kGradAhead];
+#pragma unroll
+            for (int i = 0; i < kGradAhead; ++i) {
+                const uint32_t row = __builtin_amdgcn_readlane(mine.at, j0 + i);
+                v[i] = typename W::type{};
+                if (at < a.dim) v[i] = load_words((const T *)a.dy + (int64_t)row * a.dy_stride, at, a.dim);
+            }
+#pragma unroll
+            for (int i = 0; i < kGradAhead; ++i) {
+                if (t0 + j0 + i >= end) break;
+                const uint32_t next = __builtin_amdgcn_readlane(mine.key, j0 + i);
+                if (next != key) {
+                    finish(false);
+                    key = next;
+                    from_front = false;
+                    sum = typename W::floats{};
+                }
+                sum += __builtin_convertvector(v[i], typename W::floats);
+            }
+        }
+    }
+    finish(key == back);
+}
+
+// A run that begins in one tile and ends in another: its parts, added up by eight waves and then in their order.
+constexpr int kJoinWaves = 8;
+template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(GradArgs a)
+{
+    typedef Words<T> W;
+    __shared__ typename W::floats part[kJoinWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t tile = blockIdx.x, end = (tile + 1) * (uint32_t)a.run;
+    if (end >= a.n) return;
+    const uint32_t key = a.tokens[end].key;
+    if (key >= a.vocab || a.tokens[end - 1].key != key) return;
+    const uint32_t begin = tile * (uint32_t)a.run;
+    // (the run's first tile does it: it begins there, behind the tile's begin or at it with another id in front)
+    if (a.tokens[begin].key == key && begin && a.tokens[begin - 1].key == key) return;
+    const uint32_t last = (first_of(a.tokens, a.n, key + 1) - 1) / (uint32_t)a.run;
+    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    typename W::floats sum{};
+    const auto piece = [&](uint32_t t) {
+        typename W::floats v{};
+        if (t <= last && at < a.dim) {
+            const float *p = a.parts + ((int64_t)t * 2 + (t == tile)) * a.dim;
+            if (at + W::kCount <= a.dim) {
+                __builtin_memcpy(&v, p + at, sizeof(v));
+            } else {
+#pragma unroll
+                for (int i = 0; i < W::kCount; ++i)
+                    if (at + i < a.dim) v[i] = p[at + i];
+            }
+        }
+        return v;
+    };
+    for (uint32_t t = tile + wave; t <= last; t += kJoinWaves * 4) {
+        typename W::floats v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = piece(t + i * kJoinWaves);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += v[i];
+    }
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave || at >= a.dim) return;
+    for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
+    store_words((T *)a.grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
 }
 
 }  // namespace dnatok
@@ -58,9 +425,13 @@ static int check_embedding(const char *who, int32_t id_bytes, int64_t n, int64_t
     EMBED_REQUIRE(dtype == DNATOK_F32 || dtype == DNATOK_BF16 || dtype == DNATOK_F16, "unknown element type");
     EMBED_REQUIRE(n >= 0 && vocab >= 0 && dim >= 0, "bad size");
     EMBED_REQUIRE(stride >= 0, "negative stride");
-    DNATOK_REQUIRE(n < (1ll << 31) && vocab < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: at most 2^31 tokens and rows", who);
+    DNATOK_REQUIRE(n < (1ll << 31) && vocab < (1ll << 31) - 1 && dim <= (1ll << 22), DNATOK_E_TOO_LARGE,
+                   "%s: at most 2^31 tokens and rows of 2^22 elements", who);
     return DNATOK_OK;
 }
+
+// Blocks of 64 x 16 bytes of a row.
+static int64_t blocks_of(int64_t dim, int64_t size) { return (dim * size + 1023) / 1024; }
 
 template <typename Fn> static void with_ids(int32_t id_bytes, Fn fn)
 {
@@ -80,15 +451,75 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
         using T = decltype(t);
         with_ids(id_bytes, [&](auto i) {
             using ID = decltype(i);
-            embed_kernel<T, ID><<<(unsigned)(n < 65536 ? n : 65536), 256, 0, (hipStream_t)stream>>>(
-                (const ID *)ids, n, (const T *)weight, weight_stride, vocab, dim, scale, (T *)y);
+            // runs of a multiple of kEmbedAhead tokens, some 16,384 waves where there are so many
+            const int64_t blocks = blocks_of(dim, sizeof(T)), waves = 16384 / blocks + 1;
+            int64_t run = (n + waves - 1) / waves;
+            run = (run + kEmbedAhead - 1) / kEmbedAhead * kEmbedAhead;
+            embed_kernel<T, ID><<<dim3((unsigned)((n + run * 4 - 1) / (run * 4)), (unsigned)blocks), 256, 0, (hipStream_t)stream>>>(
+                (const ID *)ids, n, (int32_t)run, (const T *)weight, weight_stride, vocab, dim, scale, (T *)y);
         });
     });
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
 }
 
-extern "C" size_t dnatok_embedding_work_bytes(int64_t n, int64_t vocab, int64_t dim) { return 0; }
+// What the backward pass needs besides its arguments: tokens sorted by id (twice, where they go from one place to the other), counts of
+// digits, and parts of sums.
+struct GradPlan {
+    uint32_t tiles, sort_tiles;
+    int32_t run, passes, bits;
+    size_t other, counts, totals, parts, bytes;    // offsets
+};
+static GradPlan plan_of(int64_t n, int64_t vocab, int64_t dim)
+{
+    GradPlan p{};
+    int bits = 1;
+    while ((vocab >> bits) != 0) ++bits;           // (keys go up to vocab itself)
+    p.passes = (bits + 7) / 8;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    p.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
+    // tiles as long as leaves some 4,096 waves; shorter ones write more parts of sums, longer ones leave CUs without work
+    const int64_t blocks = blocks_of(dim, 2);
+    p.run = 16;
+    while (p.run < (1 << 20) && n / p.run * blocks > 4096) p.run *= 2;
+    p.tiles = (uint32_t)((n + p.run - 1) / p.run);
+    const bool small = n <= kSmallSort;
+    const auto place = [&](size_t bytes) {
+        const size_t at = p.bytes;
+        p.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    place((size_t)n * sizeof(Token));
+    p.other = place(small ? 0 : (size_t)n * sizeof(Token));
+    p.counts = place(small ? 0 : (size_t)p.sort_tiles * kDigits * 4);
+    p.totals = place(small ? 0 : kDigits * 4);
+    p.parts = place((size_t)p.tiles * 2 * dim * 4);
+    return p;
+}
+
+extern "C" size_t dnatok_embedding_work_bytes(int64_t n, int64_t vocab, int64_t dim)
+{
+    return n > 0 && vocab > 0 && dim > 0 ? plan_of(n, vocab, dim).bytes : 0;
+}
+
+template <typename ID>
+static const Token *sort_tokens(const ID *ids, uint32_t n, uint32_t vocab, const GradPlan &p, char *work, hipStream_t s)
+{
+    Token *from = (Token *)work, *to = (Token *)(work + p.other);
+    if (n <= kSmallSort) {
+        sort_small_kernel<ID><<<1, kSmallThreads, 0, s>>>(ids, n, vocab, p.passes, p.bits, from);
+        return from;
+    }
+    uint32_t *counts = (uint32_t *)(work + p.counts), *totals = (uint32_t *)(work + p.totals);
+    for (int pass = 0; pass < p.passes; ++pass) {
+        const ID *source = pass ? nullptr : ids;
+        sort_count_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts);
+        sort_scan_kernel<<<1u << p.bits, 256, 0, s>>>(counts, p.sort_tiles, totals);
+        sort_place_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts, totals, to);
+        std::swap(from, to);
+    }
+    return from;
+}
 
 extern "C" int dnatok_embedding_backward(const void *ids, int32_t id_bytes, int64_t n, const void *dy, int64_t dy_stride, int32_t dtype,
                                          int64_t vocab, int64_t dim, const float *scale_h, void *grad, void *work, size_t work_bytes,
@@ -99,14 +530,25 @@ extern "C" int dnatok_embedding_backward(const void *ids, int32_t id_bytes, int6
     if (vocab == 0 || dim == 0) return DNATOK_OK;
     EMBED_REQUIRE((n == 0 || (ids && dy)) && grad && scale_h, "null buffer");
     EMBED_REQUIRE(work_bytes >= dnatok_embedding_work_bytes(n, vocab, dim) && (work || !work_bytes), "work space too small");
+    EMBED_REQUIRE((uintptr_t)work % 16 == 0, "work space must be 16-byte aligned");
     const float scale = *scale_h;
-    with_type(dtype, [&](auto t) {
-        using T = decltype(t);
+    hipStream_t s = (hipStream_t)stream;
+    GradPlan p{};
+    const Token *tokens = nullptr;
+    if (n) {
+        p = plan_of(n, vocab, dim);
         with_ids(id_bytes, [&](auto i) {
             using ID = decltype(i);
-            embed_grad_kernel<T, ID><<<(unsigned)vocab, 256, 0, (hipStream_t)stream>>>((const ID *)ids, n, (const T *)dy, dy_stride,
-                                                                                        dim, scale, (T *)grad);
+            tokens = sort_tokens((const ID *)ids, (uint32_t)n, (uint32_t)vocab, p, (char *)work, s);
         });
+    }
+    with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        const GradArgs a{tokens, (uint32_t)n, (uint32_t)vocab, p.tiles, p.run, dy, dy_stride, dim, scale, grad,
+                         (float *)((char *)work + p.parts)};
+        const unsigned blocks = (unsigned)blocks_of(dim, sizeof(T)), zeros = (unsigned)((vocab + kZeroRows * 4 - 1) / (kZeroRows * 4));
+        embed_grad_kernel<T><<<dim3((p.tiles + 3) / 4 + zeros, blocks), 256, 0, s>>>(a);
+        if (p.tiles > 1) embed_join_kernel<T><<<dim3(p.tiles - 1, blocks), kJoinWaves * 64, 0, s>>>(a);
     });
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
