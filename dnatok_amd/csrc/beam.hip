@@ -18,122 +18,295 @@ __device__ __forceinline__ uint32_t ordered(float v)
 }
 __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u); }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 struct Candidate {
     float logit;
     int32_t token;                                 // -1: none
 };
+struct Part {                                      // of a row's sum of exponentials
+    double sum;
+    float top;
+};
 
-// A workgroup to a row: its sum, then its largest again and again.
-template <typename T>
-__global__ __launch_bounds__(256) void beam_rows_kernel(const T *logits, int64_t stride, int32_t vocab, int32_t width,
-                                                        Candidate *found, double *sums)
+constexpr int kRowThreads = 1024, kRowWaves = kRowThreads / 64;
+constexpr int kSlice = 32768;                      // most tokens of a slice: 32 to a thread
+constexpr int kListed = 1024;                      // candidates that are ranked against each other
+
+// The largest of the workgroup's values.
+template <typename V> __device__ __forceinline__ V workgroup_max(V v, V *room)
 {
-    __shared__ uint64_t best[4];
-    __shared__ double part[4];
-    const int64_t row = blockIdx.x;
-    const T *z = logits + row * stride;
-    uint64_t last = ~0ull;
-    float top = 0.0f;
-    for (int i = -1; i < width; ++i) {
-        uint64_t mine = 0;
-        for (int v = threadIdx.x; v < vocab; v += 256) {
-            const uint64_t key = (uint64_t)ordered(to_float(z[v])) << 32 | (uint32_t)~v;
-            if (key < last && key > mine) mine = key;
-        }
-        for (int d = 32; d; d >>= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)mine, d);
-            mine = other > mine ? other : mine;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
-        __syncthreads();
-        for (int w = 0; w < 4; ++w) mine = best[w] > mine ? best[w] : mine;
-        const float value = from_ordered((uint32_t)(mine >> 32));
-        if (i < 0) {
-            top = value;
-            double sum = 0.0;
-            for (int v = threadIdx.x; v < vocab; v += 256) sum += expf(to_float(z[v]) - top);
-            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
-            __syncthreads();
-            if (threadIdx.x == 0) sums[row] = (double)top + log(part[0] + part[1] + part[2] + part[3]);
-            continue;
-        }
-        if (threadIdx.x == 0) found[row * width + i] = mine ? Candidate{value, (int32_t)~(uint32_t)mine} : Candidate{-INFINITY, -1};
-        last = mine;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const V other = __shfl_xor(v, d);
+        v = other > v ? other : v;
     }
-}
-
-// A wave to a group: the beams' lists merged.
-__global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, const double *sums, const float *scores, const uint8_t *finished,
-                                                        int32_t eos, int32_t beams, int32_t width, float *out_scores, int32_t *tokens,
-                                                        int32_t *parents)
-{
-    __shared__ int32_t at[128];
-    const int64_t group = blockIdx.x;
-    for (int b = threadIdx.x; b < beams; b += 64) at[b] = 0;
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int i = 0; i < width; ++i) {
-        double value = -INFINITY;
-        int32_t beam = 0x7FFFFFFF, token = -1;
-        for (int b = threadIdx.x; b < beams; b += 64) {
-            const int64_t row = group * beams + b;
-            double v = -INFINITY;
-            int32_t t = -1;
-            if (finished && finished[row]) {
-                if (at[b] == 0) {
-                    v = scores[row];
-                    t = eos;
-                }
-            } else if (at[b] < width) {
-                const Candidate c = found[row * width + at[b]];
-                const double sum = sums[row];
-                if (c.token >= 0 && sum < INFINITY && sum > -INFINITY) {
-                    v = (double)scores[row] + ((double)c.logit - sum);
-                    t = c.token;
-                }
-            }
-            if (v > value) {
-                value = v;
-                beam = b;
-                token = t;
-            }
+    v = room[0];
+#pragma unroll
+    for (int w = 1; w < kRowWaves; ++w) v = room[w] > v ? room[w] : v;
+    __syncthreads();
+    return v;
+}
+
+// A workgroup to a slice of a row, 32 tokens to a thread at most, held in registers.  The width-th largest of the threads' largest (to
+// 16 bits) is a bound that the slice's `width` largest are not below, and few others are above it: those are listed
+// and ranked by counting who is in front.  Where the list does not hold them (many equal ones), the largest is looked for again
+// and again.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(const T *logits, int64_t stride, int32_t vocab, int32_t slice,
+                                                                int32_t width, Candidate *found, Part *parts)
+{
+    constexpr int kCount = 16 / sizeof(T), kSteps = kSlice / kRowThreads / kCount;
+    typedef T words __attribute__((ext_vector_type(kCount)));
+    __shared__ uint64_t list[kListed], best[kRowWaves];
+    __shared__ double sums[kRowWaves];
+    __shared__ uint32_t tops[kRowWaves], counts[2][kRowWaves], listed;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.y, index = row * gridDim.x + blockIdx.x;
+    const int32_t first = blockIdx.x * slice, here = vocab - first < slice ? vocab - first : slice;
+    const T *z = logits + row * stride + first;
+    if (threadIdx.x == 0) listed = 0;
+    words v[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        const int at = (j * kRowThreads + threadIdx.x) * kCount;
+        if (at + kCount <= here) {
+            __builtin_memcpy(&v[j], z + at, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) v[j][e] = at + e < here ? z[at + e] : (T)-INFINITY;
         }
-        for (int d = 32; d; d >>= 1) {
-            const double v = __shfl_xor(value, d);
-            const int32_t b = __shfl_xor(beam, d), t = __shfl_xor(token, d);
-            if (v > value || (v == value && b < beam)) {
-                value = v;
-                beam = b;
-                token = t;
-            }
+    }
+    // candidates in the order of integers; -inf and NaN are 0: none
+    const auto key_of = [](T value) {
+        const float f = (float)value;
+        return f > -INFINITY ? ordered(f) : 0u;
+    };
+    uint32_t mine = 0, odd = 0;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            const uint32_t k = key_of(v[j][e]);
+            mine = k > mine ? k : mine;
+            odd |= (float)v[j][e] != (float)v[j][e];
         }
-        const bool none = !(value > -INFINITY);
-        if (threadIdx.x == 0) {
-            out_scores[group * width + i] = none ? -INFINITY : (float)value;
-            tokens[group * width + i] = none ? -1 : token;
-            parents[group * width + i] = none ? i % beams : beam;
-            if (!none) ++at[beam];
-        }
+    const uint32_t highest = workgroup_max(mine, tops);
+    const float top = highest ? from_ordered(highest) : -INFINITY;
+    float sum = odd ? NAN : 0.0f;
+    if (highest) {
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+            if (j * kRowThreads * kCount < here)
+#pragma unroll
+                for (int e = 0; e < kCount; ++e) sum += expf((float)v[j][e] - top);
+    }
+    double all = sum;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+    if (lane == 0) sums[wave] = all;
+
+    // the bound: bits of it from the highest on, as long as `width` threads reach it
+    uint32_t bound = 0;
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t next = bound | 1u << bit;
+        const uint64_t reach = __ballot(mine >= next);
+        if (lane == 0) counts[bit & 1][wave] = __popcll(reach);
         __syncthreads();
+        uint32_t n = 0;
+#pragma unroll
+        for (int w = 0; w < kRowWaves; ++w) n += counts[bit & 1][w];
+        if (n >= (uint32_t)width) bound = next;
+    }
+    bound = bound ? bound : 1;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) {
+            const uint32_t k = key_of(v[j][e]);
+            if (k >= bound) {
+                const uint32_t at = atomicAdd(&listed, 1u);
+                if (at < kListed) list[at] = (uint64_t)k << 32 | (uint32_t)~(first + (j * kRowThreads + threadIdx.x) * kCount + e);
+            }
+        }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kRowWaves; ++w) all += sums[w];
+        parts[index] = Part{all, top};
+    }
+    found += index * width;
+    const auto candidate = [](uint64_t key) { return Candidate{from_ordered((uint32_t)(key >> 32)), (int32_t)~(uint32_t)key}; };
+    const uint32_t n = listed;
+    if (n <= kListed) {
+        const uint64_t own = threadIdx.x < n ? list[threadIdx.x] : 0;
+        uint32_t rank = 0;
+        if (threadIdx.x < n)
+            for (uint32_t i = 0; i < n; ++i) rank += list[i] > own;
+        if (threadIdx.x < n && rank < (uint32_t)width) found[rank] = candidate(own);
+        for (int i = n + threadIdx.x; i < width; i += kRowThreads) found[i] = Candidate{-INFINITY, -1};
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int i = 0; i < width; ++i) {
+        uint64_t next = 0;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+            for (int e = 0; e < kCount; ++e) {
+                const uint64_t k = (uint64_t)key_of(v[j][e]) << 32 | (uint32_t)~(first + (j * kRowThreads + threadIdx.x) * kCount + e);
+                if (k < last && k > next) next = k;
+            }
+        last = workgroup_max((unsigned long long)next, (unsigned long long *)best);
+        if (threadIdx.x == 0) found[i] = last >> 32 ? candidate(last) : Candidate{-INFINITY, -1};
     }
 }
 
-constexpr int kReorderTensors = 16;
+// A wave to a group: the lists of its beams' slices, each in falling order, merged.  A lane has the best of what is left of its
+// lists (list l is lane l % 64's); lists are in the order of beams and tokens.
+constexpr int kMergeStaged = 4096;                 // candidates that are read into LDS at once
+template <bool STAGED>
+__global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, const Part *parts, const float *scores, const uint8_t *finished,
+                                                        int32_t eos, int32_t beams, int32_t slices, int32_t width, int32_t *places,
+                                                        float *out_scores, int32_t *tokens, int32_t *parents)
+{
+    __shared__ Candidate held[STAGED ? kMergeStaged : 1];
+    __shared__ double sums[128];
+    __shared__ float before[128];
+    __shared__ uint8_t ended[128];
+    const int lane = threadIdx.x;
+    const int64_t group = blockIdx.x;
+    const int lists = beams * slices;
+    found += group * lists * width;
+    parts += group * lists;
+    places += group * lists;                       // how many of each list were taken
+    if (STAGED)
+        for (int i = lane; i < lists * width; i += 64) held[i] = found[i];
+    for (int b = lane; b < beams; b += 64) {
+        float top = -INFINITY;
+        for (int s = 0; s < slices; ++s) top = fmaxf(top, parts[b * slices + s].top);
+        double sum = 0.0;
+        for (int s = 0; s < slices; ++s) {
+            const Part p = parts[b * slices + s];
+            if (p.sum != 0.0) sum += p.sum * exp((double)p.top - (double)top);     // (a NaN stays one)
+        }
+        sums[b] = (double)top + log(sum);
+        before[b] = scores[group * beams + b];
+        ended[b] = finished ? finished[group * beams + b] : 0;
+    }
+    for (int l = lane; l < lists; l += 64) places[l] = 0;
+    __syncthreads();
+    const auto value = [&](int l, int at, float *logit, int32_t *token) {
+        const int b = l / slices;
+        *token = -1;
+        *logit = 0.0f;
+        if (ended[b]) {
+            if (at == 0 && l == b * slices) {
+                *token = eos;
+                return (double)before[b];
+            }
+            return -(double)INFINITY;
+        }
+        if (at >= width) return -(double)INFINITY;
+        const Candidate c = STAGED ? held[l * width + at] : found[(int64_t)l * width + at];
+        const double sum = sums[b];
+        if (c.token < 0 || !(sum < INFINITY && sum > -INFINITY)) return -(double)INFINITY;
+        *token = c.token;
+        *logit = c.logit;
+        return (double)before[b] + ((double)c.logit - sum);
+    };
+    double mine = -INFINITY;
+    float logit = 0.0f;
+    int32_t token = -1, list = lists;
+    const auto look = [&] {
+        mine = -INFINITY;
+        list = lists;
+        for (int l = lane; l < lists; l += 64) {
+            float z;
+            int32_t t;
+            const double v = value(l, places[l], &z, &t);
+            if (v > mine || (v == mine && v > -INFINITY && l / slices == list / slices && z > logit)) {
+                mine = v;
+                logit = z;
+                token = t;
+                list = l;
+            }
+        }
+    };
+    look();
+    for (int i = 0; i < width; ++i) {
+        double best = mine;
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+            const double other = __shfl_xor(best, d);
+            best = other > best ? other : best;
+        }
+        if (!(best > -INFINITY)) {
+            for (int j = i + lane; j < width; j += 64) {
+                out_scores[group * width + j] = -INFINITY;
+                tokens[group * width + j] = -1;
+                parents[group * width + j] = j % beams;
+            }
+            return;
+        }
+        // of equal ones the lowest beam's, of that beam's the one with the largest logit, the lowest list's
+        uint64_t equal = __ballot(mine == best);
+        int winner = __builtin_ctzll(equal);
+        for (equal &= equal - 1; equal; equal &= equal - 1) {
+            const int l = __builtin_ctzll(equal);
+            const int list_l = __shfl(list, l), list_w = __shfl(list, winner);
+            const float z_l = __shfl(logit, l), z_w = __shfl(logit, winner);
+            const int beam_l = list_l / slices, beam_w = list_w / slices;
+            if (beam_l < beam_w || (beam_l == beam_w && (z_l > z_w || (z_l == z_w && list_l < list_w)))) winner = l;
+        }
+        if (lane == winner) {
+            out_scores[group * width + i] = (float)mine;
+            tokens[group * width + i] = token;
+            parents[group * width + i] = list / slices;
+            ++places[list];
+            look();
+        }
+    }
+}
+
+constexpr int kReorderTensors = 16, kReorderBlock = 16384;             // bytes of a row to a workgroup
 struct Reorder {
     dnatok_rows t[kReorderTensors];
 };
 
-// Row r of a group's `width` is row parents[r] of its `beams`.
+// Row r of a group's `width` is row parents[r] of its `beams`, 16, 4 or 1 bytes to a lane.
 __global__ __launch_bounds__(256) void reorder_kernel(Reorder all, const int32_t *parents, int64_t rows, int32_t beams, int32_t width)
 {
     const dnatok_rows t = all.t[blockIdx.z];
+    const int64_t from = (int64_t)blockIdx.x * kReorderBlock;
+    if (from >= t.bytes) return;
+    const int64_t end = t.bytes - from < kReorderBlock ? t.bytes : from + kReorderBlock;
+    const uint64_t places = (uint64_t)t.in | (uint64_t)t.out | (uint64_t)t.bytes | (uint64_t)t.in_stride | (uint64_t)t.out_stride;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const int32_t parent = parents[r];
         const bool known = parent >= 0 && parent < beams;
         const uint8_t *in = (const uint8_t *)t.in + (r / width * beams + (known ? parent : 0)) * t.in_stride;
         uint8_t *out = (uint8_t *)t.out + r * t.out_stride;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < t.bytes; i += (int64_t)gridDim.x * 256) out[i] = known ? in[i] : 0;
+        if (places % 16 == 0) {
+            u32x4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = from + (i * 256 + threadIdx.x) * 16;
+                v[i] = u32x4{0, 0, 0, 0};
+                if (at < end && known) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(in + at));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t at = from + (i * 256 + threadIdx.x) * 16;
+                if (at < end) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4 *>(out + at));
+            }
+        } else if (places % 4 == 0) {
+            for (int64_t at = from + threadIdx.x * 4; at < end; at += 1024)
+                *reinterpret_cast<uint32_t *>(out + at) = known ? *reinterpret_cast<const uint32_t *>(in + at) : 0u;
+        } else {
+            for (int64_t at = from + threadIdx.x; at < end; at += 256) out[at] = known ? in[at] : 0;
+        }
     }
 }
 
@@ -143,10 +316,20 @@ using namespace dnatok;
 
 #define BEAM_REQUIRE(cond, text) DNATOK_REQUIRE(cond, DNATOK_E_INVALID, "%s: " text, who)
 
+// Slices of a row: as few as hold it, or as many as make 256 workgroups, of 4,096 tokens and more.
+static int64_t slice_of(int64_t rows, int64_t vocab)
+{
+    const int64_t fewest = (vocab + kSlice - 1) / kSlice, most = (vocab + 4095) / 4096;
+    int64_t slices = 256 / rows;
+    slices = slices < fewest ? fewest : slices > most ? most : slices;
+    return (vocab + slices - 1) / slices;
+}
+
 extern "C" size_t dnatok_beam_work_bytes(int64_t groups, int32_t beams, int64_t vocab, int32_t width)
 {
     if (groups <= 0 || beams <= 0 || width <= 0 || vocab <= 0) return 0;
-    return (size_t)groups * beams * (8 + 8 * (size_t)width);
+    const int64_t rows = groups * beams, slice = slice_of(rows, vocab);
+    return (size_t)(rows * ((vocab + slice - 1) / slice)) * (sizeof(Part) + 4 + sizeof(Candidate) * (size_t)width);
 }
 
 extern "C" int dnatok_beam_select(const void *logits, int64_t stride, int32_t dtype, int64_t groups, int32_t beams, int64_t vocab,
@@ -165,13 +348,25 @@ extern "C" int dnatok_beam_select(const void *logits, int64_t stride, int32_t dt
     BEAM_REQUIRE(work && work_bytes >= dnatok_beam_work_bytes(groups, beams, vocab, width), "work space too small");
     BEAM_REQUIRE((uintptr_t)work % 16 == 0, "work space must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
-    double *sums = (double *)work;
-    Candidate *found = (Candidate *)(sums + groups * beams);
+    const int64_t rows = groups * beams, slice = slice_of(rows, vocab), slices = (vocab + slice - 1) / slice;
+    Part *parts = (Part *)work;
+    Candidate *found = (Candidate *)(parts + rows * slices);
+    int32_t *places = (int32_t *)(found + rows * slices * width);
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        beam_rows_kernel<T><<<(unsigned)(groups * beams), 256, 0, s>>>((const T *)logits, stride, (int32_t)vocab, width, found, sums);
+        for (int64_t first = 0; first < rows; first += 65535) {        // (a grid's second dimension ends there)
+            const int64_t here = rows - first < 65535 ? rows - first : 65535;
+            beam_rows_kernel<T><<<dim3((unsigned)slices, (unsigned)here), kRowThreads, 0, s>>>(
+                (const T *)logits + first * stride, stride, (int32_t)vocab, (int32_t)slice, width, found + first * slices * width,
+                parts + first * slices);
+        }
     });
-    beam_merge_kernel<<<(unsigned)groups, 64, 0, s>>>(found, sums, scores, finished, eos, beams, width, out_scores, tokens, parents);
+    if (beams * slices * width <= kMergeStaged)
+        beam_merge_kernel<true><<<(unsigned)groups, 64, 0, s>>>(found, parts, scores, finished, eos, beams, (int32_t)slices, width, places,
+                                                                 out_scores, tokens, parents);
+    else
+        beam_merge_kernel<false><<<(unsigned)groups, 64, 0, s>>>(found, parts, scores, finished, eos, beams, (int32_t)slices, width, places,
+                                                                  out_scores, tokens, parents);
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
 }
@@ -184,7 +379,7 @@ extern "C" int dnatok_reorder_rows(const dnatok_rows *tensors_h, int32_t n, cons
     BEAM_REQUIRE(n == 0 || tensors_h, "null list");
     DNATOK_REQUIRE(groups < (1ll << 31), DNATOK_E_TOO_LARGE, "%s: at most 2^31 groups", who);
     for (int i = 0; i < n; ++i)
-        BEAM_REQUIRE(tensors_h[i].bytes >= 0 && tensors_h[i].in_stride >= 0 && tensors_h[i].out_stride >= 0, "negative size or stride");
+        BEAM_REQUIRE(tensors_h[i].bytes >= 0 && tensors_h[i].bytes < (1ll << 37) && tensors_h[i].in_stride >= 0 && tensors_h[i].out_stride >= 0, "a size or stride is negative or too large");
     const int64_t rows = groups * width;
     if (rows == 0 || n == 0) return DNATOK_OK;
     BEAM_REQUIRE(parents, "null buffer");
@@ -193,7 +388,11 @@ extern "C" int dnatok_reorder_rows(const dnatok_rows *tensors_h, int32_t n, cons
         Reorder all{};
         const int32_t here = n - first < kReorderTensors ? n - first : kReorderTensors;
         for (int i = 0; i < here; ++i) all.t[i] = tensors_h[first + i];
-        reorder_kernel<<<dim3(16, (unsigned)(rows < 65535 ? rows : 65535), (unsigned)here), 256, 0, (hipStream_t)stream>>>(all, parents, rows,
+        int64_t most = 0;
+        for (int i = 0; i < here; ++i) most = tensors_h[first + i].bytes > most ? tensors_h[first + i].bytes : most;
+        if (most == 0) continue;
+        const unsigned blocks = (unsigned)((most + kReorderBlock - 1) / kReorderBlock);
+        reorder_kernel<<<dim3(blocks, (unsigned)(rows < 65535 ? rows : 65535), (unsigned)here), 256, 0, (hipStream_t)stream>>>(all, parents, rows,
                                                                                                               beams, width);
     }
     DNATOK_HIP_TRY(hipGetLastError());
