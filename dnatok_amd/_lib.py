@@ -45,11 +45,6 @@ class LinearShape(ctypes.Structure):
                 ("scale", ctypes.c_float), ("with_offsets", c_int32)]
 
 
-class Rows(ctypes.Structure):
-    """dnatok_rows of include/dnatok_hip.h."""
-    _fields_ = [("input", c_void_p), ("out", c_void_p), ("bytes", c_int64), ("in_stride", c_int64), ("out_stride", c_int64)]
-
-
 class NormStep(ctypes.Structure):
     """dnatok_norm_step of include/dnatok_hip.h."""
     _fields_ = [("kind", c_int32), ("flags", c_int32), ("pattern_len", c_int32), ("content_len", c_int32),

@@ -20,6 +20,14 @@ __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_flo
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// exp(d) for d <= 0 to an ulp or two: what the product with log2(e) is rounded off by is multiplied on.  (-inf is far enough at -200.)
+__device__ __forceinline__ float exp_of(float d)
+{
+    d = fmaxf(d, -200.0f);
+    const float e = 1.44269504f * d, rest = fmaf(1.92596299e-8f, d, fmaf(1.44269504f, d, -e)), v = __builtin_amdgcn_exp2f(e);
+    return fmaf(v, 0.693147181f * rest, v);
+}
+
 struct Candidate {
     float logit;
     int32_t token;                                 // -1: none
@@ -101,7 +109,7 @@ __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(const T *logits,
         for (int j = 0; j < kSteps; ++j)
             if (j * kRowThreads * kCount < here)
 #pragma unroll
-                for (int e = 0; e < kCount; ++e) sum += expf((float)v[j][e] - top);
+                for (int e = 0; e < kCount; ++e) sum += exp_of((float)v[j][e] - top);
     }
     double all = sum;
 #pragma unroll
@@ -172,6 +180,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, 
                                                         float *out_scores, int32_t *tokens, int32_t *parents)
 {
     __shared__ Candidate held[STAGED ? kMergeStaged : 1];
+    __shared__ int32_t taken[STAGED ? kMergeStaged : 1];               // how many of each list (without room here, in places)
     __shared__ double sums[128];
     __shared__ float before[128];
     __shared__ uint8_t ended[128];
@@ -180,7 +189,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, 
     const int lists = beams * slices;
     found += group * lists * width;
     parts += group * lists;
-    places += group * lists;                       // how many of each list were taken
+    places += group * lists;
     if (STAGED)
         for (int i = lane; i < lists * width; i += 64) held[i] = found[i];
     for (int b = lane; b < beams; b += 64) {
@@ -195,7 +204,15 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, 
         before[b] = scores[group * beams + b];
         ended[b] = finished ? finished[group * beams + b] : 0;
     }
-    for (int l = lane; l < lists; l += 64) places[l] = 0;
+    const auto set_taken = [&](int l, int32_t n) {
+        if constexpr (STAGED) taken[l] = n;
+        else places[l] = n;
+    };
+    const auto get_taken = [&](int l) {
+        if constexpr (STAGED) return taken[l];
+        else return places[l];
+    };
+    for (int l = lane; l < lists; l += 64) set_taken(l, 0);
     __syncthreads();
     const auto value = [&](int l, int at, float *logit, int32_t *token) {
         const int b = l / slices;
@@ -225,7 +242,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, 
         for (int l = lane; l < lists; l += 64) {
             float z;
             int32_t t;
-            const double v = value(l, places[l], &z, &t);
+            const double v = value(l, get_taken(l), &z, &t);
             if (v > mine || (v == mine && v > -INFINITY && l / slices == list / slices && z > logit)) {
                 mine = v;
                 logit = z;
@@ -264,7 +281,7 @@ __global__ __launch_bounds__(64) void beam_merge_kernel(const Candidate *found, 
             out_scores[group * width + i] = (float)mine;
             tokens[group * width + i] = token;
             parents[group * width + i] = list / slices;
-            ++places[list];
+            set_taken(list, get_taken(list) + 1);
             look();
         }
     }

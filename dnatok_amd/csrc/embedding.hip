@@ -37,6 +37,15 @@ template <typename T> __device__ __forceinline__ void store_words(T *row, int64_
     }
 }
 
+// Where a lane's sixteen bytes begin: the last ones of a row end with it, so that they overlap those in front of them and hold (and write)
+// the same values there.  -1: none.  (Only rows of less than sixteen bytes are taken by elements.)
+template <typename T> __device__ __forceinline__ int64_t words_at(int64_t dim)
+{
+    const int64_t at = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * Words<T>::kCount;
+    if (at >= dim) return -1;
+    return at + Words<T>::kCount > dim && dim >= Words<T>::kCount ? dim - Words<T>::kCount : at;
+}
+
 // ---- rows for ids --------------------------------------------------------------------------------------
 
 constexpr int kEmbedAhead = 8;                     // rows that a wave has under way
@@ -49,7 +58,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, in
     typedef Words<T> W;
     const int lane = threadIdx.x & 63;
     const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * run;
-    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    const int64_t at = words_at<T>(dim);
     for (int64_t t0 = first; t0 < first + run && t0 < n; t0 += kEmbedAhead) {
         const int here = n - t0 < kEmbedAhead ? (int)(n - t0) : kEmbedAhead;
         int64_t mine = lane < here ? (int64_t)ids[t0 + lane] : -1;
@@ -60,11 +69,11 @@ __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, in
         for (int i = 0; i < kEmbedAhead; ++i) {
             const int32_t id = __builtin_amdgcn_readlane(low, i);
             v[i] = typename W::type{};
-            if (id >= 0 && at < dim) v[i] = load_words(weight + id * w_stride, at, dim);
+            if (id >= 0 && at >= 0) v[i] = load_words(weight + id * w_stride, at, dim);
         }
 #pragma unroll
         for (int i = 0; i < kEmbedAhead; ++i) {
-            if (i >= here || at >= dim) break;
+            if (i >= here || at < 0) break;
             // (a row of no id is zeros whatever the scale is)
             store_words(y + (t0 + i) * dim, at, dim,
                         __builtin_convertvector(__builtin_convertvector(v[i], typename W::floats) * scale, typename W::type));
@@ -77,7 +86,8 @@ __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, in
 // Keys are ids, those outside the table the number behind its last row.  A pass sorts by up to eight of their bits: a workgroup
 // counts its tile's digits, a scan gives each tile its place for each digit, and a workgroup writes its tile there, the tokens of one
 // digit in their order.  So tokens of one id stay in their order, and a sum over them is the same in every call.
-constexpr int kSortTile = 4096, kSortThreads = 256, kSortWaves = kSortThreads / 64, kDigits = 256;
+constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64, kDigits = 256;
+constexpr int kFewPerLane = 4, kManyPerLane = 32;    // tokens of a tile to a thread: tiles of 1,024, or of 8,192 above 2^22 tokens
 constexpr int kSmallSort = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 
 struct Token {
@@ -99,18 +109,25 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool he
     return same;
 }
 
-template <typename ID>
+template <typename ID, int PER>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
                                                                   int shift, int bits, uint32_t *counts)
 {
     __shared__ uint32_t count[kDigits];
     for (int i = threadIdx.x; i < kDigits; i += kSortThreads) count[i] = 0;
     __syncthreads();
-    const uint32_t first = blockIdx.x * kSortTile, mask = (1u << bits) - 1;
+    const uint32_t first = blockIdx.x * (kSortThreads * PER), mask = (1u << bits) - 1;
     const int lane = threadIdx.x & 63;
-    for (uint32_t i = first + threadIdx.x; i - threadIdx.x < first + kSortTile && i - threadIdx.x < n; i += kSortThreads) {
-        const bool here = i < n;
-        const uint32_t digit = here ? (ids ? key_of(ids[i], vocab) : tokens[i].key) >> shift & mask : 0;
+    uint32_t key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint32_t i = first + j * kSortThreads + threadIdx.x;
+        key[j] = i < n ? (ids ? key_of(ids[i], vocab) : tokens[i].key) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const bool here = first + j * kSortThreads + threadIdx.x < n;
+        const uint32_t digit = key[j] >> shift & mask;
         const uint64_t same = same_digit(digit, bits, here);
         if (here && (same & ((1ull << lane) - 1)) == 0) atomicAdd(&count[digit], (uint32_t)__popcll(same));
     }
@@ -138,19 +155,19 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t *counts, uint32
     if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-template <typename ID>
+template <typename ID, int PER>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
                                                                   int shift, int bits, const uint32_t *counts, const uint32_t *totals,
                                                                   Token *out)
 {
     __shared__ uint32_t place[kSortWaves][kDigits], part[4];
-    constexpr int kPerLane = kSortTile / kSortThreads;
+    constexpr int kPerLane = PER;
     const uint32_t mask = (1u << bits) - 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) place[0][i] = 0;
     __syncthreads();
     // a wave has neighbouring tokens, 64 at a time
-    const uint32_t first = blockIdx.x * kSortTile + wave * (kSortTile / kSortWaves);
+    const uint32_t first = blockIdx.x * (kSortThreads * PER) + wave * (64 * PER);
     uint32_t key[kPerLane], at[kPerLane];
     uint64_t same[kPerLane];
 #pragma unroll
@@ -305,7 +322,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
 {
     typedef Words<T> W;
     const int lane = threadIdx.x & 63;
-    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    const int64_t at = words_at<T>(a.dim);
     const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6);
     T *grad = (T *)a.grad;
     if (tile >= (a.tiles + 3) / 4 * 4) {
@@ -319,7 +336,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
         while (rows) {
             const int i = __builtin_ctzll(rows);
             rows &= rows - 1;
-            if (at < a.dim) store_words(grad + (int64_t)(row - lane + i) * a.dim, at, a.dim, typename W::type{});
+            if (at >= 0) store_words(grad + (int64_t)(row - lane + i) * a.dim, at, a.dim, typename W::type{});
         }
         return;
     }
@@ -330,12 +347,16 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
     uint32_t key = a.tokens[begin].key;
     bool from_front = key == front;
     const auto finish = [&](bool goes_on) {
-        if (key >= a.vocab || at >= a.dim) return;
+        if (key >= a.vocab || at < 0) return;
         if (from_front || goes_on) {
             float *part = a.parts + ((int64_t)tile * 2 + !from_front) * a.dim;
+            if (at + W::kCount <= a.dim) {
+                __builtin_memcpy(part + at, &sum, sizeof(sum));
+            } else {
 #pragma unroll
-            for (int i = 0; i < W::kCount; ++i)
-                if (at + i < a.dim) part[at + i] = sum[i];
+                for (int i = 0; i < W::kCount; ++i)
+                    if (at + i < a.dim) part[at + i] = sum[i];
+            }
         } else {
             store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
         }
@@ -349,45 +370,58 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
             for (int i = 0; i < kGradAhead; ++i) {
                 const uint32_t row = __builtin_amdgcn_readlane(mine.at, j0 + i);
                 v[i] = typename W::type{};
-                if (at < a.dim) v[i] = load_words((const T *)a.dy + (int64_t)row * a.dy_stride, at, a.dim);
+                if (at >= 0) v[i] = load_words((const T *)a.dy + (int64_t)row * a.dy_stride, at, a.dim);
             }
+            const int here = end - t0 - j0 < (uint32_t)kGradAhead ? (int)(end - t0 - j0) : kGradAhead;
 #pragma unroll
             for (int i = 0; i < kGradAhead; ++i) {
-                if (t0 + j0 + i >= end) break;
-                const uint32_t next = __builtin_amdgcn_readlane(mine.key, j0 + i);
-                if (next != key) {
-                    finish(false);
-                    key = next;
-                    from_front = false;
-                    sum = typename W::floats{};
+                if (i < here) {
+                    const uint32_t next = __builtin_amdgcn_readlane(mine.key, j0 + i);
+                    if (next != key) {
+                        finish(false);
+                        key = next;
+                        from_front = false;
+                        sum = typename W::floats{};
+                    }
+                    sum += __builtin_convertvector(v[i], typename W::floats);
                 }
-                sum += __builtin_convertvector(v[i], typename W::floats);
             }
         }
     }
     finish(key == back);
 }
 
-// A run that begins in one tile and ends in another: its parts, added up by eight waves and then in their order.
-constexpr int kJoinWaves = 8;
+// A run that begins in one tile and ends in another: its parts, added up by sixteen waves and then in their order.
+constexpr int kJoinWaves = 16, kJoinAhead = 8;
 template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(GradArgs a)
 {
     typedef Words<T> W;
     __shared__ typename W::floats part[kJoinWaves][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t tile = blockIdx.x, end = (tile + 1) * (uint32_t)a.run;
+    const uint32_t tile = blockIdx.x, begin = tile * (uint32_t)a.run, end = begin + (uint32_t)a.run;
     if (end >= a.n) return;
-    const uint32_t key = a.tokens[end].key;
-    if (key >= a.vocab || a.tokens[end - 1].key != key) return;
-    const uint32_t begin = tile * (uint32_t)a.run;
+    const uint32_t next = end + (uint32_t)a.run < a.n ? end + (uint32_t)a.run : a.n - 1;
+    const uint32_t key = a.tokens[end].key, mine = a.tokens[end - 1].key, head = a.tokens[begin].key,
+                   front = begin ? a.tokens[begin - 1].key : ~0u, after = a.tokens[next].key;
+    if (key >= a.vocab || mine != key) return;
     // (the run's first tile does it: it begins there, behind the tile's begin or at it with another id in front)
-    if (a.tokens[begin].key == key && begin && a.tokens[begin - 1].key == key) return;
-    const uint32_t last = (first_of(a.tokens, a.n, key + 1) - 1) / (uint32_t)a.run;
-    const int64_t at = ((int64_t)blockIdx.y * 64 + lane) * W::kCount;
+    if (head == key && front == key) return;
+    uint32_t last = tile + 1;
+    if (after == key) {                            // the last token of the id: 64 places are looked at at once
+        uint32_t lo = next, hi = a.n;              // (lo has it, hi does not)
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo - 1 + 63) / 64, at = lo + step * (lane + 1);
+            const int n = __popcll(__ballot(at < hi && a.tokens[at < hi ? at : lo].key == key));
+            lo += step * n;
+            hi = hi - lo > step ? lo + step : hi;
+        }
+        last = lo / (uint32_t)a.run;
+    }
+    const int64_t at = words_at<T>(a.dim);
     typename W::floats sum{};
     const auto piece = [&](uint32_t t) {
         typename W::floats v{};
-        if (t <= last && at < a.dim) {
+        if (t <= last && at >= 0) {
             const float *p = a.parts + ((int64_t)t * 2 + (t == tile)) * a.dim;
             if (at + W::kCount <= a.dim) {
                 __builtin_memcpy(&v, p + at, sizeof(v));
@@ -399,18 +433,27 @@ template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_j
         }
         return v;
     };
-    for (uint32_t t = tile + wave; t <= last; t += kJoinWaves * 4) {
-        typename W::floats v[4];
+    if (last - tile < kJoinWaves) {                // few: one wave, no sums to be joined
+        if (wave) return;
+        for (uint32_t t = tile; t <= last; t += 2) {
+            const auto v = piece(t), u = piece(t + 1);
+            sum += v;
+            sum += u;
+        }
+    } else {
+        for (uint32_t t = tile + wave; t <= last; t += kJoinWaves * kJoinAhead) {
+            typename W::floats v[kJoinAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = piece(t + i * kJoinWaves);
+            for (int i = 0; i < kJoinAhead; ++i) v[i] = piece(t + i * kJoinWaves);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v[i];
+            for (int i = 0; i < kJoinAhead; ++i) sum += v[i];
+        }
+        part[wave][lane] = sum;
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
     }
-    part[wave][lane] = sum;
-    __syncthreads();
-    if (wave || at >= a.dim) return;
-    for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
-    store_words((T *)a.grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
+    if (at >= 0) store_words((T *)a.grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
 }
 
 }  // namespace dnatok
@@ -466,7 +509,7 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
 // What the backward pass needs besides its arguments: tokens sorted by id (twice, where they go from one place to the other), counts of
 // digits, and parts of sums.
 struct GradPlan {
-    uint32_t tiles, sort_tiles;
+    uint32_t tiles, sort_tiles, sort_tile;
     int32_t run, passes, bits;
     size_t other, counts, totals, parts, bytes;    // offsets
 };
@@ -477,11 +520,12 @@ static GradPlan plan_of(int64_t n, int64_t vocab, int64_t dim)
     while ((vocab >> bits) != 0) ++bits;           // (keys go up to vocab itself)
     p.passes = (bits + 7) / 8;
     p.bits = (bits + p.passes - 1) / p.passes;
-    p.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
-    // tiles as long as leaves some 4,096 waves; shorter ones write more parts of sums, longer ones leave CUs without work
+    p.sort_tile = kSortThreads * (n <= (1 << 22) ? kFewPerLane : kManyPerLane);
+    p.sort_tiles = (uint32_t)((n + p.sort_tile - 1) / p.sort_tile);
+    // tiles as long as leaves some 2,048 waves; shorter ones write more parts of sums, longer ones leave CUs without work
     const int64_t blocks = blocks_of(dim, 2);
     p.run = 16;
-    while (p.run < (1 << 20) && n / p.run * blocks > 4096) p.run *= 2;
+    while (p.run < (1 << 20) && n / p.run * blocks > 2048) p.run *= 2;
     p.tiles = (uint32_t)((n + p.run - 1) / p.run);
     const bool small = n <= kSmallSort;
     const auto place = [&](size_t bytes) {
@@ -513,9 +557,13 @@ static const Token *sort_tokens(const ID *ids, uint32_t n, uint32_t vocab, const
     uint32_t *counts = (uint32_t *)(work + p.counts), *totals = (uint32_t *)(work + p.totals);
     for (int pass = 0; pass < p.passes; ++pass) {
         const ID *source = pass ? nullptr : ids;
-        sort_count_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts);
-        sort_scan_kernel<<<1u << p.bits, 256, 0, s>>>(counts, p.sort_tiles, totals);
-        sort_place_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts, totals, to);
+        const auto sort = [&](auto per) {
+            sort_count_kernel<ID, per()><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts);
+            sort_scan_kernel<<<1u << p.bits, 256, 0, s>>>(counts, p.sort_tiles, totals);
+            sort_place_kernel<ID, per()><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts, totals, to);
+        };
+        if (p.sort_tile == kSortThreads * kFewPerLane) sort(std::integral_constant<int, kFewPerLane>{});
+        else sort(std::integral_constant<int, kManyPerLane>{});
         std::swap(from, to);
     }
     return from;

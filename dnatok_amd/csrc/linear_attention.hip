@@ -158,7 +158,7 @@ static size_t slots_bytes(const dnatok_linear_shape *s, int64_t cuts) { return (
 // Where rows are cut, so that one long row has many workgroups: at multiples of `cut` tokens.  What runs at once is two workgroups of
 // four waves on each of 256 CUs, or one of eight.  Rows (of all heads) that are fewer are cut into as many pieces as run at
 // once; more than that are cut where they are longer than about half of a CU's share, so that no long one is left running alone.  A
-// multiple or a whole part of the mean length, so that rows of one length are cut into equal pieces or not at all.
+// multiple or a whole part of the mean length, 512 tokens at least, so that rows of one length are cut into equal pieces or not at all.
 struct Cuts {
     int64_t cut, cuts;
 };
@@ -168,7 +168,10 @@ static Cuts cuts_of(const dnatok_linear_shape *s)
     if (s->total == 0 || s->n_rows == 0 || (!s->with_offsets && rows > running / 2)) return Cuts{512, 0};
     const int64_t mean = (s->total + s->n_rows - 1) / s->n_rows, pieces = running / rows, share = (rows + running) / (2 * running);
     int64_t cut = rows <= running ? (mean + pieces - 1) / pieces : mean * (share < 1 ? 1 : share);
-    cut = cut < 512 ? 512 : cut;
+    if (cut < 512) {
+        const int64_t whole = mean / 512;
+        cut = whole ? (mean + whole - 1) / whole : (511 + mean) / mean * mean;
+    }
     return Cuts{cut, (s->total - 1) / cut};
 }
 

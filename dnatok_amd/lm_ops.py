@@ -8,6 +8,7 @@ reference has no counterpart.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 from typing import Optional, Sequence, Tuple, Union
@@ -235,11 +236,40 @@ def _forward_only(name: str, *tensors) -> None:
 
 # ---- linear attention -------------------------------------------------------------------------
 
+class _LinearPlan:
+    """What calls of the same sizes have in common: their description for the C entries, and the sizes of their buffers."""
+
+    def __init__(self, *fields):
+        self.held = _lib.LinearShape(*fields)
+        self.shape, L = ctypes.addressof(self.held), _lib.lib()
+        self.states = L.dnatok_linear_attention_states_bytes(self.shape) // 4
+        self.work, self.work_back = (L.dnatok_linear_attention_work_bytes(self.shape, i) for i in (0, 1))
+
+
 @functools.lru_cache(maxsize=1024)
-def _linear_shape(*fields) -> Tuple["_lib.LinearShape", int]:
-    """A call's sizes, and their address, kept for the next call of the same sizes."""
-    shape = _lib.LinearShape(*fields)
-    return shape, ctypes.addressof(shape)
+def _linear_plan(dtypes, devices, qs, q_stride, ks, k_stride, vs, v_stride, dy_stride, n_rows, scale, reverse, with_offsets) -> _LinearPlan:
+    """Checks what linear attention takes for each token, q [N, H, Dk], k [N, G, Dk] and v [N, G, Dv]: once for calls of the
+    same sizes."""
+    if len(ks) != 3 or len(vs) != 3 or ks[0] != qs[0] or ks[2] != qs[2] or vs[:2] != ks[:2]:
+        raise ValueError("q, k and v must be [.., H, Dk], [.., G, Dk] and [.., G, Dv] of the same tokens")
+    (total, heads, dim_k), (_, kv_heads, dim_v) = qs, vs
+    if heads == 0 or kv_heads == 0 or heads % kv_heads:
+        raise ValueError("q's heads must be a multiple of k's and v's")
+    if not 1 <= dim_k <= 128 or not 1 <= dim_v <= 128:
+        raise ValueError("heads have 1 to 128 elements")
+    for what, dtype, device, shape, stride in zip("qkv", dtypes, devices, (qs, ks, vs), (q_stride, k_stride, v_stride)):
+        if dtype is not dtypes[0] or device != devices[0] or (shape[2] > 1 and stride[2] != 1):
+            raise ValueError(f"{what} must be a {dtypes[0]} tensor on {devices[0]} with a head's elements next to each other")
+    scale = dim_k ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < 3.4e38 or abs(scale) < 1e-37:
+        raise ValueError("scale must be a finite number other than 0")
+    return _LinearPlan(_DTYPES[dtypes[0]], reverse, n_rows, total, heads, kv_heads, dim_k, dim_v, *q_stride[:2], *k_stride[:2],
+                       *v_stride[:2], *dy_stride[:2], scale, with_offsets)
+
+
+def _plan_of(q, k, v, n_rows, scale, reverse, with_offsets, dy=None) -> _LinearPlan:
+    return _linear_plan((q.dtype, k.dtype, v.dtype), (q.device, k.device, v.device), q.shape, q.stride(), k.shape, k.stride(), v.shape,
+                        v.stride(), (0, 0) if dy is None else dy.stride(), n_rows, scale, reverse, with_offsets)
 
 
 class _LinearAttention(torch.autograd.Function):
@@ -255,9 +285,7 @@ class _LinearAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast):
         q, k, v, log_decay, offsets, h0, states = ctx.saved_tensors
-        device, L = q.device, _lib.lib()
-        total, heads, dim_k = q.shape
-        dim_v = v.shape[2]
+        device, (total, heads, _), dim_v = q.device, q.shape, v.shape[2]
         if dy is None:
             dy = torch.zeros((1, 1, 1), dtype=q.dtype, device=device).expand(total, heads, dim_v)
         if dim_v > 1 and dy.stride(2) != 1:
@@ -266,57 +294,33 @@ class _LinearAttention(torch.autograd.Function):
             dlast = dlast.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
         dh0 = torch.empty_like(h0) if h0 is not None and ctx.needs_input_grad[6] else None
-        _, shape = _shape_of(q, k, v, ctx.n_rows, ctx.scale, ctx.reverse, offsets, dy)
-        need = L.dnatok_linear_attention_work_bytes(shape, 1)
+        plan = _plan_of(q, k, v, ctx.n_rows, ctx.scale, int(ctx.reverse), int(offsets is not None), dy)
+        need = plan.work_back
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        _run("dnatok_linear_attention_backward", device, shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+        _run("dnatok_linear_attention_backward", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
              _ptr(offsets), _ptr(h0), dy.data_ptr(), _ptr(dlast), _ptr(states), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
              _ptr(dh0), _ptr(work), need)
         return dq, dk, dv, None, None, None, dh0, None, None
 
 
-def _shape_of(q, k, v, n_rows, scale, reverse, offsets, dy=None):
-    a, b, c, d = q.stride(), k.stride(), v.stride(), (0, 0) if dy is None else dy.stride()
-    total, heads, dim_k = q.shape
-    return _linear_shape(_DTYPES[q.dtype], int(reverse), n_rows, total, heads, k.shape[1], dim_k, v.shape[2], a[0], a[1], b[0], b[1],
-                         c[0], c[1], d[0], d[1], scale, int(offsets is not None))
-
-
 def _linear_forward(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse, keep_states):
-    total, heads, dim_k = q.shape
-    device, L, dim_v = q.device, _lib.lib(), v.shape[2]
-    _, shape = _shape_of(q, k, v, n_rows, scale, reverse, offsets)
+    (total, heads, dim_k), device, dim_v = q.shape, q.device, v.shape[2]
+    plan = _plan_of(q, k, v, n_rows, scale, int(reverse), int(offsets is not None))
     y = torch.empty((total, heads, dim_v), dtype=q.dtype, device=device)
     last = torch.empty((n_rows, heads, dim_k, dim_v), dtype=torch.float32, device=device)
-    states = None
+    states, need = None, plan.work
     if keep_states:
-        states = torch.empty(L.dnatok_linear_attention_states_bytes(shape) // 4, dtype=torch.float32, device=device)
-    need = L.dnatok_linear_attention_work_bytes(shape, 0)
+        states, need = torch.empty(plan.states, dtype=torch.float32, device=device), 0
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _run("dnatok_linear_attention", device, shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(offsets),
+    _run("dnatok_linear_attention", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(offsets),
          _ptr(h0), y.data_ptr(), last.data_ptr(), _ptr(states), _ptr(work), need)
     return y, last, states
 
 
-def _require_heads(name: str, q, k, v, log_decay, scale) -> float:
-    """Checks what linear attention takes for each token: q [N, H, Dk], k [N, G, Dk], v [N, G, Dv].  Returns the scale."""
-    if k.dim() != 3 or v.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or v.shape[:2] != k.shape[:2]:
-        raise ValueError("q, k and v must be [.., H, Dk], [.., G, Dk] and [.., G, Dv] of the same tokens")
-    (_, heads, dim_k), (_, kv_heads, dim_v) = q.shape, v.shape
-    if heads == 0 or kv_heads == 0 or heads % kv_heads:
-        raise ValueError("q's heads must be a multiple of k's and v's")
-    if not 1 <= dim_k <= 128 or not 1 <= dim_v <= 128:
-        raise ValueError("heads have 1 to 128 elements")
-    for what, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype is not q.dtype or t.device != q.device or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{what} must be a {q.dtype} tensor on {q.device} with a head's elements next to each other")
-    _require(log_decay, "log_decay", (heads,), torch.float32, q.device)
+def _require_decay(name: str, log_decay: torch.Tensor, heads: int, device: torch.device) -> None:
+    _require(log_decay, "log_decay", (heads,), torch.float32, device)
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient for log_decay")
-    scale = dim_k ** -0.5 if scale is None else float(scale)
-    if not abs(scale) < 3.4e38 or abs(scale) < 1e-37:
-        raise ValueError("scale must be a finite number other than 0")
-    return scale
 
 
 def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -351,9 +355,10 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
 
 
 def _linear_attention(q, k, v, log_decay, offsets, n_rows, h0, scale, reverse):
-    scale = _require_heads("linear_attention", q, k, v, log_decay, scale)
+    _plan_of(q, k, v, n_rows, scale, int(reverse), int(offsets is not None))
     if n_rows == 0 and q.shape[0]:
         raise ValueError("tokens without rows")
+    _require_decay("linear_attention", log_decay, q.shape[1], q.device)
     _require(h0, "h0", (n_rows, q.shape[1], q.shape[2], v.shape[2]), torch.float32, q.device)
     _no_tangent("linear_attention", q, k, v, log_decay, h0)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
@@ -389,8 +394,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if q.dim() != 3:
         raise ValueError("q must be [B, H, Dk]")
     device = q.device
-    scale = _require_heads("linear_attention_step", q, k, v, log_decay, scale)
-    shape = (q.shape[0], q.shape[1], q.shape[2], v.shape[2])
+    plan = _plan_of(q, k, v, q.shape[0], scale, 0, 0)
+    shape = (*q.shape, v.shape[2])
+    _require_decay("linear_attention_step", log_decay, shape[1], device)
     _require(state, "state", shape, torch.float32, device)
     _require(out_state, "out_state", shape, torch.float32, device)
     _forward_only("linear_attention_step", q, k, v, log_decay, state, out_state)
@@ -399,8 +405,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         out_state = torch.empty(shape, dtype=torch.float32, device=device)
     else:
         _require_apart("linear_attention_step", out_state, q, k, v, log_decay, state, same=state)
-    _run("dnatok_linear_attention_step", device, _shape_of(q, k, v, shape[0], scale, False, None)[1], q.data_ptr(), k.data_ptr(),
-         v.data_ptr(), log_decay.data_ptr(), _ptr(state), y.data_ptr(), out_state.data_ptr())
+    _run("dnatok_linear_attention_step", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+         _ptr(state), y.data_ptr(), out_state.data_ptr())
     return y, out_state
 
 
@@ -721,6 +727,11 @@ class TokenGrammar:
 
 # ---- beam search ------------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=256)
+def _beam_work(groups: int, beams: int, vocab: int, width: int) -> int:
+    return _lib.lib().dnatok_beam_work_bytes(groups, beams, vocab, width)
+
+
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: Optional[int] = None, *,
                 finished: Optional[torch.Tensor] = None, eos_id: Optional[int] = None
                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -748,9 +759,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: Optional[int]
     if finished is not None and (eos_id is None or not 0 <= eos_id < vocab):
         raise ValueError("finished needs an eos_id in the vocabulary")
     _forward_only("beam_select", logits, scores)
-    new = torch.empty((groups, width), dtype=torch.float32, device=device)
-    tokens, parents = (torch.empty((groups, width), dtype=torch.int32, device=device) for _ in range(2))
-    need = _lib.lib().dnatok_beam_work_bytes(groups, beams, vocab, width)
+    new = torch.empty_like(scores) if width == beams else torch.empty((groups, width), dtype=torch.float32, device=device)
+    tokens, parents = torch.empty((2, groups, width), dtype=torch.int32, device=device).unbind(0)
+    need = _beam_work(groups, beams, vocab, width)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _run("dnatok_beam_select", device, logits.data_ptr(), stride, _DTYPES[logits.dtype], groups, beams, vocab, scores.data_ptr(),
          _ptr(finished), eos_id if finished is not None else 0, width, new.data_ptr(), tokens.data_ptr(), parents.data_ptr(), _ptr(work),
@@ -777,7 +788,7 @@ def reorder_rows(tensors: Sequence[torch.Tensor], parents: torch.Tensor, *,
         return out
     beams = None
     for t in tensors:
-        if t.dim() < 1 or t.device != device or t.is_complex() or not t[:1].is_contiguous():
+        if t.dim() < 1 or t.device != device or t.is_complex() or not (t.is_contiguous() or t[:1].is_contiguous()):
             raise ValueError(f"tensors must be [B * K, ..] on {device} with contiguous rows")
         here = t.shape[0] // groups if groups else 1
         if (beams is not None and here != beams) or here * groups != t.shape[0]:
@@ -795,11 +806,10 @@ def reorder_rows(tensors: Sequence[torch.Tensor], parents: torch.Tensor, *,
         out = [torch.empty((groups * width, *t.shape[1:]), dtype=t.dtype, device=device) for t in tensors]
     if groups * width == 0:
         return out
-    rows = (_lib.Rows * len(tensors))()
-    for r, t, o in zip(rows, tensors, out):
+    rows = array.array("q")                        # dnatok_rows of include/dnatok_hip.h
+    for t, o in zip(tensors, out):
         size = t.element_size()
-        r.input, r.out = t.data_ptr(), o.data_ptr()
-        r.bytes = r.out_stride = t.numel() // t.shape[0] * size
-        r.in_stride = t.stride(0) * size
-    _run("dnatok_reorder_rows", device, ctypes.addressof(rows), len(tensors), parents.data_ptr(), groups, beams, width)
+        row = t.numel() // t.shape[0] * size
+        rows.extend((t.data_ptr(), o.data_ptr(), row, t.stride(0) * size, row))
+    _run("dnatok_reorder_rows", device, rows.buffer_info()[0], len(tensors), parents.data_ptr(), groups, beams, width)
     return out
