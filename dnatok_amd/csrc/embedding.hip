@@ -292,6 +292,8 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(const ID *ids
 constexpr int kGradAhead = 8;                      // rows of dy that a wave has under way
 constexpr int kZeroRows = 64;                      // rows of the gradient that a wave looks at for ids that do not occur
 
+// (The pointers that are written through are arguments of their own: kept in here, the compiler at times no longer knew that they
+// point to memory.)
 struct GradArgs {
     const Token *tokens;
     uint32_t n, vocab, tiles;
@@ -299,8 +301,6 @@ struct GradArgs {
     const void *dy;
     int64_t dy_stride, dim;
     float scale;
-    void *grad;
-    float *parts;                                  // [tiles, 2, dim]: of the runs at a tile's begin and end that go on elsewhere
 };
 
 // The first token whose key is not below `key`.
@@ -316,15 +316,14 @@ __device__ __forceinline__ uint32_t first_of(const Token *tokens, uint32_t n, ui
 }
 
 // A wave to a tile of the sorted tokens and 64 x 16 bytes of their rows: it adds up runs of one id.  A run inside the tile is a
-// row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts.  Further waves clear the
+// row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts [tiles, 2, dim].  Further waves clear the
 // rows of ids that do not occur.
-template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a)
+template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, float *parts, T *grad)
 {
     typedef Words<T> W;
     const int lane = threadIdx.x & 63;
     const int64_t at = words_at<T>(a.dim);
     const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6);
-    T *grad = (T *)a.grad;
     if (tile >= (a.tiles + 3) / 4 * 4) {
         const uint32_t row = (tile - (a.tiles + 3) / 4 * 4) * kZeroRows + lane;
         bool empty = row < a.vocab;
@@ -349,7 +348,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
     const auto finish = [&](bool goes_on) {
         if (key >= a.vocab || at < 0) return;
         if (from_front || goes_on) {
-            float *part = a.parts + ((int64_t)tile * 2 + !from_front) * a.dim;
+            float *part = parts + ((int64_t)tile * 2 + !from_front) * a.dim;
             if (at + W::kCount <= a.dim) {
                 __builtin_memcpy(part + at, &sum, sizeof(sum));
             } else {
@@ -393,7 +392,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
 
 // A run that begins in one tile and ends in another: its parts, added up by sixteen waves and then in their order.
 constexpr int kJoinWaves = 16, kJoinAhead = 8;
-template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(GradArgs a)
+template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(GradArgs a, const float *parts, T *grad)
 {
     typedef Words<T> W;
     __shared__ typename W::floats part[kJoinWaves][64];
@@ -422,7 +421,7 @@ template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_j
     const auto piece = [&](uint32_t t) {
         typename W::floats v{};
         if (t <= last && at >= 0) {
-            const float *p = a.parts + ((int64_t)t * 2 + (t == tile)) * a.dim;
+            const float *p = parts + ((int64_t)t * 2 + (t == tile)) * a.dim;
             if (at + W::kCount <= a.dim) {
                 __builtin_memcpy(&v, p + at, sizeof(v));
             } else {
@@ -453,7 +452,7 @@ template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_j
         if (wave) return;
         for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
     }
-    if (at >= 0) store_words((T *)a.grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
+    if (at >= 0) store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
 }
 
 }  // namespace dnatok
@@ -592,11 +591,11 @@ extern "C" int dnatok_embedding_backward(const void *ids, int32_t id_bytes, int6
     }
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const GradArgs a{tokens, (uint32_t)n, (uint32_t)vocab, p.tiles, p.run, dy, dy_stride, dim, scale, grad,
-                         (float *)((char *)work + p.parts)};
+        const GradArgs a{tokens, (uint32_t)n, (uint32_t)vocab, p.tiles, p.run, dy, dy_stride, dim, scale};
+        float *parts = (float *)((char *)work + p.parts);
         const unsigned blocks = (unsigned)blocks_of(dim, sizeof(T)), zeros = (unsigned)((vocab + kZeroRows * 4 - 1) / (kZeroRows * 4));
-        embed_grad_kernel<T><<<dim3((p.tiles + 3) / 4 + zeros, blocks), 256, 0, s>>>(a);
-        if (p.tiles > 1) embed_join_kernel<T><<<dim3(p.tiles - 1, blocks), kJoinWaves * 64, 0, s>>>(a);
+        embed_grad_kernel<T><<<dim3((p.tiles + 3) / 4 + zeros, blocks), 256, 0, s>>>(a, parts, (T *)grad);
+        if (p.tiles > 1) embed_join_kernel<T><<<dim3(p.tiles - 1, blocks), kJoinWaves * 64, 0, s>>>(a, parts, (T *)grad);
     });
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;
