@@ -432,8 +432,9 @@ extern "C" int dnatok_beam_select(const void *logits, int64_t stride, int32_t dt
     BEAM_REQUIRE(groups >= 0 && beams > 0 && vocab > 0 && width > 0, "bad size");
     BEAM_REQUIRE(stride >= 0, "negative stride");
     BEAM_REQUIRE(!finished || (eos >= 0 && eos < vocab), "finished beams need an end in the vocabulary");
-    DNATOK_REQUIRE(beams <= 128 && width <= 128 && vocab < (1ll << 31) && groups * beams < (1ll << 31), DNATOK_E_TOO_LARGE,
-                   "%s: at most 128 beams, before and after, and 2^31 rows of 2^31 tokens", who);
+    // (a grid ends at 2^32 threads, and a group has 64)
+    DNATOK_REQUIRE(beams <= 128 && width <= 128 && vocab < (1ll << 31) && groups < (1ll << 26) && groups * beams < (1ll << 31),
+                   DNATOK_E_TOO_LARGE, "%s: at most 128 beams, before and after, less than 2^26 groups, 2^31 rows and 2^31 tokens", who);
     if (groups == 0) return DNATOK_OK;
     BEAM_REQUIRE(logits && scores && out_scores && tokens && parents, "null buffer");
     BEAM_REQUIRE(work && work_bytes >= dnatok_beam_work_bytes(groups, beams, vocab, width), "work space too small");

@@ -116,7 +116,9 @@ static int check_shape(const char *who, const dnatok_linear_shape *s)
     LINEAR_REQUIRE(s->dtype == DNATOK_F32 || s->dtype == DNATOK_BF16 || s->dtype == DNATOK_F16, "unknown element type");
     LINEAR_REQUIRE(s->n_rows >= 0 && s->total >= 0 && s->heads > 0 && s->kv_heads > 0 && s->dim_k > 0 && s->dim_v > 0, "bad size");
     LINEAR_REQUIRE(s->heads % s->kv_heads == 0, "the heads must be a multiple of those of the keys and values");
-    LINEAR_REQUIRE(s->scale != 0.0f && __builtin_isfinite(s->scale), "the scale must be a finite number other than 0");
+    constexpr float kFarScale = 1099511627776.0f;  // (gradients of states are held divided by it)
+    LINEAR_REQUIRE(__builtin_fabsf(s->scale) >= 1.0f / kFarScale && __builtin_fabsf(s->scale) <= kFarScale,
+                   "the scale must be 2^-40 to 2^40 in size");
     LINEAR_REQUIRE(s->q_token >= 0 && s->q_head >= 0 && s->k_token >= 0 && s->k_head >= 0 && s->v_token >= 0 && s->v_head >= 0 &&
                        s->dy_token >= 0 && s->dy_head >= 0, "negative stride");
     constexpr int64_t kFar = (1ll << 31) / 64 / 4;
@@ -132,8 +134,9 @@ static int check_call(const char *who, const dnatok_linear_shape &s, const int64
     LINEAR_REQUIRE(!offsets == !s.with_offsets, "the shape must say whether there are offsets");
     LINEAR_REQUIRE(s.n_rows > 0 || s.total == 0, "tokens without rows");
     LINEAR_REQUIRE(offsets || s.n_rows == 0 || s.total % s.n_rows == 0, "rows of one length must fill the axis");
-    DNATOK_REQUIRE((s.n_rows + (s.total >> 9) + kOutside) < (1ll << 24) / s.heads, DNATOK_E_TOO_LARGE,
-                   "%s: at most 2^24 rows and pieces of rows times heads", who);
+    // (a grid ends at 2^32 threads, and a piece has up to 512)
+    DNATOK_REQUIRE((s.n_rows + (s.total >> 9) + kOutside) * s.heads < (1ll << 23), DNATOK_E_TOO_LARGE,
+                   "%s: less than 2^23 rows and pieces of rows times heads", who);
     return DNATOK_OK;
 }
 

@@ -260,16 +260,17 @@ def _linear_plan(dtypes, devices, qs, q_stride, ks, k_stride, vs, v_stride, dy_s
     for what, dtype, device, shape, stride in zip("qkv", dtypes, devices, (qs, ks, vs), (q_stride, k_stride, v_stride)):
         if dtype is not dtypes[0] or device != devices[0] or (shape[2] > 1 and stride[2] != 1):
             raise ValueError(f"{what} must be a {dtypes[0]} tensor on {devices[0]} with a head's elements next to each other")
-    scale = dim_k ** -0.5 if scale is None else float(scale)
-    if not abs(scale) < 3.4e38 or abs(scale) < 1e-37:
-        raise ValueError("scale must be a finite number other than 0")
+    scale = dim_k ** -0.5 if scale is None else scale
+    if not 2.0 ** -40 <= abs(scale) <= 2.0 ** 40:
+        raise ValueError("scale must be 2^-40 to 2^40 in size")
     return _LinearPlan(_DTYPES[dtypes[0]], reverse, n_rows, total, heads, kv_heads, dim_k, dim_v, *q_stride[:2], *k_stride[:2],
                        *v_stride[:2], *dy_stride[:2], scale, with_offsets)
 
 
 def _plan_of(q, k, v, n_rows, scale, reverse, with_offsets, dy=None) -> _LinearPlan:
     return _linear_plan((q.dtype, k.dtype, v.dtype), (q.device, k.device, v.device), q.shape, q.stride(), k.shape, k.stride(), v.shape,
-                        v.stride(), (0, 0) if dy is None else dy.stride(), n_rows, scale, reverse, with_offsets)
+                        v.stride(), (0, 0) if dy is None else dy.stride(), n_rows, None if scale is None else float(scale), reverse,
+                        with_offsets)
 
 
 class _LinearAttention(torch.autograd.Function):
@@ -334,8 +335,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     :func:`gated_scan` (rows may be empty; tokens in no row give zeros, also as gradients), or dense rows [B, T, .., ..]
     without offsets (copied where they do not lie like packed ones); float32, bfloat16 or float16, the elements of a head
     next to each other (parts of one projection's output will do).  H is a multiple of G: neighbouring heads share keys and
-    values.  Dk and Dv go up to 128.  ``log_decay`` float32 [H] is at most 0 (-inf: nothing is kept); ``scale`` is
-    Dk ** -0.5 if not given.  ``h0`` float32 [B, H, Dk, Dv] is the state in front of each row, zero if not given; ``reverse``
+    values.  Dk and Dv go up to 128.  ``log_decay`` float32 [H] is at most 0 (-inf: nothing is kept); ``scale`` is a number of
+    2^-40 to 2^40 in size, Dk ** -0.5 if not given.  ``h0`` float32 [B, H, Dk, Dv] is the state in front of each row, zero if not given; ``reverse``
     runs rows from their last token to their first.  States and sums are held in 32 bits.  Differentiable (once) with
     respect to q, k, v and h0."""
     _require_floats(q, "q")
@@ -419,6 +420,11 @@ def _host_float(value: float) -> Tuple[ctypes.c_float, int]:
     return held, ctypes.addressof(held)
 
 
+@functools.lru_cache(maxsize=1024)
+def _embedding_work(n: int, vocab: int, dim: int) -> int:
+    return _lib.lib().dnatok_embedding_work_bytes(n, vocab, dim)
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale):
@@ -429,24 +435,26 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        (ids,), (vocab, dim), device, L = ctx.saved_tensors, ctx.shape, dy.device, _lib.lib()
+        (ids,), (vocab, dim), device = ctx.saved_tensors, ctx.shape, dy.device
         n = ids.numel()
         dy = dy.reshape(n, dim)
         if dim > 1 and dy.stride(1) != 1:
             dy = dy.contiguous()
         grad = torch.empty((vocab, dim), dtype=ctx.dtype, device=device)
-        need = L.dnatok_embedding_work_bytes(n, vocab, dim)
+        need = _embedding_work(n, vocab, dim)
         work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        held, at = _host_float(ctx.scale)
         _run("dnatok_embedding_backward", device, ids.data_ptr(), ids.element_size(), n, dy.data_ptr(), dy.stride(0),
-             _DTYPES[ctx.dtype], vocab, dim, _host_float(ctx.scale)[1], grad.data_ptr(), _ptr(work), need)
+             _DTYPES[ctx.dtype], vocab, dim, at, grad.data_ptr(), _ptr(work), need)
         return None, grad, None
 
 
 def _embed(ids, weight, scale):
     vocab, dim = weight.shape
     y = torch.empty((*ids.shape, dim), dtype=weight.dtype, device=weight.device)
+    held, at = _host_float(scale)
     _run("dnatok_embedding", weight.device, ids.data_ptr(), ids.element_size(), ids.numel(), weight.data_ptr(), weight.stride(0),
-         _DTYPES[weight.dtype], vocab, dim, _host_float(scale)[1], y.data_ptr())
+         _DTYPES[weight.dtype], vocab, dim, at, y.data_ptr())
     return y
 
 

@@ -503,7 +503,7 @@ typedef struct dnatok_linear_shape {
     int32_t heads, kv_heads, dim_k, dim_v;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;
     int64_t dy_token, dy_head;         /* backward pass only */
-    float scale;                       /* finite and not 0 */
+    float scale;                       /* 2^-40 to 2^40 in size */
     int32_t with_offsets;              /* whether the call will have offsets (for the sizes of states and work) */
 } dnatok_linear_shape;
 
@@ -527,7 +527,7 @@ int dnatok_linear_attention_step(const dnatok_linear_shape *shape_h, const void 
                                  const float *log_decay, const float *state, void *y, float *new_state, void *stream);
 
 /* Rows of an embedding: y[t] = scale weight[ids[t]], [n, dim] of `dtype`, back to back; ids of 4 or 8 bytes; an id outside 0 ..
- * vocab - 1 gives a row of zeros.  scale_h points to host memory. */
+ * vocab - 1 gives a row of zeros.  scale_h points to a finite number in host memory. */
 int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, const void *weight, int64_t weight_stride, int32_t dtype,
                      int64_t vocab, int64_t dim, const float *scale_h, void *y, void *stream);
 

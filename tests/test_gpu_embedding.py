@@ -66,6 +66,13 @@ def test_tokens_and_types(n, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 64, 65, 127, 128, 129, 130])
+@pytest.mark.parametrize("vocab,dim", [(1, 40), (3, 5), (11, 203), (5000, 64), (270001, 8)])
+def test_few_tokens(vocab, dim, n, dtype):
+    check(n, vocab, dim, dtype, -0.25, outside=0.2, seed=n, idtype=torch.int64 if n % 2 else torch.int32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [1, 2, 3, 7, 8, 9, 63, 64, 65, 100, 203, 255, 256, 257, 512, 513, 1000, 1024, 2048, 2049])
 def test_dims(dim, dtype):
     check(700, 50, dim, dtype, 3.0)

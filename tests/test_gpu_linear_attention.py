@@ -355,3 +355,15 @@ def test_refusals():
     with pytest.raises(ValueError, match="overlaps"):
         part = h0.view(-1)[:2 * 4 * 8].view(2, 4, 8)
         lm_ops.linear_attention_step(part, k[:2], v[:2], ld, h0, out_state=h0)
+
+
+def test_a_scale_that_is_changed_in_place():
+    """The scale is taken as the number that it is when it is given."""
+    q, k, v, ld, off, h0, _, _ = inputs([9, 3], 2, 2, 8, 8, torch.float32)
+    scale, offsets = torch.tensor(1.0), torch.tensor(off, device=DEV)
+    one, _ = lm_ops.linear_attention(q, k, v, ld, offsets, h0=h0, scale=scale)
+    scale.fill_(2.0)                               # (twice each result, exactly)
+    two, _ = lm_ops.linear_attention(q, k, v, ld, offsets, h0=h0, scale=scale)
+    assert torch.equal(two, one * 2)
+    with pytest.raises(ValueError):
+        lm_ops.linear_attention(q, k, v, ld, offsets, scale=2.0 ** -50)

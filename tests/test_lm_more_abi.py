@@ -40,7 +40,7 @@ def step(**change):
 
 
 BAD = [dict(dtype=3), dict(dtype=-1), dict(n_rows=-1), dict(total=-1), dict(heads=0), dict(kv_heads=0), dict(heads=3), dict(dim_k=0),
-       dict(dim_v=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q_token=-64), dict(k_head=-16),
+       dict(dim_v=-1), dict(scale=0.0), dict(scale=2.0 ** -41), dict(scale=-2.0 ** 41), dict(scale=float("nan")), dict(scale=float("inf")), dict(q_token=-64), dict(k_head=-16),
        dict(v_token=-1), dict(dy_head=-24)]
 LARGE = [dict(dim_k=129), dict(dim_v=129), dict(q_token=2 ** 40), dict(k_token=2 ** 31 // 256), dict(v_token=2 ** 62), dict(heads=65536, kv_heads=1),
          dict(dy_token=2 ** 25)]
@@ -61,6 +61,8 @@ def test_attention_refuses_calls_that_do_not_fit():
     assert forward(work_bytes=16, **cut) == INVALID and forward(work=None, **cut) == INVALID and forward(work=P + 4, **cut) == INVALID
     assert backward(work_bytes=16, **cut) == INVALID and backward(states=None, **cut) == INVALID
     assert forward(n_rows=1 << 24, total=1 << 24) == TOO_LARGE
+    single = dict(heads=1, kv_heads=1, n_rows=1 << 23, total=1 << 23)
+    assert forward(**single) == TOO_LARGE and backward(**single) == TOO_LARGE          # a grid has less than 2^32 threads
     assert _lib.lib().dnatok_linear_attention(None, P, P, P, P, None, None, P, P, None, P, 0, None) == INVALID
     assert _lib.lib().dnatok_linear_attention_step(shape(n_rows=65536), P, P, P, P, P, P, P, None) == TOO_LARGE
     assert _lib.lib().dnatok_linear_attention_work_bytes(None, 1) == 0
@@ -69,6 +71,7 @@ def test_attention_refuses_calls_that_do_not_fit():
 def test_embedding_refuses():
     L, one = _lib.lib(), ctypes.c_float(1.0)
     at = ctypes.addressof(one)
+    odd = [ctypes.c_float(float(x)) for x in ("inf", "nan")]
 
     def rows(ids=P, id_bytes=4, n=8, weight=P, stride=16, dtype=1, vocab=4, dim=16, scale=at, y=P):
         return L.dnatok_embedding(ids, id_bytes, n, weight, stride, dtype, vocab, dim, scale, y, None)
@@ -76,13 +79,13 @@ def test_embedding_refuses():
     def grad(ids=P, id_bytes=4, n=8, dy=P, stride=16, dtype=1, vocab=4, dim=16, scale=at, out=P, work=P, work_bytes=1 << 40):
         return L.dnatok_embedding_backward(ids, id_bytes, n, dy, stride, dtype, vocab, dim, scale, out, work, work_bytes, None)
 
-    common = [dict(id_bytes=2), dict(n=-1), dict(vocab=-1), dict(dim=-1), dict(stride=-16), dict(dtype=7), dict(ids=None), dict(scale=None)]
-    for call, more in ((rows, [dict(weight=None), dict(y=None)]), (grad, [dict(dy=None), dict(out=None), dict(work_bytes=8), dict(work=None),
-                                                                          dict(work=P + 8)])):
+    common = [*(dict(scale=ctypes.addressof(x)) for x in odd), dict(id_bytes=2), dict(n=-1), dict(vocab=-1), dict(dim=-1), dict(stride=-16), dict(dtype=7), dict(ids=None), dict(scale=None)]
+    for call, more in ((rows, [dict(weight=None), dict(y=None)]), (grad, [dict(dy=None), dict(out=None), dict(n=500, work_bytes=8),
+                                                                          dict(n=500, work=None), dict(n=500, work=P + 8)])):
         assert [call(**c) for c in common + more] == [INVALID] * len(common + more)
         assert [call(**c) for c in (dict(n=2 ** 31), dict(vocab=2 ** 31), dict(dim=2 ** 23))] == [TOO_LARGE] * 3
     assert rows(n=0) == 0 and rows(dim=0) == 0 and grad(vocab=0) == 0 and grad(dim=0) == 0       # nothing to do
-    assert L.dnatok_embedding_work_bytes(0, 10, 10) == 0
+    assert L.dnatok_embedding_work_bytes(0, 10, 10) == 0 and L.dnatok_embedding_work_bytes(500, 10, 10) > 0
 
 
 def test_beam_search_refuses():
@@ -95,7 +98,7 @@ def test_beam_search_refuses():
     bad = [dict(dtype=5), dict(groups=-1), dict(beams=0), dict(vocab=0), dict(width=0), dict(stride=-1), dict(logits=None), dict(scores=None),
            dict(out=None), dict(work=None), dict(work_bytes=8), dict(work=P + 8), dict(finished=P, eos=100), dict(finished=P, eos=-1)]
     assert [select(**c) for c in bad] == [INVALID] * len(bad)
-    assert [select(**c) for c in (dict(beams=129), dict(width=129), dict(vocab=2 ** 31), dict(groups=2 ** 31))] == [TOO_LARGE] * 4
+    assert [select(**c) for c in (dict(beams=129), dict(width=129), dict(vocab=2 ** 31), dict(groups=2 ** 31), dict(groups=2 ** 26, beams=1))] == [TOO_LARGE] * 5
     assert select(groups=0) == 0
     rows = (ctypes.c_int64 * 5)(P, P, 16, 16, 16)
     at = ctypes.addressof(rows)
