@@ -50,7 +50,8 @@ template <typename T> __device__ __forceinline__ int64_t words_at(int64_t dim)
 
 constexpr int kEmbedAhead = 8;                     // rows that a wave has under way
 
-// A wave copies a run of tokens' rows, sixteen bytes to a lane.
+// A wave copies a run of tokens' rows, sixteen bytes to a lane, eight rows under way.  Bound by the writes: 524,288 rows of 512 bfloat16
+// (537 MB; the table stays in the caches) 113 us, 4.75 TB/s, as much as a copy; 1,000,003 rows of 203 floats 168 us, 4.8 TB/s.
 template <typename T, typename ID>
 __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, int32_t run, const T *weight, int64_t w_stride,
                                                     int64_t vocab, int64_t dim, float scale, T *y)
@@ -84,9 +85,11 @@ __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, in
 
 // Keys are ids, those outside the table the number behind its last row.  A pass sorts by up to eight of their bits: a workgroup
 // counts its tile's digits, a scan gives each tile its place for each digit, and a workgroup writes its tile there, the tokens of one
-// digit in their order.  So tokens of one id stay in their order, and a sum over them is the same in every call.
+// digit in their order.  So tokens of one id stay in their order, and a sum over them is the same in every call.  Tiles of 1,024 tokens:
+// a pass over 262,144 takes 5 + 3 + 7 us.  (Tiles of 8,192 leave CUs without work: 40,000 tokens and 32,000 ids 108 us for the whole
+// gradient instead of 46, 262,144 163 instead of 99, 8,000,000 no difference.)
 constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64, kDigits = 256;
-constexpr int kFewPerLane = 4, kManyPerLane = 32;    // tokens of a tile to a thread: tiles of 1,024, or of 8,192 above 2^22 tokens
+constexpr int kSortPerLane = 4, kSortTile = kSortThreads * kSortPerLane;
 constexpr int kSmallSort = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
 
 struct Token {
@@ -108,23 +111,23 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool he
     return same;
 }
 
-template <typename ID, int PER>
+template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
                                                                   int shift, int bits, uint32_t *counts)
 {
     __shared__ uint32_t count[kDigits];
     for (int i = threadIdx.x; i < kDigits; i += kSortThreads) count[i] = 0;
     __syncthreads();
-    const uint32_t first = blockIdx.x * (kSortThreads * PER), mask = (1u << bits) - 1;
+    const uint32_t first = blockIdx.x * kSortTile, mask = (1u << bits) - 1;
     const int lane = threadIdx.x & 63;
-    uint32_t key[PER];
+    uint32_t key[kSortPerLane];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
+    for (int j = 0; j < kSortPerLane; ++j) {
         const uint32_t i = first + j * kSortThreads + threadIdx.x;
         key[j] = i < n ? (ids ? key_of(ids[i], vocab) : tokens[i].key) : 0;
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
+    for (int j = 0; j < kSortPerLane; ++j) {
         const bool here = first + j * kSortThreads + threadIdx.x < n;
         const uint32_t digit = key[j] >> shift & mask;
         const uint64_t same = same_digit(digit, bits, here);
@@ -154,19 +157,19 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t *counts, uint32
     if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-template <typename ID, int PER>
+template <typename ID>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const ID *ids, const Token *tokens, uint32_t n, uint32_t vocab,
                                                                   int shift, int bits, const uint32_t *counts, const uint32_t *totals,
                                                                   Token *out)
 {
     __shared__ uint32_t place[kSortWaves][kDigits], part[4];
-    constexpr int kPerLane = PER;
+    constexpr int kPerLane = kSortPerLane;
     const uint32_t mask = (1u << bits) - 1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) place[0][i] = 0;
     __syncthreads();
     // a wave has neighbouring tokens, 64 at a time
-    const uint32_t first = blockIdx.x * (kSortThreads * PER) + wave * (64 * PER);
+    const uint32_t first = blockIdx.x * kSortTile + wave * (64 * kPerLane);
     uint32_t key[kPerLane], at[kPerLane];
     uint64_t same[kPerLane];
 #pragma unroll
@@ -224,7 +227,8 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const ID *ids,
     }
 }
 
-// Up to kSmallSort tokens in one workgroup: the same passes in LDS.
+// Up to kSmallSort tokens in one workgroup: the same passes in LDS, one launch instead of six.  (The whole gradient for 2,500 and 8,000
+// tokens, 32,000 rows of 512 bfloat16: 28 and 33 us, with launches of their own 35 and 37.)
 template <typename ID>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(const ID *ids, uint32_t n, uint32_t vocab, int passes, int bits,
                                                                    Token *out)
@@ -316,7 +320,8 @@ __device__ __forceinline__ uint32_t first_of(const Token *tokens, uint32_t n, ui
 
 // A wave to a tile of the sorted tokens and 64 x 16 bytes of their rows: it adds up runs of one id.  A run inside the tile is a
 // row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts [tiles, 2, dim].  Further waves clear the
-// rows of ids that do not occur.
+// rows of ids that do not occur.  Eight rows of dy under way: 262,144 rows of 512 bfloat16 in the order of 32,000 ids 89 us (301 MB,
+// 3.4 TB/s), 1,000,003 rows of 203 floats and 12 ids 227 us (812 MB, 3.6 TB/s).  (Sixteen rows under way: 118 instead of 89.)
 template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, float *parts, T *grad)
 {
     typedef Words<T> W;
@@ -524,10 +529,11 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
         using T = decltype(t);
         with_ids(id_bytes, [&](auto i) {
             using ID = decltype(i);
-            // runs of a multiple of kEmbedAhead tokens, some 16,384 waves where there are so many
-            const int64_t blocks = blocks_of(dim, sizeof(T)), waves = 16384 / blocks + 1;
-            int64_t run = (n + waves - 1) / waves;
-            run = (run + kEmbedAhead - 1) / kEmbedAhead * kEmbedAhead;
+            // sixteen tokens to a wave, or eight if that leaves it no more than 32,768 (524,288 rows of 512 bfloat16: 113.1 us with
+            // sixteen, 114.5 with eight, 115.9 with 32; 1,000,003 of 203 floats: 168 with sixteen, 178 with 32, 183 with 64)
+            const int64_t blocks = blocks_of(dim, sizeof(T));
+            int64_t run = n * blocks <= 32768 * kEmbedAhead ? kEmbedAhead : 2 * kEmbedAhead;
+            while (n / run > (1 << 22)) run *= 2;  // (a grid ends at 2^32 threads)
             embed_kernel<T, ID><<<dim3((unsigned)((n + run * 4 - 1) / (run * 4)), (unsigned)blocks), 256, 0, (hipStream_t)stream>>>(
                 (const ID *)ids, n, (int32_t)run, (const T *)weight, weight_stride, vocab, dim, scale, (T *)y);
         });
@@ -539,7 +545,7 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
 // What the backward pass needs besides its arguments: tokens sorted by id (twice, where they go from one place to the other), counts of
 // digits, and parts of sums.
 struct GradPlan {
-    uint32_t tiles, sort_tiles, sort_tile;
+    uint32_t tiles, sort_tiles;
     int32_t run, passes, bits;
     size_t other, counts, totals, parts, bytes;    // offsets
 };
@@ -550,12 +556,12 @@ static GradPlan plan_of(int64_t n, int64_t vocab, int64_t dim)
     while ((vocab >> bits) != 0) ++bits;           // (keys go up to vocab itself)
     p.passes = (bits + 7) / 8;
     p.bits = (bits + p.passes - 1) / p.passes;
-    p.sort_tile = kSortThreads * (n <= (1 << 22) ? kFewPerLane : kManyPerLane);
-    p.sort_tiles = (uint32_t)((n + p.sort_tile - 1) / p.sort_tile);
-    // tiles as long as leaves some 2,048 waves; shorter ones write more parts of sums, longer ones leave CUs without work
-    const int64_t blocks = blocks_of(dim, 2);
+    p.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
+    // about 2,048 waves if a row fills one with 16-bit elements, more if it leaves lanes idle: shorter tiles write more parts of sums,
+    // longer ones leave CUs without work (the whole gradient, bfloat16: 262,144 x 512 99 us, with half or twice the waves 111 and 108;
+    // 1,000,003 x 203 149, 166 and 172; 8,000,000 x 32, 16,384 waves, 727, 778 and, with a quarter, 970)
     p.run = 16;
-    while (p.run < (1 << 20) && n / p.run * blocks > 2048) p.run *= 2;
+    while (p.run < (1 << 20) && n / p.run * (dim < 64 ? 64 : dim) > (1 << 20)) p.run *= 2;
     p.tiles = (uint32_t)((n + p.run - 1) / p.run);
     const bool small = n <= kSmallSort;
     const auto place = [&](size_t bytes) {
@@ -587,13 +593,9 @@ static const Token *sort_tokens(const ID *ids, uint32_t n, uint32_t vocab, const
     uint32_t *counts = (uint32_t *)(work + p.counts), *totals = (uint32_t *)(work + p.totals);
     for (int pass = 0; pass < p.passes; ++pass) {
         const ID *source = pass ? nullptr : ids;
-        const auto sort = [&](auto per) {
-            sort_count_kernel<ID, per()><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts);
-            sort_scan_kernel<<<1u << p.bits, 256, 0, s>>>(counts, p.sort_tiles, totals);
-            sort_place_kernel<ID, per()><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts, totals, to);
-        };
-        if (p.sort_tile == kSortThreads * kFewPerLane) sort(std::integral_constant<int, kFewPerLane>{});
-        else sort(std::integral_constant<int, kManyPerLane>{});
+        sort_count_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts);
+        sort_scan_kernel<<<1u << p.bits, 256, 0, s>>>(counts, p.sort_tiles, totals);
+        sort_place_kernel<ID><<<p.sort_tiles, kSortThreads, 0, s>>>(source, from, n, vocab, pass * p.bits, p.bits, counts, totals, to);
         std::swap(from, to);
     }
     return from;

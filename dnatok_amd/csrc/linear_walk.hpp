@@ -239,8 +239,10 @@ __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); 
 
 // ---- the walk ----------------------------------------------------------------------------------------
 
-// Whether LDS holds two chunks of the operands, so that the next one is there when a chunk is done.
-template <typename T, int KD, int CD> constexpr bool kTwoChunks = sizeof(T) == 2 && (KD <= 64 || CD > 64);
+// Whether LDS holds two chunks of the operands, so that the next one is there when a chunk is done: where a workgroup has the CU to
+// itself.  (256 rows of 1,024 tokens and 4 heads of 128 x 128: 336 us, with one chunk 346; smaller heads have a second workgroup on
+// the CU, and want the room: 128 x 64 takes 209, with two 275; 64 rows of 8,192 and 8 heads of 64 x 64 506, with two 542.)
+template <typename T, int KD, int CD> constexpr bool kTwoChunks = sizeof(T) == 2 && KD > 64 && CD > 64;
 
 template <typename T, int KD, int CD> struct alignas(16) Chunk {
     Tile<T, KD> a, b;
@@ -383,6 +385,14 @@ __device__ __forceinline__ const char *base_of(const Operand &o, int head, int s
 
 // One workgroup to a piece of a row and a head.  A wave has sixteen of the state's columns, which no other wave needs; scores are
 // shared.  Of 32-bit operands no more than one workgroup of four waves fits beside tiles of 128 x 64.
+//
+// 64 x 64 of bfloat16, 64 rows of 8,192 tokens, 8 heads: 500 us for 2.15 GB, 4.3 TB/s of the 4.75 that a copy reaches.  128 x 128, 256 rows
+// of 1,024 tokens, 4 heads: 340 us for 1.07 GB, bound by the length of a chunk's chain (scores, barrier, two products, state) with
+// two waves to a SIMD: matrix instructions busy 0.25, vector 0.38; without the loads it takes 12 % less, without the state's
+// products 18 %, with one part of scores and T instead of two 7 %.  (The columns of a head in two workgroups, which each compute all
+// scores, took 7 % more.  With 64 x 64, three workgroups to a CU spill registers: 888 us instead of 508.)
+// 48 x 40 in 32 bits, 876,000 tokens of long reads, 6 heads: 1,510 us, matrix instructions of 32 bits busy 0.39.  (As two float16
+// each, three products instead of one: a training step took 8,690 instead of 7,230, with registers spilled.)
 template <typename T, int KD, int CD, bool TAIL>
 __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 64 ? 1 : 2) void walk_kernel(WalkArgs w)
 {
@@ -693,7 +703,8 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     }
 }
 
-// What each piece that does not end its row adds to the state: into the slot of the cut behind it.
+// What each piece that does not end its row adds to the state: into the slot of the cut behind it.  One row of 262,147 tokens, 4 heads of
+// 128 x 128 of float16: 140 us for 0.54 GB, 30 more for the slots' states, then the walk.
 template <typename T, int KD, int CD, bool TAIL>
 __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 64 ? 1 : 2) void piece_kernel(WalkArgs w)
 {
