@@ -5,14 +5,17 @@
 namespace dnatok {
 
 constexpr int kSlotThreads = 256;
+__host__ __device__ __forceinline__ int64_t slot_parts(const WalkArgs &w)
+{
+    return ((int64_t)w.b.dim * w.c.dim + kSlotThreads - 1) / kSlotThreads;
+}
 
 // The slots' states from what the pieces add: a thread has one cell of a head's state and runs through a row's cuts.  What comes next is
 // requested before what is done is stored (a wait for a load is one for the stores in front of it).  63 cuts of 4 heads of 128 x 128,
-// 33 MB: 31 us, four round trips of sixteen cuts each.
+// 33 MB: 35 us, four round trips of sixteen cuts each.
 __global__ __launch_bounds__(kSlotThreads) void slots_kernel(WalkArgs w)
 {
     constexpr int kAhead = 16;
-    const int head = blockIdx.y;
     const int64_t cells = (int64_t)w.b.dim * w.c.dim, cut = blockIdx.x + 1, at = cut * w.cut;
     const int64_t row = uniform(last_row(w.n_rows, at, [&](int64_t r) { return row_at(w, r); }));
     if (row < 0) return;
@@ -20,29 +23,32 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(WalkArgs w)
     if (at <= lo || at >= hi) return;
     const int64_t first = lo / w.cut + 1, last = (hi - 1) / w.cut, n = last - first + 1;
     if (cut != (w.reverse ? last : first)) return;
-    const int64_t i = (int64_t)blockIdx.z * kSlotThreads + threadIdx.x;
-    if (i >= cells) return;
-    const float ld = log_decay_of(w, head);
-    float state = w.start ? w.start_scale * w.start[(row * w.heads + head) * cells + i] : 0.0f;
     const int64_t outer = w.reverse ? hi - last * w.cut : first * w.cut - lo;
-    const Left left = left_after(ld, (float)w.cut);
-    state = decayed(state, left_after(ld, (float)outer));
-    float *slot = w.slots + ((w.reverse ? last : first) - 1) * w.heads * cells + head * cells + i;
     const int64_t next = (w.reverse ? -1 : 1) * w.heads * cells;
-    float added[kAhead], coming[kAhead];
+    for (int64_t at_once = blockIdx.y; at_once < slot_parts(w) * w.heads; at_once += gridDim.y) {
+        const int head = (int)(at_once % w.heads);
+        const int64_t i = at_once / w.heads * kSlotThreads + threadIdx.x;
+        if (i >= cells) continue;
+        const float ld = log_decay_of(w, head);
+        float state = w.start ? w.start_scale * w.start[(row * w.heads + head) * cells + i] : 0.0f;
+        const Left left = left_after(ld, (float)w.cut);
+        state = decayed(state, left_after(ld, (float)outer));
+        float *slot = w.slots + ((w.reverse ? last : first) - 1) * w.heads * cells + head * cells + i;
+        float added[kAhead], coming[kAhead];
 #pragma unroll
-    for (int e = 0; e < kAhead; ++e) added[e] = e < n ? slot[e * next] : 0.0f;
-    for (int64_t j = 0; j < n; j += kAhead) {
+        for (int e = 0; e < kAhead; ++e) added[e] = e < n ? slot[e * next] : 0.0f;
+        for (int64_t j = 0; j < n; j += kAhead) {
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) coming[e] = j + kAhead + e < n ? slot[(kAhead + e) * next] : 0.0f;
+            for (int e = 0; e < kAhead; ++e) coming[e] = j + kAhead + e < n ? slot[(kAhead + e) * next] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) {
-            state += added[e];
-            if (j + e < n) slot[e * next] = state;
-            state = decayed(state, left);
-            added[e] = coming[e];
+            for (int e = 0; e < kAhead; ++e) {
+                state += added[e];
+                if (j + e < n) slot[e * next] = state;
+                state = decayed(state, left);
+                added[e] = coming[e];
+            }
+            slot += kAhead * next;
         }
-        slot += kAhead * next;
     }
 }
 
@@ -189,8 +195,10 @@ template <typename T> static void fill_slots(const WalkArgs &w, hipStream_t s)
 {
     if (!w.cuts) return;
     launch_pieces<T>(w, s);
-    const unsigned parts = (unsigned)((w.b.dim * w.c.dim + kSlotThreads - 1) / kSlotThreads);
-    slots_kernel<<<dim3((unsigned)w.cuts, (unsigned)w.heads, parts), kSlotThreads, 0, s>>>(w);
+    // about 8,192 workgroups: most cuts begin no row's slots and leave at once, but one row's may be all that there is (255 cuts of 256
+    // rows, 4 heads of 128 x 128: 10 us, a workgroup to each part 29, 1,024 workgroups 5; 63 cuts of one row 35, 36 and 127)
+    const int64_t all = slot_parts(w) * w.heads, some = 8192 / w.cuts + 1;
+    slots_kernel<<<dim3((unsigned)w.cuts, (unsigned)(all < some ? all : some)), kSlotThreads, 0, s>>>(w);
 }
 
 extern "C" size_t dnatok_linear_attention_states_bytes(const dnatok_linear_shape *s)
