@@ -39,11 +39,25 @@ template <typename T> __device__ __forceinline__ void store_words(T *row, int64_
 
 // Where a lane's sixteen bytes begin: the last ones of a row end with it, so that they overlap those in front of them and hold (and write)
 // the same values there.  -1: none.  (Only rows of less than sixteen bytes are taken by elements.)
-template <typename T> __device__ __forceinline__ int64_t words_at(int64_t dim)
+template <typename T> __device__ __forceinline__ int64_t word_at(int64_t word, int64_t dim)
 {
-    const int64_t at = ((int64_t)blockIdx.y * 64 + (threadIdx.x & 63)) * Words<T>::kCount;
+    const int64_t at = word * Words<T>::kCount;
     if (at >= dim) return -1;
     return at + Words<T>::kCount > dim && dim >= Words<T>::kCount ? dim - Words<T>::kCount : at;
+}
+template <typename T> __device__ __forceinline__ int64_t words_at(int64_t dim)
+{
+    return word_at<T>((int64_t)blockIdx.y * 64 + (threadIdx.x & 63), dim);
+}
+
+// Rows that fill no more than half of a wave: 64 >> shift of them lie next to each other in it.  -1: wider ones.
+static int narrow_shift(int64_t dim, int64_t size)
+{
+    const int64_t words = (dim * size + 15) / 16;
+    if (words > 32) return -1;
+    int shift = 0;
+    while ((1 << shift) < words) ++shift;
+    return shift;
 }
 
 // ---- rows for ids --------------------------------------------------------------------------------------
@@ -78,6 +92,34 @@ __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, in
             store_words(y + (t0 + i) * dim, at, dim,
                         __builtin_convertvector(__builtin_convertvector(v[i], typename W::floats) * scale, typename W::type));
         }
+    }
+}
+
+// The same for narrow rows.  (1,000,000 rows of 16, 64, 128 and 256 bfloat16: 12, 25, 44 and 103 us, with a row to a wave 63, 63, 66 and
+// 123; bytes written at the rate of a copy 7, 27, 54 and 108.)
+template <typename T, typename ID>
+__global__ __launch_bounds__(256) void embed_narrow_kernel(const ID *ids, int64_t n, int32_t run, int shift, const T *weight, int64_t w_stride,
+                                                           int64_t vocab, int64_t dim, float scale, T *y)
+{
+    typedef Words<T> W;
+    const int lane = threadIdx.x & 63, mine = lane >> shift, rows = 64 >> shift;
+    const int64_t first = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * run, end = n - first < run ? n : first + run;
+    const int64_t at = word_at<T>(lane & ((1 << shift) - 1), dim);
+    for (int64_t t0 = first + mine; t0 < end; t0 += kEmbedAhead * rows) {
+        int64_t id[kEmbedAhead];
+        typename W::type v[kEmbedAhead];
+#pragma unroll
+        for (int i = 0; i < kEmbedAhead; ++i) id[i] = t0 + i * rows < end ? (int64_t)ids[t0 + i * rows] : -1;
+#pragma unroll
+        for (int i = 0; i < kEmbedAhead; ++i) {
+            v[i] = typename W::type{};
+            if (id[i] >= 0 && id[i] < vocab && at >= 0) v[i] = load_words(weight + id[i] * w_stride, at, dim);
+        }
+#pragma unroll
+        for (int i = 0; i < kEmbedAhead; ++i)
+            if (t0 + i * rows < end && at >= 0)
+                store_words(y + (t0 + i * rows) * dim, at, dim,
+                            __builtin_convertvector(__builtin_convertvector(v[i], typename W::floats) * scale, typename W::type));
     }
 }
 
@@ -228,7 +270,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const ID *ids,
 }
 
 // Up to kSmallSort tokens in one workgroup: the same passes in LDS, one launch instead of six.  (The whole gradient for 2,500 and 8,000
-// tokens, 32,000 rows of 512 bfloat16: 28 and 33 us, with launches of their own 35 and 37.)
+// tokens, 32,000 rows of 512 bfloat16: 30 and 35 us, with launches of their own 37 and 39.)
 template <typename ID>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(const ID *ids, uint32_t n, uint32_t vocab, int passes, int bits,
                                                                    Token *out)
@@ -318,6 +360,42 @@ __device__ __forceinline__ uint32_t first_of(const Token *tokens, uint32_t n, ui
     return lo;
 }
 
+// The rows of ids that do not occur, for a wave's kZeroRows rows.
+template <typename T> __device__ __forceinline__ void clear_absent(const GradArgs &a, uint32_t rows, T *grad)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t at = words_at<T>(a.dim);
+    const uint32_t row = rows * kZeroRows + lane;
+    bool empty = row < a.vocab;
+    if (empty) {
+        const uint32_t i = first_of(a.tokens, a.n, row);
+        empty = i == a.n || a.tokens[i].key != row;
+    }
+    uint64_t left = __ballot(empty);
+    while (left) {
+        const int i = __builtin_ctzll(left);
+        left &= left - 1;
+        if (at >= 0) store_words(grad + (int64_t)(row - lane + i) * a.dim, at, a.dim, typename Words<T>::type{});
+    }
+}
+
+// A lane's part of a run's sum: a row of the gradient, or of `part` if the run goes on outside of the tile.
+template <typename T> __device__ __forceinline__ void put_sum(const GradArgs &a, uint32_t key, bool goes_on, float *part, T *grad, int64_t at,
+                                                              const typename Words<T>::floats &sum)
+{
+    typedef Words<T> W;
+    if (key >= a.vocab || at < 0) return;
+    if (!goes_on) {
+        store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
+    } else if (at + W::kCount <= a.dim) {
+        __builtin_memcpy(part + at, &sum, sizeof(sum));
+    } else {
+#pragma unroll
+        for (int i = 0; i < W::kCount; ++i)
+            if (at + i < a.dim) part[at + i] = sum[i];
+    }
+}
+
 // A wave to a tile of the sorted tokens and 64 x 16 bytes of their rows: it adds up runs of one id.  A run inside the tile is a
 // row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts [tiles, 2, dim].  Further waves clear the
 // rows of ids that do not occur.  Eight rows of dy under way: 262,144 rows of 512 bfloat16 in the order of 32,000 ids 89 us (301 MB,
@@ -329,18 +407,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
     const int64_t at = words_at<T>(a.dim);
     const uint32_t tile = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (tile >= (a.tiles + 3) / 4 * 4) {
-        const uint32_t row = (tile - (a.tiles + 3) / 4 * 4) * kZeroRows + lane;
-        bool empty = row < a.vocab;
-        if (empty) {
-            const uint32_t i = first_of(a.tokens, a.n, row);
-            empty = i == a.n || a.tokens[i].key != row;
-        }
-        uint64_t rows = __ballot(empty);
-        while (rows) {
-            const int i = __builtin_ctzll(rows);
-            rows &= rows - 1;
-            if (at >= 0) store_words(grad + (int64_t)(row - lane + i) * a.dim, at, a.dim, typename W::type{});
-        }
+        clear_absent(a, tile - (a.tiles + 3) / 4 * 4, grad);
         return;
     }
     if (tile >= a.tiles) return;
@@ -350,19 +417,7 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
     uint32_t key = a.tokens[begin].key;
     bool from_front = key == front;
     const auto finish = [&](bool goes_on) {
-        if (key >= a.vocab || at < 0) return;
-        if (from_front || goes_on) {
-            float *part = parts + ((int64_t)tile * 2 + !from_front) * a.dim;
-            if (at + W::kCount <= a.dim) {
-                __builtin_memcpy(part + at, &sum, sizeof(sum));
-            } else {
-#pragma unroll
-                for (int i = 0; i < W::kCount; ++i)
-                    if (at + i < a.dim) part[at + i] = sum[i];
-            }
-        } else {
-            store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
-        }
+        put_sum<T>(a, key, from_front || goes_on, parts + ((int64_t)tile * 2 + !from_front) * a.dim, grad, at, sum);
     };
     for (uint32_t t0 = begin; t0 < end; t0 += 64) {
         const uint32_t mine_at = t0 + lane < end ? t0 + lane : end - 1;
@@ -394,9 +449,63 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(G
     finish(key == back);
 }
 
+// The same for rows that fill no more than a quarter of a wave: 64 >> shift tiles to a wave, each with as many of its lanes.  (1,000,000 x 64
+// bfloat16: 32 us, with a tile to a wave and twice the tiles 60; of two rows to a wave 1,000,000 x 192 takes 160 us instead of 157.)
+template <typename T> __global__ __launch_bounds__(256) void embed_grad_narrow_kernel(GradArgs a, int shift, float *parts, T *grad)
+{
+    typedef Words<T> W;
+    const int lane = threadIdx.x & 63, rows = 64 >> shift;
+    const uint32_t blocks = (a.tiles + rows * 4 - 1) / (rows * 4);
+    if (blockIdx.x >= blocks) {
+        clear_absent(a, (blockIdx.x - blocks) * 4 + (threadIdx.x >> 6), grad);
+        return;
+    }
+    const uint32_t tile = (blockIdx.x * 4 + (threadIdx.x >> 6)) * rows + (lane >> shift);
+    if (tile >= a.tiles) return;
+    const int64_t at = word_at<T>(lane & ((1 << shift) - 1), a.dim);
+    const uint32_t begin = tile * a.run, end = a.n - begin < (uint32_t)a.run ? a.n : begin + a.run;
+    const uint32_t front = begin ? a.tokens[begin - 1].key : ~0u, back = end < a.n ? a.tokens[end].key : ~0u;
+    typename W::floats sum{};
+    Token coming[kGradAhead];
+#pragma unroll
+    for (int i = 0; i < kGradAhead; ++i) coming[i] = a.tokens[begin + i < end ? begin + i : end - 1];
+    uint32_t key = coming[0].key;
+    bool from_front = key == front;
+    const auto finish = [&](bool goes_on) {
+        put_sum<T>(a, key, from_front || goes_on, parts + ((int64_t)tile * 2 + !from_front) * a.dim, grad, at, sum);
+    };
+    for (uint32_t t0 = begin; t0 < end; t0 += kGradAhead) {
+        Token token[kGradAhead];
+        typename W::type v[kGradAhead];
+#pragma unroll
+        for (int i = 0; i < kGradAhead; ++i) {
+            token[i] = coming[i];
+            v[i] = typename W::type{};
+            if (at >= 0) v[i] = load_words((const T *)a.dy + (int64_t)token[i].at * a.dy_stride, at, a.dim);
+        }
+#pragma unroll
+        for (int i = 0; i < kGradAhead; ++i) {
+            const uint32_t t = t0 + kGradAhead + i;
+            coming[i] = a.tokens[t < end ? t : end - 1];
+        }
+#pragma unroll
+        for (int i = 0; i < kGradAhead; ++i) {
+            if (t0 + i >= end) break;
+            if (token[i].key != key) {
+                finish(false);
+                key = token[i].key;
+                from_front = false;
+                sum = typename W::floats{};
+            }
+            sum += __builtin_convertvector(v[i], typename W::floats);
+        }
+    }
+    finish(key == back);
+}
+
 // Few tokens: a wave to a row of the gradient looks through all of their ids, and adds up what it finds.  One launch and no sort: 128
-// tokens take 4.3, 4.2 and 9.7 us with 12, 4,096 and 32,000 rows of 512 bfloat16 (sorted 13.3, 21.0 and 24.3), and where all are
-// one id, which one wave then adds up, 16.5, 16.8 and 22.6 (13.9, 22.7 and 26.0); 256 of one id take 31 (25).
+// tokens take 4.3, 4.5 and 9.4 us with 12, 4,096 and 32,000 rows of 512 bfloat16 (sorted 13.9, 22.6 and 25.5), and where all are
+// one id, which one wave then adds up, 16.5, 16.8 and 21.9 (15.0, 24.8 and 27.6); 256 of one id take 31 (27).
 constexpr int kFewTokens = 128;
 template <typename T, typename ID>
 __global__ __launch_bounds__(256) void embed_grad_few_kernel(const ID *ids, uint32_t n, const T *dy, int64_t dy_stride, int64_t vocab, int64_t dim,
@@ -425,38 +534,21 @@ __global__ __launch_bounds__(256) void embed_grad_few_kernel(const ID *ids, uint
     }
 }
 
-// A run that begins in one tile and ends in another: its parts, added up by sixteen waves and then in their order.
+// Runs that begin in one tile and end in another: their parts, added up in order.  A wave to a tile looks whether such a run begins there,
+// and adds it up by itself if it ends less than sixteen tiles on; a longer one is added up by the workgroup's waves and then in
+// their order.  (With a workgroup to each tile 7,800 tiles took 38 us, most of them to begin waves that leave at once.)
 constexpr int kJoinWaves = 16, kJoinAhead = 8;
 template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_join_kernel(GradArgs a, const float *parts, T *grad)
 {
     typedef Words<T> W;
     __shared__ typename W::floats part[kJoinWaves][64];
+    __shared__ uint32_t lasts[kJoinWaves], keys[kJoinWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t tile = blockIdx.x, begin = tile * (uint32_t)a.run, end = begin + (uint32_t)a.run;
-    if (end >= a.n) return;
-    const uint32_t next = end + (uint32_t)a.run < a.n ? end + (uint32_t)a.run : a.n - 1;
-    const uint32_t key = a.tokens[end].key, mine = a.tokens[end - 1].key, head = a.tokens[begin].key,
-                   front = begin ? a.tokens[begin - 1].key : ~0u, after = a.tokens[next].key;
-    if (key >= a.vocab || mine != key) return;
-    // (the run's first tile does it: it begins there, behind the tile's begin or at it with another id in front)
-    if (head == key && front == key) return;
-    uint32_t last = tile + 1;
-    if (after == key) {                            // the last token of the id: 64 places are looked at at once
-        uint32_t lo = next, hi = a.n;              // (lo has it, hi does not)
-        while (hi - lo > 1) {
-            const uint32_t step = (hi - lo - 1 + 63) / 64, at = lo + step * (lane + 1);
-            const int n = __popcll(__ballot(at < hi && a.tokens[at < hi ? at : lo].key == key));
-            lo += step * n;
-            hi = hi - lo > step ? lo + step : hi;
-        }
-        last = lo / (uint32_t)a.run;
-    }
     const int64_t at = words_at<T>(a.dim);
-    typename W::floats sum{};
-    const auto piece = [&](uint32_t t) {
+    const auto piece = [&](uint32_t t, uint32_t first, uint32_t last) {
         typename W::floats v{};
         if (t <= last && at >= 0) {
-            const float *p = parts + ((int64_t)t * 2 + (t == tile)) * a.dim;
+            const float *p = parts + ((int64_t)t * 2 + (t == first)) * a.dim;
             if (at + W::kCount <= a.dim) {
                 __builtin_memcpy(&v, p + at, sizeof(v));
             } else {
@@ -467,27 +559,66 @@ template <typename T> __global__ __launch_bounds__(kJoinWaves * 64) void embed_j
         }
         return v;
     };
-    if (last - tile < kJoinWaves) {                // few: one wave, no sums to be joined
-        if (wave) return;
-        for (uint32_t t = tile; t <= last; t += 2) {
-            const auto v = piece(t), u = piece(t + 1);
+    const auto put = [&](uint32_t key, const typename W::floats &sum) {
+        if (at >= 0) store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
+    };
+    // the last tile of the run that ends this one, if it begins here and goes on: it begins there, behind the tile's begin or at it with
+    // another id in front
+    const auto find = [&](uint32_t tile, uint32_t *of) -> uint32_t {
+        const uint32_t begin = tile * (uint32_t)a.run, end = begin + (uint32_t)a.run;
+        if (end >= a.n) return 0;
+        const uint32_t next = end + (uint32_t)a.run < a.n ? end + (uint32_t)a.run : a.n - 1;
+        const uint32_t key = a.tokens[end].key, mine = a.tokens[end - 1].key, head = a.tokens[begin].key,
+                       front = begin ? a.tokens[begin - 1].key : ~0u, after = a.tokens[next].key;
+        if (key >= a.vocab || mine != key || (head == key && front == key)) return 0;
+        *of = key;
+        if (after != key) return tile + 1;
+        uint32_t lo = next, hi = a.n;              // the last token of the id, 64 places at once (lo has it, hi does not)
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo - 1 + 63) / 64, place = lo + step * (lane + 1);
+            const int n = __popcll(__ballot(place < hi && a.tokens[place < hi ? place : lo].key == key));
+            lo += step * n;
+            hi = hi - lo > step ? lo + step : hi;
+        }
+        return lo / (uint32_t)a.run;
+    };
+    const uint32_t own = blockIdx.x * kJoinWaves + wave;
+    uint32_t key = 0, last = own < a.tiles ? find(own, &key) : 0;
+    if (last && last - own < kJoinWaves) {
+        typename W::floats sum{};
+        for (uint32_t t = own; t <= last; t += 2) {
+            const auto v = piece(t, own, last), u = piece(t + 1, own, last);
             sum += v;
             sum += u;
         }
-    } else {
-        for (uint32_t t = tile + wave; t <= last; t += kJoinWaves * kJoinAhead) {
+        put(key, sum);
+        last = 0;
+    }
+    if (lane == 0) {
+        lasts[wave] = last;
+        keys[wave] = key;
+    }
+    __syncthreads();
+    for (int w = 0; w < kJoinWaves; ++w) {
+        const uint32_t first = blockIdx.x * kJoinWaves + w;
+        last = lasts[w];
+        if (!last) continue;
+        typename W::floats sum{};
+        for (uint32_t t = first + wave; t <= last; t += kJoinWaves * kJoinAhead) {
             typename W::floats v[kJoinAhead];
 #pragma unroll
-            for (int i = 0; i < kJoinAhead; ++i) v[i] = piece(t + i * kJoinWaves);
+            for (int i = 0; i < kJoinAhead; ++i) v[i] = piece(t + i * kJoinWaves, first, last);
 #pragma unroll
             for (int i = 0; i < kJoinAhead; ++i) sum += v[i];
         }
         part[wave][lane] = sum;
         __syncthreads();
-        if (wave) return;
-        for (int w = 1; w < kJoinWaves; ++w) sum += part[w][lane];
+        if (wave == 0) {
+            for (int i = 1; i < kJoinWaves; ++i) sum += part[i][lane];
+            put(keys[w], sum);
+        }
+        __syncthreads();
     }
-    if (at >= 0) store_words(grad + (int64_t)key * a.dim, at, a.dim, __builtin_convertvector(sum * a.scale, typename W::type));
 }
 
 }  // namespace dnatok
@@ -531,6 +662,15 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
             using ID = decltype(i);
             // sixteen tokens to a wave, or eight if that leaves it no more than 32,768 (524,288 rows of 512 bfloat16: 113.1 us with
             // sixteen, 114.5 with eight, 115.9 with 32; 1,000,003 of 203 floats: 168 with sixteen, 178 with 32, 183 with 64)
+            const int shift = narrow_shift(dim, sizeof(T));
+            if (shift >= 0) {
+                const int64_t once = kEmbedAhead * (64 >> shift);
+                int64_t run = n <= 32768 * once ? once : 2 * once;
+                while (n / run > (1 << 22)) run *= 2;
+                embed_narrow_kernel<T, ID><<<(unsigned)((n + run * 4 - 1) / (run * 4)), 256, 0, (hipStream_t)stream>>>(
+                    (const ID *)ids, n, (int32_t)run, shift, (const T *)weight, weight_stride, vocab, dim, scale, (T *)y);
+                return;
+            }
             const int64_t blocks = blocks_of(dim, sizeof(T));
             int64_t run = n * blocks <= 32768 * kEmbedAhead ? kEmbedAhead : 2 * kEmbedAhead;
             while (n / run > (1 << 22)) run *= 2;  // (a grid ends at 2^32 threads)
@@ -557,11 +697,12 @@ static GradPlan plan_of(int64_t n, int64_t vocab, int64_t dim)
     p.passes = (bits + 7) / 8;
     p.bits = (bits + p.passes - 1) / p.passes;
     p.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
-    // about 2,048 waves if a row fills one with 16-bit elements, more if it leaves lanes idle: shorter tiles write more parts of sums,
-    // longer ones leave CUs without work (the whole gradient, bfloat16: 262,144 x 512 99 us, with half or twice the waves 111 and 108;
-    // 1,000,003 x 203 149, 166 and 172; 8,000,000 x 32, 16,384 waves, 727, 778 and, with a quarter, 970)
+    // about 2,048 waves of wide rows, of 16-bit elements, or 1,024 with several narrow ones: shorter tiles write more parts of sums, longer
+    // ones leave CUs without work (the whole gradient, bfloat16: 262,144 x 512 95 us, with half or twice the waves 110 and 96; 1,000,003 x
+    // 203 149, 167 and 172; 1,000,000 x 64 86, 106 and 87; 8,000,000 x 32 433, with half 544)
+    const int64_t narrow = (1 << 19) / (dim < 32 ? 32 : dim), wide = (1 << 20) / (dim < 128 ? 128 : dim);
     p.run = 16;
-    while (p.run < (1 << 20) && n / p.run * (dim < 64 ? 64 : dim) > (1 << 20)) p.run *= 2;
+    while (p.run < (1 << 20) && n / p.run > (narrow > wide ? narrow : wide)) p.run *= 2;
     p.tiles = (uint32_t)((n + p.run - 1) / p.run);
     const bool small = n <= kSmallSort;
     const auto place = [&](size_t bytes) {
@@ -638,8 +779,15 @@ extern "C" int dnatok_embedding_backward(const void *ids, int32_t id_bytes, int6
         const GradArgs a{tokens, (uint32_t)n, (uint32_t)vocab, p.tiles, p.run, dy, dy_stride, dim, scale};
         float *parts = (float *)((char *)work + p.parts);
         const unsigned blocks = (unsigned)blocks_of(dim, sizeof(T)), zeros = (unsigned)((vocab + kZeroRows * 4 - 1) / (kZeroRows * 4));
-        embed_grad_kernel<T><<<dim3((p.tiles + 3) / 4 + zeros, blocks), 256, 0, s>>>(a, parts, (T *)grad);
-        if (p.tiles > 1) embed_join_kernel<T><<<dim3(p.tiles - 1, blocks), kJoinWaves * 64, 0, s>>>(a, parts, (T *)grad);
+        const int shift = narrow_shift(dim, sizeof(T));
+        if (shift >= 0 && shift <= 4) {
+            const unsigned each = 4 * (64 >> shift);
+            embed_grad_narrow_kernel<T><<<(p.tiles + each - 1) / each + zeros, 256, 0, s>>>(a, shift, parts, (T *)grad);
+        } else {
+            embed_grad_kernel<T><<<dim3((p.tiles + 3) / 4 + zeros, blocks), 256, 0, s>>>(a, parts, (T *)grad);
+        }
+        if (p.tiles > 1)
+            embed_join_kernel<T><<<dim3((p.tiles - 1 + kJoinWaves - 1) / kJoinWaves, blocks), kJoinWaves * 64, 0, s>>>(a, parts, (T *)grad);
     });
     DNATOK_HIP_TRY(hipGetLastError());
     return DNATOK_OK;

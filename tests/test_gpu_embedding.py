@@ -184,3 +184,36 @@ def test_refusals():
     for scale in (float("nan"), float("inf")):
         with pytest.raises(ValueError, match="scale"):
             lm_ops.embedding(ids, weight, scale=scale)
+
+
+def test_narrow_rows_of_many_tokens():
+    """Rows of a few bytes lie next to each other in a wave, two rounds of them where there are very many."""
+    n, vocab = 17_000_003, 50
+    g = torch.Generator(device=DEV).manual_seed(3)
+    ids = torch.randint(-1, vocab + 1, (n,), generator=g, device=DEV, dtype=torch.int32)
+    weight = torch.randn((vocab, 3), generator=g, device=DEV).bfloat16()
+    y = lm_ops.embedding(ids, weight)
+    known = (ids >= 0) & (ids < vocab)
+    for lo in range(0, n, 4_000_000):
+        i, k = ids[lo:lo + 4_000_000].long().clamp(0, vocab - 1), known[lo:lo + 4_000_000]
+        assert torch.equal(y[lo:lo + 4_000_000], torch.where(k[:, None], weight[i], 0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 3, 40, 2000])
+@pytest.mark.parametrize("dim", [1, 4, 9, 16, 33, 64, 100, 128, 129, 200, 256])
+def test_gradients_of_narrow_rows(dim, vocab, dtype):
+    check(20011, vocab, dim, dtype, 0.125, outside=0.05, seed=dim)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 5])
+@pytest.mark.parametrize("run", [255, 256, 257, 271, 272, 273, 300])
+def test_runs_that_end_at_tiles(run, vocab):
+    """Ids of so many tokens each (tiles have sixteen): runs that begin and end at tiles, that one wave joins and that several do."""
+    ids = torch.arange(vocab * run, device=DEV, dtype=torch.int32) // run
+    ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(run)).to(DEV)]
+    g = torch.Generator().manual_seed(vocab)
+    weight = torch.randn((vocab + 1, 24), generator=g).to(DEV).requires_grad_(True)
+    dy = torch.randn((ids.numel(), 24), generator=g).to(DEV)
+    grad, = torch.autograd.grad(lm_ops.embedding(ids, weight), weight, dy)
+    compare_grad(grad, ids, dy, 1.0)
