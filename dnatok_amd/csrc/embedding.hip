@@ -508,8 +508,8 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_narrow_k
 // one id, which one wave then adds up, 16.5, 16.8 and 21.9 (15.0, 24.8 and 27.6); 256 of one id take 31 (27).
 constexpr int kFewTokens = 128;
 template <typename T, typename ID>
-__global__ __launch_bounds__(256) void embed_grad_few_kernel(const ID *ids, uint32_t n, const T *dy, int64_t dy_stride, int64_t vocab, int64_t dim,
-                                                             float scale, T *grad)
+__global__ __launch_bounds__(256) void embed_grad_few_kernel(const ID *ids, uint32_t n, const T *dy, int64_t dy_stride, int64_t vocab,
+                                                             int64_t dim, float scale, T *grad)
 {
     typedef Words<T> W;
     const int lane = threadIdx.x & 63;
@@ -660,8 +660,8 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
         using T = decltype(t);
         with_ids(id_bytes, [&](auto i) {
             using ID = decltype(i);
-            // sixteen tokens to a wave, or eight if that leaves it no more than 32,768 (524,288 rows of 512 bfloat16: 113.1 us with
-            // sixteen, 114.5 with eight, 115.9 with 32; 1,000,003 of 203 floats: 168 with sixteen, 178 with 32, 183 with 64)
+            // two rounds of rows to a wave, or one if that takes no more than 32,768 waves (524,288 rows of 512 bfloat16: 113.1 us with
+            // two, 114.5 with one, 115.9 with four; 1,000,003 of 203 floats: 168 with two, 178 with four, 183 with eight)
             const int shift = narrow_shift(dim, sizeof(T));
             if (shift >= 0) {
                 const int64_t once = kEmbedAhead * (64 >> shift);
