@@ -20,12 +20,21 @@ __device__ __forceinline__ float from_ordered(uint32_t u) { return __uint_as_flo
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// exp(d) for d <= 0 to an ulp or two: what the product with log2(e) is rounded off by is multiplied on.  (-inf is far enough at -200.)
-__device__ __forceinline__ float exp_of(float d)
+// exp(v - top) for v <= top to an ulp or two: what the difference and its product with log2(e) are rounded off by is multiplied on (a
+// difference of 10 is off by up to 8 roundings of a float, and so would the sum be if most of it is such terms; 16-bit numbers have none
+// that matters).  (-inf is far enough at -200.)
+template <typename T> __device__ __forceinline__ float exp_of(float v, float top)
 {
+    float d = v - top, off = 0.0f;
+    if constexpr (sizeof(T) == 4) {
+        const float back = d - v;
+        off = (v - (d - back)) - (top + back);
+        off = d > -200.0f ? off : 0.0f;            // (and not inf - inf)
+    }
     d = fmaxf(d, -200.0f);
-    const float e = 1.44269504f * d, rest = fmaf(1.92596299e-8f, d, fmaf(1.44269504f, d, -e)), v = __builtin_amdgcn_exp2f(e);
-    return fmaf(v, 0.693147181f * rest, v);
+    const float e = 1.44269504f * d, rest = fmaf(1.44269504f, off, fmaf(1.92596299e-8f, d, fmaf(1.44269504f, d, -e))),
+                power = __builtin_amdgcn_exp2f(e);
+    return fmaf(power, 0.693147181f * rest, power);
 }
 
 struct Candidate {
@@ -152,15 +161,15 @@ __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(const T *logits,
         const float nth = width <= 8 && here >= kRowThreads * kCount ? nth_largest(tops, kRowWaves, width) : nth_largest(groups, kGroups, width);
         if (lane == 0) bound_of = nth;
     }
-    float sum = odd ? NAN : 0.0f;
+    // (in 64 bits from the first term on: in 32 a thread that has the largest one would lose all below 2^-24 of it)
+    double all = odd ? NAN : 0.0;
     if (top > -INFINITY) {
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
             if (j * kRowThreads * kCount < here)
 #pragma unroll
-                for (int e = 0; e < kCount; ++e) sum += exp_of((float)v[j][e] - top);
+                for (int e = 0; e < kCount; ++e) all += exp_of<T>((float)v[j][e], top);
     }
-    double all = sum;
 #pragma unroll
     for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
     if (lane == 0) sums[wave] = all;
