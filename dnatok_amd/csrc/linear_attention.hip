@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kSlotThreads) void slots_kernel(WalkArgs w)
         const int head = (int)(at_once % w.heads);
         const int64_t i = at_once / w.heads * kSlotThreads + threadIdx.x;
         if (i >= cells) continue;
-        const float ld = log_decay_of(w, head);
+        const float ld = log_decay_of(w.log_decay, head);
         float state = w.start ? w.start_scale * w.start[(row * w.heads + head) * cells + i] : 0.0f;
         const Left left = left_after(ld, (float)w.cut);
         state = decayed(state, left_after(ld, (float)outer));

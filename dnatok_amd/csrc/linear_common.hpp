@@ -131,22 +131,31 @@ __device__ __forceinline__ Piece piece_of(const WalkArgs &w, int64_t item)
 
 // ---- the state -------------------------------------------------------------------------------------
 
-// What is left of a state after n steps: by the factor, or by 1 - it.  (A factor next to 1, rounded once and multiplied thousands of times,
-// would be a wrong rate.)
+// What is left of a state after n steps (one at least): by the factor, or by 1 - it.  (A factor next to 1, rounded once and multiplied
+// thousands of times, would be a wrong rate.)  keeps: not if a step leaves nothing at all, whatever the state is.
+constexpr float kNothingLeft = -1e30f;
 struct Left {
     float factor, lost;
+    bool keeps;
 };
 __device__ __forceinline__ Left left_after(float log_decay, float n)
 {
     // factor s - lost s: one of them is 0, and the other the more exact one
     const float lost = -expm1f(n * log_decay);
-    return lost < 0.5f ? Left{1.0f, lost} : Left{expf(n * log_decay), 0.0f};
+    const bool keeps = !(log_decay <= kNothingLeft);
+    return lost < 0.5f ? Left{1.0f, lost, keeps} : Left{expf(n * log_decay), 0.0f, keeps};
 }
-__device__ __forceinline__ float decayed(float s, const Left &l) { return fmaf(-l.lost, s, l.factor * s); }
-
-__device__ __forceinline__ float log_decay_of(const WalkArgs &w, int head)
+// (An infinity stays one as long as anything is left of a state, also where the factor has become 0, and a NaN stays one; a decay that is
+// NaN makes one.)
+__device__ __forceinline__ float decayed(float s, const Left &l)
 {
-    return __builtin_elementwise_maximum(w.log_decay[head], -1e30f);    // (so that -inf times no step at all is 0; keeps a NaN)
+    const float v = fmaf(-l.lost, s, l.factor * s);
+    return __builtin_fabsf(s) < INFINITY ? v : l.keeps ? s + 0.0f * l.factor : 0.0f;
+}
+
+__device__ __forceinline__ float log_decay_of(const float *log_decay, int head)
+{
+    return __builtin_elementwise_maximum(log_decay[head], kNothingLeft);        // (so that -inf times no step at all is 0; keeps a NaN)
 }
 
 }  // namespace dnatok

@@ -237,7 +237,7 @@ __device__ __forceinline__ void put(OUT *rows, int pitch, int dim, int n, int co
 // itself the compiler asks for one operand, waits, and uses it.)
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// ---- the walk ----------------------------------------------------------------------------------------
+// ---- chunks in LDS -----------------------------------------------------------------------------------
 
 // Whether LDS holds two chunks of the operands, so that the next one is there when a chunk is done: where a workgroup has the CU to
 // itself.  (256 rows of 1,024 tokens and 4 heads of 128 x 128: 336 us, with one chunk 346; smaller heads have a second workgroup on
@@ -383,6 +383,132 @@ __device__ __forceinline__ const char *base_of(const Operand &o, int head, int s
     return (const char *)o.p + head / o.shared * o.head * size;
 }
 
+// ---- infinities and NaN ------------------------------------------------------------------------------
+
+// In the products an infinity becomes a NaN at once: its parts are inf and inf - inf, what masks it or has decayed to nothing is 0 times
+// it, and terms of the recurrence that are never added there meet.  Such outputs and cells of states are not finite, whatever became
+// of them, and no others are touched; so a wave that finds any goes through its piece once more, step by step as the recurrence
+// is written, and replaces those.  (An infinite value in each row's first token: 64 rows of 8,192 tokens, 8 heads of 64 x 64, 12.0 ms
+instead of 0.53; one row of 262,147 in 63 pieces, 4 heads of 128 x 128, 8.7 instead of 0.55.)
+__device__ __forceinline__ bool is_finite(float v) { return __builtin_fabsf(v) < INFINITY; }
+template <int N> __device__ __forceinline__ bool any_not_finite(const f32x4 (&v)[N])
+{
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = __builtin_elementwise_maximum(most, __builtin_fabsf(v[i][r]));      // (keeps a NaN)
+    return __builtin_amdgcn_ballot_w64(!is_finite(most)) != 0;
+}
+
+// A number that the compiler knows nothing of: what it would find out (which rows are there), it finds out again, and does not keep it through
+// the walk in registers that are needed there.
+__device__ __forceinline__ int forgotten(int v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
+// Another lane's four numbers.
+template <typename V> __device__ __forceinline__ V from_lane(V v, int lane)
+{
+    constexpr int kWords = sizeof(V) / 4;
+    typedef int words __attribute__((ext_vector_type(kWords)));
+    words w = __builtin_bit_cast(words, v);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = __shfl(w[i], lane);
+    return __builtin_bit_cast(V, w);
+}
+
+// The steps of a piece, one at a time: out(step, values) for sixteen steps at a time from the step `quiet` on (OUT), of which a lane has step
+// lane % 16 and columns 4 (lane / 16) .. + 3 of the wave's sixteen, and what becomes of the state, of which it has column lane % 16
+// and rows 4 (lane / 16) .. + 3 of each sixteen.  Operands are fetched for sixteen steps at once, a lane having one step's, and handed
+// round.  Where all of a wave's state is NaN (training that went astray), so is all that follows.
+template <typename T, int KD, bool TAIL, bool OUT, typename Fn>
+__device__ __forceinline__ void by_steps(const WalkArgs &w, const Piece &p, int head, float log_decay, int column, int lane, f32x4 (&state)[KD / 16],
+                                         int64_t quiet, Fn out)
+{
+    typedef typename Four<T>::type four;
+    constexpr int KT = KD / 16;
+    const Left left = left_after(log_decay, 1.0f);
+    const int g = lane >> 4, l16 = lane & 15, db = w.b.dim, dc = w.c.dim;
+    const int64_t length = p.hi - p.lo;
+    const T *pa = OUT ? (const T *)base_of(w.a, head, sizeof(T)) : nullptr, *pb = (const T *)base_of(w.b, head, sizeof(T)),
+            *pc = (const T *)base_of(w.c, head, sizeof(T));
+    const auto four_of = [](const T *row, int m, int dim) {
+        four v{};
+        if (!TAIL) {
+            if (m < dim) __builtin_memcpy(&v, row + m, sizeof(v));
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (m + r < dim) v[r] = row[m + r];
+        }
+        return v;
+    };
+    bool lost = false;
+    for (int64_t first = 0; first < length; first += 16) {
+        const int here = length - first < 16 ? (int)(length - first) : 16;
+        const bool puts = OUT && first >= quiet;
+        const int64_t mine = first + l16, t = w.reverse ? p.hi - 1 - mine : p.lo + mine;
+        f32x4 value = {NAN, NAN, NAN, NAN};
+        if (!lost) {
+            four a[KT]{}, b[KT]{}, c{};
+            if (l16 < here) {
+                c = four_of(pc + t * w.c.token + column + 4 * g, 0, dc - column - 4 * g);
+                const T *row = pb + t * w.b.token + 4 * g;
+                int rows = forgotten(db - 4 * g);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) b[kt] = four_of(row, 16 * kt, rows);
+                if (puts) {
+                    row = pa + t * w.a.token + 4 * g;
+                    rows = forgotten(db - 4 * g);
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) a[kt] = four_of(row, 16 * kt, rows);
+                }
+            }
+#pragma unroll 1
+            for (int j = 0; j < here; ++j) {
+                const int rows = forgotten(db - 4 * g);
+                const four columns = from_lane(c, 16 * (l16 >> 2) + j);
+                float mine_of = (float)columns[0], sum = 0.0f;
+#pragma unroll
+                for (int r = 1; r < 4; ++r) mine_of = (l16 & 3) == r ? (float)columns[r] : mine_of;
+                bool all = left.keeps;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const four bj = from_lane(b[kt], 16 * g + j), aj = puts ? from_lane(a[kt], 16 * g + j) : four{};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool is = 16 * kt + r < rows;            // (a row that is none times an infinity would be NaN)
+                        float s = state[kt][r];
+                        if (!w.decayed) s = decayed(s, left);
+                        if (is) s = fmaf((float)bj[r], mine_of, s);
+                        if (is) sum = fmaf((float)aj[r], s, sum);
+                        if (w.decayed) s = decayed(s, left);
+                        state[kt][r] = s;
+                        all &= !is || column + l16 >= dc || s != s;
+                    }
+                }
+                lost = __builtin_amdgcn_ballot_w64(!all) == 0;
+                if (puts) {
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = w.scale * __shfl(sum, 4 * g + r);
+                        value[r] = l16 == j ? v : value[r];
+                    }
+                }
+                if (lost) break;                   // (the steps behind this one have their NaN)
+            }
+        }
+        if (puts && l16 < here) out(t, value);
+    }
+}
+
+// ---- the walks ---------------------------------------------------------------------------------------
+
 // One workgroup to a piece of a row and a head.  A wave has sixteen of the state's columns, which no other wave needs; scores are
 // shared.  Of 32-bit operands no more than one workgroup of four waves fits beside tiles of 128 x 64.
 //
@@ -422,7 +548,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     }
     const Piece p = piece_of(w, item);
     if (p.none) return;
-    const float ld = log_decay_of(w, head);
+    const float ld = log_decay_of(w.log_decay, head);
     const int late = w.decayed ? 1 : 0;
     const bool reverse = w.reverse;
     const int64_t length = p.hi - p.lo;
@@ -457,14 +583,16 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
 
     // what is in front of the piece
     f32x4 state[KT];
+    const auto begin = [&](int lane) {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) state[kt] = f32x4{0, 0, 0, 0};
-    if (starts ? w.start != nullptr : true) {
+        for (int kt = 0; kt < KT; ++kt) state[kt] = f32x4{0, 0, 0, 0};
+        if (starts && !w.start) return;
         const int64_t slot = (reverse ? p.hi : p.lo) / w.cut;
         const float *from = starts ? w.start + (p.row * w.heads + head) * cells : w.slots + ((slot - 1) * w.heads + head) * cells;
         const float scale = starts ? w.start_scale : 1.0f;
         each_cell<KD>(w, column, lane, w.transposed, [&](int kt, int r, int at) { state[kt][r] = scale * from[at]; });
-    }
+    };
+    begin(lane);
 
     for (int i = threadIdx.x; i <= kChunk; i += kThreads) lds.power[i] = expf((float)i * ld);
     // scores of sixteen steps with those before them, and the state's share of a step
@@ -488,6 +616,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     fetch(kChunk);
     __syncthreads();
     int turn = 0;
+    int64_t odd_from = length;                     // the first chunk of which not all results are finite
     for (int64_t done = 0; done < length; done += kChunk, turn ^= kTwo) {
         const int n = count_of(done);
         const Chunk<T, KD, CD> &chunk = lds.chunk[turn];
@@ -679,6 +808,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
 #pragma unroll
                 for (int ts = 0; ts < TS; ++ts) c8[ts] = chunk.c.column(D * ts, column, lane);
             }
+            if (any_not_finite(out) && odd_from > done) odd_from = done;
             const int64_t cell = (first_of(done, n) * w.heads + head) * dc;
             int row[4];
 #pragma unroll
@@ -697,16 +827,37 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
             __syncthreads();
         }
     }
-    if (ends && w.end) {
-        float *to = w.end + (p.row * w.heads + head) * cells;
-        each_cell<KD>(w, column, lane, false, [&](int kt, int r, int at) { to[at] = w.end_scale * state[kt][r]; });
+    float *end = ends && w.end ? w.end + (p.row * w.heads + head) * cells : nullptr;
+    if (end) each_cell<KD>(w, column, lane, false, [&](int kt, int r, int at) { end[at] = w.end_scale * state[kt][r]; });
+    if (__builtin_expect(column < dc && length > 0 && (odd_from < length || any_not_finite(state)), false)) {
+        const int lane2 = forgotten(lane), g2 = lane2 >> 4;
+        begin(lane2);
+        // (a lane looks at what it wrote itself)
+        by_steps<T, KD, TAIL, true>(w, p, head, ld, column, lane2, state, odd_from, [&](int64_t t, const f32x4 &v) {
+            const int64_t at = (t * w.heads + head) * dc + column + 4 * g2;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (column + 4 * g2 + r >= dc) break;
+                if (w.out32) {
+                    float *place = (float *)w.out + at + r;
+                    if (!is_finite(*place)) *place = v[r];
+                } else {
+                    T *place = (T *)w.out + at + r;
+                    if (!is_finite((float)*place)) *place = (T)v[r];
+                }
+            }
+        });
+        if (end)
+            each_cell<KD>(w, column, lane2, false, [&](int kt, int r, int at) {
+                if (!is_finite(end[at])) end[at] = w.end_scale * state[kt][r];
+            });
     }
 }
 
 // What each piece that does not end its row adds to the state: into the slot of the cut behind it.  One row of 262,147 tokens, 4 heads of
 // 128 x 128 of float16: 140 us for 0.54 GB, 30 more for the slots' states, then the walk.
 template <typename T, int KD, int CD, bool TAIL>
-__global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 64 ? 1 : 2) void piece_kernel(WalkArgs w)
+__global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 64 ? 1 : sizeof(T) == 4 && KD == 64 ? 3 : 2) void piece_kernel(WalkArgs w)
 {
     typedef typename Frag<T>::type frag;
     constexpr int KT = KD / 16, kThreads = threads_of(CD), D = Frag<T>::kDepth, TS = kChunk / D;
@@ -715,7 +866,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     const int head = blockIdx.x % w.heads;
     const Piece p = piece_of(w, blockIdx.x / w.heads);
     if (p.none || (w.reverse ? p.front : p.back)) return;
-    const float ld = log_decay_of(w, head);
+    const float ld = log_decay_of(w.log_decay, head);
     const int late = w.decayed ? 1 : 0;
     const bool reverse = w.reverse;
     const int64_t length = p.hi - p.lo;
@@ -756,6 +907,15 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     const int64_t slot = (reverse ? p.lo : p.hi) / w.cut;
     float *to = w.slots + ((slot - 1) * w.heads + head) * (int64_t)db * dc;
     each_cell<KD>(w, column, lane, false, [&](int kt, int r, int at) { to[at] = state[kt][r]; });
+    if (__builtin_expect(column < dc && any_not_finite(state), false)) {
+        const int lane2 = forgotten(lane);
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) state[kt] = f32x4{0, 0, 0, 0};
+        by_steps<T, KD, TAIL, false>(w, p, head, ld, column, lane2, state, 0, [](int64_t, const f32x4 &) {});
+        each_cell<KD>(w, column, lane2, false, [&](int kt, int r, int at) {
+            if (!is_finite(to[at])) to[at] = state[kt][r];
+        });
+    }
 }
 
 // ---- launches -----------------------------------------------------------------------------------------

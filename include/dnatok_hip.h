@@ -494,7 +494,8 @@ int dnatok_logits_process(const void *logits, int64_t logits_stride, int32_t dty
  * elements next to each other, strides in elements between tokens and between heads.  log_decay float[heads] is at most 0
  * (-inf: nothing is kept).  Rows, offsets and reverse are those of dnatok_gated_scan; so is what happens to tokens in no row.  h0
  * float[n_rows, heads, dim_k, dim_v] (NULL: zeros) is T in front of a row's first step, last (NULL allowed) receives T behind its last
- * one.  A row's y depends on no token behind it, also where that holds infinities or NaN.  states (NULL allowed) receives what the
+ * one.  A row's y depends on no token behind it, also where that holds infinities or NaN, and those go on as the recurrence has them: an
+infinite T stays so as long as log_decay is above -1e30 (below it, and at -inf, nothing is left of any T).  states (NULL allowed) receives what the
  * backward pass needs, dnatok_linear_attention_states_bytes(); work is the call's own space,
  * dnatok_linear_attention_work_bytes(), 16-byte aligned. */
 typedef struct dnatok_linear_shape {
