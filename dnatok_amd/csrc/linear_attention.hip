@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void linear_step_kernel(Operand q, Operand k, 
         qk[0][i] = to_float(qp[i]);
         qk[1][i] = to_float(kp[i]);
     }
-    const float g = expf(log_decay[head]);
+    const Left left = left_after(log_decay_of(log_decay, head), 1.0f);
     const int per = 256 / cols, col = threadIdx.x % cols, first = threadIdx.x / cols;      // (threads behind the last whole row have none)
     const int64_t at = (row * heads + head) * dk * dv;
     vec sum{}, value{};
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(256) void linear_step_kernel(Operand q, Operand k, 
             if (state) s = *reinterpret_cast<const vec *>(state + at + m * dv + col * VEC);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                s[e] = (state ? g * s[e] : 0.0f) + qk[1][m] * value[e];
-                sum[e] += qk[0][m] * s[e];
+                s[e] = fmaf(qk[1][m], value[e], decayed(s[e], left));
+                sum[e] = fmaf(qk[0][m], s[e], sum[e]);
             }
             *reinterpret_cast<vec *>(new_state + at + m * dv + col * VEC) = s;
         }

@@ -1,0 +1,63 @@
+"""Single tokens of linear attention: many of them in a row, and what is infinite."""
+import math
+
+import pytest
+import torch
+
+from dnatok_amd import lm_ops
+from tests.support import attention_reference as ref
+from tests.test_gpu_attention_infinities import DECAYS, KINDS, compare, plant
+from tests.test_gpu_linear_attention import TYPES, inputs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def test_many_steps_keep_the_rate():
+    """20,000 steps that only decay.  A step rounds a cell once, by up to u = 2^-24 of it to either side: after n steps that is some
+    sqrt(n) u (8.4e-6), and six times that is asked for of the mean over 4,096 cells, which is nearer.  exp(log_decay) rounded to 32 bits
+    is off by 2.4e-8 to 3e-8 for these rates, which over n steps is 4.8e-4 and more."""
+    n, rates = 20000, []
+    for i in range(1000):
+        ld = torch.tensor(-1e-5 * 1.01 ** i, dtype=torch.float32)
+        off = (torch.exp(ld.double()).float().double() - torch.exp(ld.double())).abs().item()
+        if off > 2.4e-8 and -ld.item() * n < 8:
+            rates.append(ld.item())
+    heads = min(len(rates), 8)
+    assert heads == 8
+    ld = torch.tensor(rates[:heads], device=DEV)
+    g = torch.Generator().manual_seed(0)
+    start = (1.0 + torch.rand((1, heads, 64, 64), generator=g)).to(DEV)
+    state = start.clone()
+    zero = torch.zeros((1, heads, 64), device=DEV)
+    for _ in range(n):
+        lm_ops.linear_attention_step(zero, zero, zero, ld, state, out_state=state)
+    rate = (state.double() / start.double()).log().mean((0, 2, 3))
+    assert (rate - n * ld.double()).abs().max().item() <= 6 * math.sqrt(n) * ref.U
+
+
+@pytest.mark.parametrize("kind", [k for k in KINDS if not k.startswith("d")])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dims", [(24, 40), (13, 7)])
+def test_infinities(dims, dtype, kind):
+    print(f"step {dims} {dtype} {kind}", flush=True)
+    data = plant(inputs([1] * 9, 6, 3, *dims, dtype, 1, decay=DECAYS), kind, 3)
+    q, k, v, ld, off, h0, _, _ = data
+    y, new = lm_ops.linear_attention_step(q, k, v, ld, h0)
+    odd = compare({"y": y, "last": new}, data, dtype, 1)
+    assert odd
+    first, _ = lm_ops.linear_attention_step(q, k, v, ld)                 # no state: the decays do not matter
+    compare({"y": first}, (q, k, v, ld, off, None, None, None), dtype, 1)
+
+
+@pytest.mark.parametrize("kind", ["v", "v of both signs", "k", "h0"])
+def test_steps_are_the_rows(kind):
+    """The prompt's way and the steps' give the same infinities."""
+    q, k, v, ld, off, h0, dy, dlast = plant(inputs([40], 6, 3, 16, 24, torch.bfloat16, 2, decay=DECAYS), kind, 20)
+    y, last = lm_ops.linear_attention(q, k, v, ld, torch.tensor(off, device=DEV), h0=h0)
+    state = h0.clone()
+    for t in range(40):
+        out, _ = lm_ops.linear_attention_step(q[t:t + 1], k[t:t + 1], v[t:t + 1], ld, state, out_state=state)
+        assert torch.equal(torch.isnan(out), torch.isnan(y[t:t + 1])), t
+        assert torch.equal(out == math.inf, y[t:t + 1] == math.inf) and torch.equal(out == -math.inf, y[t:t + 1] == -math.inf), t
+    assert torch.equal(torch.isnan(state), torch.isnan(last)) and torch.equal(torch.isinf(state), torch.isinf(last))
