@@ -119,9 +119,12 @@ using namespace dnatok;
 
 #define LINEAR_REQUIRE(cond, text) DNATOK_REQUIRE(cond, DNATOK_E_INVALID, "%s: " text, who)
 
-static int check_shape(const char *who, const dnatok_linear_shape *s)
+// Checks a shape of `tokens` tokens, and leaves it in `call` as the kernels take it: where there is one token at most, the distance to the
+// next is that of no address, whatever it says (an axis of size one may have any stride).
+static int check_shape(const char *who, const dnatok_linear_shape *given, int64_t dnatok_linear_shape::*tokens, dnatok_linear_shape *call)
 {
-    LINEAR_REQUIRE(s, "null shape");
+    LINEAR_REQUIRE(given, "null shape");
+    const dnatok_linear_shape *s = given;
     LINEAR_REQUIRE(s->dtype == DNATOK_F32 || s->dtype == DNATOK_BF16 || s->dtype == DNATOK_F16, "unknown element type");
     LINEAR_REQUIRE(s->n_rows >= 0 && s->total >= 0 && s->heads > 0 && s->kv_heads > 0 && s->dim_k > 0 && s->dim_v > 0, "bad size");
     LINEAR_REQUIRE(s->heads % s->kv_heads == 0, "the heads must be a multiple of those of the keys and values");
@@ -130,6 +133,9 @@ static int check_shape(const char *who, const dnatok_linear_shape *s)
                    "the scale must be 2^-40 to 2^40 in size");
     LINEAR_REQUIRE(s->q_token >= 0 && s->q_head >= 0 && s->k_token >= 0 && s->k_head >= 0 && s->v_token >= 0 && s->v_head >= 0 &&
                        s->dy_token >= 0 && s->dy_head >= 0, "negative stride");
+    *call = *given;
+    if (given->*tokens <= 1) call->q_token = call->k_token = call->v_token = call->dy_token = 0;
+    s = call;
     constexpr int64_t kFar = (1ll << 31) / 64 / 4;
     DNATOK_REQUIRE(s->q_token < kFar && s->k_token < kFar && s->v_token < kFar && s->dy_token < kFar && (int64_t)s->heads * 128 < kFar,
                    DNATOK_E_TOO_LARGE, "%s: tokens must lie less than 2^23 elements apart", who);
@@ -219,8 +225,9 @@ extern "C" int dnatok_linear_attention(const dnatok_linear_shape *shape, const v
                                        float *states, void *work, size_t work_bytes, void *stream)
 {
     static const char *who = "dnatok_linear_attention";
-    if (int rc = check_shape(who, shape)) return rc;
-    const dnatok_linear_shape &s = *shape;
+    dnatok_linear_shape s;
+    if (int rc = check_shape(who, shape, &dnatok_linear_shape::total, &s)) return rc;
+    shape = &s;
     if (int rc = check_call(who, s, offsets)) return rc;
     LINEAR_REQUIRE(log_decay && (s.total == 0 || (q && k && v && y)), "null buffer");
     LINEAR_REQUIRE(states || (work_bytes >= dnatok_linear_attention_work_bytes(shape, 0) && (work || !work_bytes)), "work space too small");
@@ -245,8 +252,9 @@ extern "C" int dnatok_linear_attention_backward(const dnatok_linear_shape *shape
                                                 void *work, size_t work_bytes, void *stream)
 {
     static const char *who = "dnatok_linear_attention_backward";
-    if (int rc = check_shape(who, shape)) return rc;
-    const dnatok_linear_shape &s = *shape;
+    dnatok_linear_shape s;
+    if (int rc = check_shape(who, shape, &dnatok_linear_shape::total, &s)) return rc;
+    shape = &s;
     if (int rc = check_call(who, s, offsets)) return rc;
     LINEAR_REQUIRE(log_decay && (s.total == 0 || (q && k && v && dy && dq && dk && dv)), "null buffer");
     LINEAR_REQUIRE(states || !dnatok_linear_attention_states_bytes(shape), "the forward pass' states are missing");
@@ -287,8 +295,9 @@ extern "C" int dnatok_linear_attention_step(const dnatok_linear_shape *shape, co
                                             const float *log_decay, const float *state, void *y, float *new_state, void *stream)
 {
     static const char *who = "dnatok_linear_attention_step";
-    if (int rc = check_shape(who, shape)) return rc;
-    const dnatok_linear_shape &s = *shape;
+    dnatok_linear_shape s;
+    if (int rc = check_shape(who, shape, &dnatok_linear_shape::n_rows, &s)) return rc;
+    shape = &s;
     if (s.n_rows == 0) return DNATOK_OK;
     LINEAR_REQUIRE(q && k && v && log_decay && y && new_state, "null buffer");
     DNATOK_REQUIRE(s.n_rows <= 65535, DNATOK_E_TOO_LARGE, "%s: at most 65535 rows", who);

@@ -502,7 +502,7 @@ typedef struct dnatok_linear_shape {
     int32_t dtype, reverse;
     int64_t n_rows, total;
     int32_t heads, kv_heads, dim_k, dim_v;
-    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;         /* tokens less than 2^23 apart (any number for a single one) */
     int64_t dy_token, dy_head;         /* backward pass only */
     float scale;                       /* 2^-40 to 2^40 in size */
     int32_t with_offsets;              /* whether the call will have offsets (for the sizes of states and work) */
