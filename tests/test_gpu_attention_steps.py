@@ -66,13 +66,13 @@ def test_steps_are_the_rows(kind):
 def test_a_token_out_of_a_long_prompt():
     """One token of one row, whose stride to the next is that of no address: in a step, in a row, and in its backward pass."""
     g = torch.Generator().manual_seed(3)
-    part = torch.randn((1, 1, 3 * 4 * 16), generator=g).to(DEV)
-    long = torch.empty((1, 2 ** 17, 3 * 4 * 16), device=DEV)
-    long[:, -1:] = part
+    part = torch.randn((1, 12, 16), generator=g).to(DEV)
+    long = torch.empty((1, 2 ** 17, 12, 16), device=DEV)
+    long[:, -1] = part
     ld = torch.tensor([-0.1, -0.2, -0.3, 0.0], device=DEV)
-    q, k, v = (t.view(1, 4, 16) for t in long[:, -1].split(64, 1))
+    q, k, v = long[:, -1].split(4, 1)
     assert q.stride(0) > 2 ** 23
-    want = lm_ops.linear_attention_step(*(t.view(1, 4, 16) for t in part[:, -1].split(64, 1)), ld)
+    want = lm_ops.linear_attention_step(*part.split(4, 1), ld)
     got = lm_ops.linear_attention_step(q, k, v, ld)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     off, leaves = torch.tensor([0, 1], device=DEV), [t.detach().requires_grad_(True) for t in (q, k, v)]
