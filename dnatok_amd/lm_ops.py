@@ -236,6 +236,9 @@ def _forward_only(name: str, *tensors) -> None:
 
 # ---- linear attention -------------------------------------------------------------------------
 
+_FAR_TOKENS = 1 << 23                   # elements between tokens that are too many (dnatok_linear_shape)
+
+
 class _LinearPlan:
     """What calls of the same sizes have in common: their description for the C entries, and the sizes of their buffers."""
 
@@ -391,11 +394,14 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                           out_state: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """One step of :func:`linear_attention` for one token of each row: ``q`` [B, H, Dk], ``k`` [B, G, Dk], ``v`` [B, G, Dv],
     ``state`` float32 [B, H, Dk, Dv] (zero if not given).  Returns ``(y, new_state)``; ``out_state`` receives the new state
-    and may be ``state`` itself.  Without gradients."""
+    and may be ``state`` itself.  Tokens that lie 2^23 elements apart or more (the last ones of long prompts) are copied.  Without
+    gradients."""
     _require_floats(q, "q")
     if q.dim() != 3:
         raise ValueError("q must be [B, H, Dk]")
-    device = q.device
+    device, given = q.device, (q, k, v)
+    if q.shape[0] > 1:                             # (the C entries take no tokens that lie farther apart)
+        q, k, v = (t.contiguous() if t.dim() == 3 and t.stride(0) >= _FAR_TOKENS else t for t in given)
     plan = _plan_of(q, k, v, q.shape[0], scale, 0, 0)
     shape = (*q.shape, v.shape[2])
     _require_decay("linear_attention_step", log_decay, shape[1], device)
@@ -406,7 +412,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     if out_state is None:
         out_state = torch.empty(shape, dtype=torch.float32, device=device)
     else:
-        _require_apart("linear_attention_step", out_state, q, k, v, log_decay, state, same=state)
+        _require_apart("linear_attention_step", out_state, *given, log_decay, state, same=state)
     _run("dnatok_linear_attention_step", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
          _ptr(state), y.data_ptr(), out_state.data_ptr())
     return y, out_state

@@ -80,3 +80,21 @@ def test_a_token_out_of_a_long_prompt():
     data = (q, k, v, ld, off.tolist(), None, torch.ones((1, 4, 16)), None)
     got = {"y": y, "last": last, **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(y.sum(), leaves)))}
     assert compare(got, data, torch.float32, 1) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tokens_out_of_long_prompts(dtype):
+    """The last tokens of dense prompts, 2^23 elements and more apart."""
+    q, k, v, ld, off, h0, _, _ = inputs([1] * 3, 4, 2, 16, 24, dtype, 4)
+    far = []
+    for t, apart in ((q, 2 ** 23), (k, 2 ** 23 + 7), (v, 2 ** 24)):
+        wide = torch.empty(2 * apart + t.shape[1] * t.shape[2], dtype=dtype, device=DEV)
+        far.append(torch.as_strided(wide, t.shape, (apart, t.shape[2], 1)).copy_(t))
+    want = lm_ops.linear_attention_step(q, k, v, ld, h0)
+    for mix in (far, [far[0], k, v], [q, k, far[2]]):
+        got = lm_ops.linear_attention_step(*mix, ld, h0)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(ValueError, match="overlaps"):                    # where the tokens are, not where they are copied to
+        wide = torch.zeros((2, 2 ** 23), device=DEV)
+        part = wide[:, :4 * 16].view(2, 4, 16)
+        lm_ops.linear_attention_step(part, part, part, ld, out_state=wide.view(-1)[:2 * 4 * 16 * 16].view(2, 4, 16, 16))
