@@ -237,6 +237,7 @@ def _forward_only(name: str, *tensors) -> None:
 # ---- linear attention -------------------------------------------------------------------------
 
 _FAR_TOKENS = 1 << 23                   # elements between tokens that are too many (dnatok_linear_shape)
+_STEP_ROWS = 65535                      # rows that one call of the step's entry takes
 
 
 class _LinearPlan:
@@ -399,10 +400,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     _require_floats(q, "q")
     if q.dim() != 3:
         raise ValueError("q must be [B, H, Dk]")
-    device, given = q.device, (q, k, v)
-    if q.shape[0] > 1:                             # (the C entries take no tokens that lie farther apart)
+    device, given, rows = q.device, (q, k, v), q.shape[0]
+    if rows > 1:                             # (the C entries take no tokens that lie farther apart)
         q, k, v = (t.contiguous() if t.dim() == 3 and t.stride(0) >= _FAR_TOKENS else t for t in given)
-    plan = _plan_of(q, k, v, q.shape[0], scale, 0, 0)
+    plan = _plan_of(q, k, v, rows, scale, 0, 0)
     shape = (*q.shape, v.shape[2])
     _require_decay("linear_attention_step", log_decay, shape[1], device)
     _require(state, "state", shape, torch.float32, device)
@@ -413,8 +414,15 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         out_state = torch.empty(shape, dtype=torch.float32, device=device)
     else:
         _require_apart("linear_attention_step", out_state, *given, log_decay, state, same=state)
-    _run("dnatok_linear_attention_step", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-         _ptr(state), y.data_ptr(), out_state.data_ptr())
+    if rows <= _STEP_ROWS:
+        _run("dnatok_linear_attention_step", device, plan.shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+             _ptr(state), y.data_ptr(), out_state.data_ptr())
+        return y, out_state
+    for first in range(0, rows, _STEP_ROWS):
+        here = slice(first, first + _STEP_ROWS)
+        plan = _plan_of(q[here], k[here], v[here], min(_STEP_ROWS, rows - first), scale, 0, 0)
+        _run("dnatok_linear_attention_step", device, plan.shape, q[here].data_ptr(), k[here].data_ptr(), v[here].data_ptr(),
+             log_decay.data_ptr(), None if state is None else state[here].data_ptr(), y[here].data_ptr(), out_state[here].data_ptr())
     return y, out_state
 
 

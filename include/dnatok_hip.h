@@ -522,7 +522,7 @@ int dnatok_linear_attention_backward(const dnatok_linear_shape *shape_h, const v
                                      const float *dlast, const float *states, void *dq, void *dk, void *dv, float *dh0, void *work,
                                      size_t work_bytes, void *stream);
 
-/* One step for one token of each row: q, k, v and y as above with n_rows in total's place; state (NULL: zeros) and new_state
+/* One step for one token of each row, at most 65,535: q, k, v and y as above with n_rows in total's place; state (NULL: zeros) and new_state
  * float[n_rows, heads, dim_k, dim_v], which may be the same buffer. */
 int dnatok_linear_attention_step(const dnatok_linear_shape *shape_h, const void *q, const void *k, const void *v,
                                  const float *log_decay, const float *state, void *y, float *new_state, void *stream);

@@ -98,3 +98,26 @@ def test_tokens_out_of_long_prompts(dtype):
         wide = torch.zeros((2, 2 ** 23), device=DEV)
         part = wide[:, :4 * 16].view(2, 4, 16)
         lm_ops.linear_attention_step(part, part, part, ld, out_state=wide.view(-1)[:2 * 4 * 16 * 16].view(2, 4, 16, 16))
+
+
+@pytest.mark.parametrize("rows", [65535, 65536, 140000])
+def test_many_rows(rows):
+    """As many rows as a search over many beams has: y = scale q (g h0 + k v^T) of each."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    q, k = (torch.randn((rows, 2, 8), generator=g, device=DEV) for _ in range(2))
+    v = torch.randn((rows, 1, 2, 4), generator=g, device=DEV)[:, 0, :, :]
+    h0 = torch.randn((rows, 2, 8, 4), generator=g, device=DEV)
+    ld = torch.tensor([-0.25, -2.0], device=DEV)
+    print("step of", rows, "rows", flush=True)
+    y, new = lm_ops.linear_attention_step(q, k, v, ld, h0)
+    kv = k.double()[..., None] * v.double()[:, :, None]
+    old = torch.exp(ld.double())[:, None, None] * h0.double()
+    # a cell: two products, a sum, and the decay's own roundings; y: eight of those and eight sums
+    assert ((new.double() - old - kv).abs() <= 6 * ref.U * (old.abs() + kv.abs())).all()
+    size = 8 ** -0.5 * (q.double().abs()[..., None] * (old.abs() + kv.abs())).sum(2)
+    assert ((y.double() - 8 ** -0.5 * (q.double()[..., None] * (old + kv)).sum(2)).abs() <= 20 * ref.U * size).all()
+    again, _ = lm_ops.linear_attention_step(q, k, v, ld)
+    assert ((again.double() - 8 ** -0.5 * (q.double()[..., None] * kv).sum(2)).abs() <= 20 * ref.U * size).all()
+    same = h0.clone()
+    y2, out = lm_ops.linear_attention_step(q, k, v, ld, same, out_state=same)
+    assert out is same and torch.equal(out, new) and torch.equal(y2, y)
