@@ -388,8 +388,8 @@ __device__ __forceinline__ const char *base_of(const Operand &o, int head, int s
 // In the products an infinity becomes a NaN at once: its parts are inf and inf - inf, what masks it or has decayed to nothing is 0 times
 // it, and terms of the recurrence that are never added there meet.  Such outputs and cells of states are not finite, whatever became
 // of them, and no others are touched; so a wave that finds any goes through its piece once more, step by step as the recurrence
-// is written, and replaces those.  (An infinite value in each row's first token: 64 rows of 8,192 tokens, 8 heads of 64 x 64, 12.0 ms
-instead of 0.53; one row of 262,147 in 63 pieces, 4 heads of 128 x 128, 8.7 instead of 0.55.)
+// is written, and replaces those.  (An infinite value in each row's first token: 64 rows of 8,192 tokens, 8 heads of 64 x 64,
+// 12.0 ms instead of 0.53; one row of 262,147 in 63 pieces, 4 heads of 128 x 128, 8.7 instead of 0.55.)
 __device__ __forceinline__ bool is_finite(float v) { return __builtin_fabsf(v) < INFINITY; }
 template <int N> __device__ __forceinline__ bool any_not_finite(const f32x4 (&v)[N])
 {
