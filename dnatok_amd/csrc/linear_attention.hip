@@ -149,9 +149,9 @@ static int check_call(const char *who, const dnatok_linear_shape &s, const int64
     LINEAR_REQUIRE(!offsets == !s.with_offsets, "the shape must say whether there are offsets");
     LINEAR_REQUIRE(s.n_rows > 0 || s.total == 0, "tokens without rows");
     LINEAR_REQUIRE(offsets || s.n_rows == 0 || s.total % s.n_rows == 0, "rows of one length must fill the axis");
-    // (a grid ends at 2^32 threads, and a piece has up to 512)
-    DNATOK_REQUIRE((s.n_rows + (s.total >> 9) + kOutside) * s.heads < (1ll << 23), DNATOK_E_TOO_LARGE,
-                   "%s: less than 2^23 rows and pieces of rows times heads", who);
+    // (the cuts are a grid's first dimension, which ends at 2^32 threads; rows and pieces go over several launches)
+    DNATOK_REQUIRE(s.n_rows + (s.total >> 9) + kOutside < (1ll << 23), DNATOK_E_TOO_LARGE,
+                   "%s: less than 2^23 rows and pieces of 512 tokens", who);
     return DNATOK_OK;
 }
 

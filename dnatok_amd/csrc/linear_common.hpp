@@ -40,6 +40,7 @@ struct WalkArgs {
     bool exact;                                    // whether states of 32 bits come of it
     float *slots;                                  // states at the cuts [cuts, heads, b.dim, c.dim], as `start` is laid out
     int64_t cut, cuts;                             // tokens from one to the next
+    int64_t first_item;                            // of the launch
 };
 
 constexpr int kOutside = 64;                       // workgroups that clear what is in no row

@@ -532,7 +532,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
     const int column = wave * 16, dc = w.c.dim;
     const int head = blockIdx.x % w.heads;
-    const int64_t item = blockIdx.x / w.heads;
+    const int64_t item = w.first_item + blockIdx.x / w.heads;
     if (item >= w.n_rows + w.cuts) {               // tokens in no row
         const int64_t front = row_at(w, 0), back = row_at(w, w.n_rows), waves = CD / 16, first = (item - w.n_rows - w.cuts) * waves + wave;
         const auto clear = [&](int64_t t) {
@@ -864,7 +864,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
     __shared__ PieceTiles<T, KD, CD> lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), column = wave * 16;
     const int head = blockIdx.x % w.heads;
-    const Piece p = piece_of(w, blockIdx.x / w.heads);
+    const Piece p = piece_of(w, w.first_item + blockIdx.x / w.heads);
     if (p.none || (w.reverse ? p.front : p.back)) return;
     const float ld = log_decay_of(w.log_decay, head);
     const int late = w.decayed ? 1 : 0;
@@ -937,17 +937,30 @@ template <typename T, typename Fn> void with_tiles(int32_t db, int32_t dc, Fn fn
     else if (db <= 96) deep(std::integral_constant<int, 96>{});
     else deep(std::integral_constant<int, 128>{});
 }
+// Launches of all items, a workgroup to an item and a head: as many to a launch as a grid takes, which has less than 2^32 threads.
+template <typename Fn> void in_launches(const WalkArgs &w, int64_t items, Fn fn)
+{
+    const int64_t most = (1 << 22) / w.heads;
+    for (int64_t first = 0; first < items; first += most) {
+        WalkArgs part = w;
+        part.first_item = first;
+        fn(part, (unsigned)((items - first < most ? items - first : most) * w.heads));
+    }
+}
 template <typename T> void launch_pieces(const WalkArgs &w, hipStream_t s)
 {
     with_tiles<T>(w.b.dim, w.c.dim, [&](auto kd, auto cd, auto tail) {
-        piece_kernel<T, kd(), cd(), tail()><<<(unsigned)((w.n_rows + w.cuts) * w.heads), threads_of(cd()), 0, s>>>(w);
+        in_launches(w, w.n_rows + w.cuts, [&](const WalkArgs &part, unsigned grid) {
+            piece_kernel<T, kd(), cd(), tail()><<<grid, threads_of(cd()), 0, s>>>(part);
+        });
     });
 }
 template <typename T> void launch_walk(const WalkArgs &w, hipStream_t s)
 {
-    const int64_t items = w.n_rows + w.cuts + (w.offsets ? kOutside : 0);
     with_tiles<T>(w.b.dim, w.c.dim, [&](auto kd, auto cd, auto tail) {
-        walk_kernel<T, kd(), cd(), tail()><<<(unsigned)(items * w.heads), threads_of(cd()), 0, s>>>(w);
+        in_launches(w, w.n_rows + w.cuts + (w.offsets ? kOutside : 0), [&](const WalkArgs &part, unsigned grid) {
+            walk_kernel<T, kd(), cd(), tail()><<<grid, threads_of(cd()), 0, s>>>(part);
+        });
     });
 }
 

@@ -338,7 +338,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     ``q`` [total, H, Dk], ``k`` [total, G, Dk] and ``v`` [total, G, Dv] are packed rows with ``offsets`` int64 [B + 1] as for
     :func:`gated_scan` (rows may be empty; tokens in no row give zeros, also as gradients), or dense rows [B, T, .., ..]
     without offsets (copied where they do not lie like packed ones); float32, bfloat16 or float16, the elements of a head
-    next to each other (parts of one projection's output will do).  H is a multiple of G: neighbouring heads share keys and
+    next to each other (parts of one projection's output will do), tokens less than 2^23 elements apart; less than 2^23 rows and
+    pieces of 512 tokens.  H is a multiple of G: neighbouring heads share keys and
     values.  Dk and Dv go up to 128.  ``log_decay`` float32 [H] is at most 0 (-inf: nothing is kept); ``scale`` is a number of
     2^-40 to 2^40 in size, Dk ** -0.5 if not given.  ``h0`` float32 [B, H, Dk, Dv] is the state in front of each row, zero if not given; ``reverse``
     runs rows from their last token to their first.  States and sums are held in 32 bits.  Infinities and NaN go on as the

@@ -497,7 +497,7 @@ int dnatok_logits_process(const void *logits, int64_t logits_stride, int32_t dty
  * one.  A row's y depends on no token behind it, also where that holds infinities or NaN, and those go on as the recurrence has them: an
 infinite T stays so as long as log_decay is above -1e30 (below it, and at -inf, nothing is left of any T).  states (NULL allowed) receives what the
  * backward pass needs, dnatok_linear_attention_states_bytes(); work is the call's own space,
- * dnatok_linear_attention_work_bytes(), 16-byte aligned. */
+ * dnatok_linear_attention_work_bytes(), 16-byte aligned.  Less than 2^23 rows and pieces of 512 tokens. */
 typedef struct dnatok_linear_shape {
     int32_t dtype, reverse;
     int64_t n_rows, total;

@@ -18,3 +18,10 @@ def test_the_stride_of_a_single_token_is_that_of_no_address(far):
     assert forward(q=None, **one) == INVALID and backward(dy=None, **one) == INVALID and step(**one) == INVALID
     assert forward(q=None, **{**one, "total": 2}) == TOO_LARGE and step(**{**one, "n_rows": 2}) == TOO_LARGE
     assert forward(**{**one, "q_token": -1}) == INVALID
+
+
+@pytest.mark.parametrize("heads,rows", [(16, 600000), (64, 2 ** 22), (65535, 1000)])
+def test_many_rows_of_many_heads(heads, rows):
+    many = dict(heads=heads, kv_heads=1, n_rows=rows, total=rows)
+    assert forward(q=None, **many) == INVALID and backward(dy=None, **many) == INVALID
+    assert forward(q=None, **{**many, "n_rows": 2 ** 23, "total": 2 ** 23}) == TOO_LARGE
