@@ -1,0 +1,32 @@
+"""Rows of linear attention that are really cut, against 64 bits: dense ones, and heads of 128 x 128 (tolerances: attention_reference)."""
+import pytest
+import torch
+
+from dnatok_amd import lm_ops
+from tests.test_gpu_linear_attention import DEV, TYPES, compare, inputs, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("rows,length,dims", [(1, 1100, (24, 40)), (2, 1500, (16, 16)), (3, 1025, (13, 7)), (2, 1200, (40, 72))])
+def test_dense_rows(rows, length, dims, reverse, dtype):
+    """Without offsets rows of one length are cut into equal pieces of 512 tokens and more: states, outputs and gradients."""
+    print(f"dense {rows} x {length} {dims} {dtype} reverse={reverse}", flush=True)
+    data = inputs([length] * rows, 4, 2, *dims, dtype, 31)
+    q, k, v, ld, off, h0, dy, dlast = data
+    leaves = [t.reshape(rows, length, *t.shape[1:]).detach().requires_grad_(True) for t in (q, k, v)] + [h0.detach().requires_grad_(True)]
+    y, last = lm_ops.linear_attention(*leaves[:3], ld, h0=leaves[3], reverse=reverse)
+    grads = torch.autograd.grad((y, last), leaves, (dy.view_as(y), dlast))
+    got = {"y": y.flatten(0, 1), "last": last, **{n: g.flatten(0, 1) for n, g in zip(("dq", "dk", "dv"), grads)}, "dh0": grads[3]}
+    compare(got, data, dtype, None, reverse, length)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dims", [(128, 128), (128, 64), (96, 128)])
+def test_wide_heads(dims, reverse, dtype):
+    print(f"cut rows, heads of {dims} {dtype} reverse={reverse}", flush=True)
+    data = inputs([1100, 3, 600], 2, 1, *dims, dtype, 32)
+    compare(run(*data, reverse=reverse), data, dtype, None, reverse, 1100)
