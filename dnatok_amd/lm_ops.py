@@ -293,7 +293,7 @@ class _LinearAttention(torch.autograd.Function):
         device, (total, heads, _), dim_v = q.device, q.shape, v.shape[2]
         if dy is None:
             dy = torch.zeros((1, 1, 1), dtype=q.dtype, device=device).expand(total, heads, dim_v)
-        if dim_v > 1 and dy.stride(2) != 1:
+        if (dim_v > 1 and dy.stride(2) != 1) or dy.stride(0) >= _FAR_TOKENS:     # (wherever autograd has put it)
             dy = dy.contiguous()
         if dlast is not None:
             dlast = dlast.contiguous()

@@ -30,3 +30,14 @@ def test_wide_heads(dims, reverse, dtype):
     print(f"cut rows, heads of {dims} {dtype} reverse={reverse}", flush=True)
     data = inputs([1100, 3, 600], 2, 1, *dims, dtype, 32)
     compare(run(*data, reverse=reverse), data, dtype, None, reverse, 1100)
+
+
+def test_a_gradient_at_any_place():
+    """What comes in for y lies where autograd has put it: tokens far apart, heads first, one number for all."""
+    data = inputs([2, 0, 1], 2, 1, 16, 24, torch.bfloat16, 33)
+    q, k, v, ld, off, h0, dy, dlast = data
+    far = torch.as_strided(torch.empty(2 * 2 ** 23 + 48, dtype=torch.bfloat16, device=DEV), (3, 2, 24), (2 ** 23, 24, 1)).copy_(dy)
+    want = run(*data)
+    for other in (far, dy.transpose(0, 1).contiguous().transpose(0, 1), dy.permute(2, 0, 1).contiguous().permute(1, 2, 0)):
+        got = run(q, k, v, ld, off, h0, other, dlast)
+        assert all(torch.equal(got[n], want[n]) for n in want)
