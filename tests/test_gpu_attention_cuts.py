@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from dnatok_amd import lm_ops
+from tests.support.attention_reference import U
 from tests.test_gpu_linear_attention import DEV, TYPES, compare, inputs, run
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,17 @@ def test_a_gradient_at_any_place():
     for other in (far, dy.transpose(0, 1).contiguous().transpose(0, 1), dy.permute(2, 0, 1).contiguous().permute(1, 2, 0)):
         got = run(q, k, v, ld, off, h0, other, dlast)
         assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+def test_a_state_that_lasts_is_rounded_twice_a_chunk():
+    """32 bits: what a chunk adds is summed by itself, so of 64 steps a state has two roundings, its decay's and the sum's.  With
+    log_decay = -2.5e-4 the chunks' weights, squared, add up to 31: 62 roundings of at most u of a cell, each to its own side, are some
+    sqrt(62) u = 7.9 u of the state's norm; one more for what each chunk's sum is off by."""
+    q, k, v, _, off, _, _, _ = inputs([20000], 2, 2, 16, 16, torch.float32, 34)
+    ld = torch.full((2,), -2.5e-4, device=DEV)
+    for reverse in (False, True):
+        _, last = lm_ops.linear_attention(q, k, v, ld, torch.tensor(off, device=DEV), reverse=reverse)
+        age = torch.arange(20000, device=DEV, dtype=torch.float64)
+        weight = torch.exp((age if reverse else age.flip(0)) * ld[0].double())
+        want = (k.double() * weight[:, None, None]).permute(1, 2, 0).contiguous() @ v.double().transpose(0, 1).contiguous()
+        assert (last[0].double() - want).norm() <= 9 * U * want.norm(), reverse
