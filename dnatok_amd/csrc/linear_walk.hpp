@@ -740,7 +740,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
             request(0);
             in_order();
             // whether any of the columns' cells is no finite number: 0 times it would reach the steps in front of it, so those are left
-            // out at first, and then added to the steps from theirs on
+            // out, and the steps from theirs on are left to by_steps
             uint32_t odd = 0;
 #pragma unroll
             for (int ts = 0; ts < TS; ++ts) odd |= not_finite<T>(c8[ts]);
@@ -750,7 +750,7 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
                 for (int ts = 0; ts < TS; ++ts)
 #pragma unroll
                     for (int e = 0; e < Frag<T>::kCount; ++e)
-                        if (!(__builtin_fabsf((float)c8[ts][e]) < INFINITY)) c8[ts][e] = (T)0.0f;
+                        if (!is_finite((float)c8[ts][e])) c8[ts][e] = (T)0.0f;
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -794,19 +794,16 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
                 for (int j = 0; j < 4; ++j) out[j] *= lds.up[j / 2][16 * j + l16];
             }
             if (__builtin_expect(any_odd, false)) {
+                int from[4] = {kChunk, kChunk, kChunk, kChunk};        // the first step of each column that is left out
+                for (int s = kChunk - 1; s >= 0; --s)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int last = 16 * j + l16;
-                    for (int s = 0; s <= last; ++s) {
-                        float score = 0.0f;
-                        for (int q = 0; q < SP; ++q) score += (float)lds.p[q].cell[last * Tile<T, kChunk>::kPitch + score_place<T>(s)];
-                        if constexpr (scaled) score *= lds.up[s / 32][last];
-                        for (int r = 0; r < 4; ++r) {
-                            const float v = (float)chunk.c.cell[s * Tile<T, CD>::kPitch + column + 4 * g + r];
-                            if (!(__builtin_fabsf(v) < INFINITY)) out[j][r] += score * v;
-                        }
-                    }
-                }
+                    for (int r = 0; r < 4; ++r)
+                        if (!is_finite((float)chunk.c.cell[s * Tile<T, CD>::kPitch + column + 4 * g + r])) from[r] = s;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * j + l16 >= from[r]) out[j][r] = NAN;
 #pragma unroll
                 for (int ts = 0; ts < TS; ++ts) c8[ts] = chunk.c.column(D * ts, column, lane);
             }
