@@ -106,10 +106,10 @@ __device__ __forceinline__ float nth_largest(const float *numbers, int count, in
 // A workgroup to a slice of a row, 32 tokens to a thread at most, held in registers.  The width-th largest of the waves' largest is a
 // bound that the slice's `width` largest are not below, and few others are above it: those are listed and ranked by counting who is in
 // front.  For more than eight, or where not every wave has tokens, it is that of eight lanes each; and where even those are
-// hardly more than `width`, that of the threads, found bit by bit.  (A step with 512 rows of 32,000 bfloat16, eight beams: 51.8 us,
-// bounds by eight lanes 61.4, by threads 58.2; 256 rows of floats, four beams: 30.8, 35.3 and 34.0.)  Where the
-// list does not hold them all (many equal ones), the largest is looked for again and again.  512 rows of 32,000 bfloat16: 18 us for
-// 33 MB, two workgroups to a CU: the chain from the reads to the rank, vector issue busy 0.31.
+// hardly more than `width`, that of the threads, found bit by bit.  (A step with 512 rows of 32,000 bfloat16, eight beams: 53.4 us,
+// bounds by eight lanes 61.9, by threads 59.7; 256 rows of floats, four beams: 33.5, 36.5 and 35.5.)  Where the
+// list does not hold them all (many equal ones), the largest is looked for again and again.  512 rows of 32,000 bfloat16: 19 us for
+// 33 MB, two workgroups to a CU: the chain from the reads to the rank, vector issue busy 0.32.
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void beam_rows_kernel(const T *logits, int64_t stride, int32_t vocab, int32_t slice,
                                                                 int32_t width, Candidate *found, Part *parts)
@@ -262,7 +262,7 @@ __device__ __forceinline__ double wave_max(double v)
 }
 
 // A wave to a group: the lists of its beams' slices, each in falling order, merged.  A lane has the best of what is left of its
-// lists (list l is lane l % 64's); lists are in the order of beams and tokens.  A chain of `width` steps: 8.5 us for eight of 8 beams, 5.5
+// lists (list l is lane l % 64's); lists are in the order of beams and tokens.  A chain of `width` steps: 8.7 us for eight of 8 beams, 5.7
 // for four of 4.
 constexpr int kMergeStaged = 4096;                 // candidates that are read into LDS at once
 template <bool STAGED>
@@ -378,7 +378,7 @@ struct Reorder {
     dnatok_rows t[kReorderTensors];
 };
 
-// Row r of a group's `width` is row parents[r] of its `beams`, 16, 4 or 1 bytes to a lane.  512 rows of 135 KB: 24 us, 5.7 TB/s.
+// Row r of a group's `width` is row parents[r] of its `beams`, 16, 4 or 1 bytes to a lane.  512 rows of 135 KB: 24.8 us, 5.6 TB/s.
 __global__ __launch_bounds__(256) void reorder_kernel(Reorder all, const int32_t *parents, int64_t rows, int32_t beams, int32_t width)
 {
     const dnatok_rows t = all.t[blockIdx.z];

@@ -65,7 +65,8 @@ static int narrow_shift(int64_t dim, int64_t size)
 constexpr int kEmbedAhead = 8;                     // rows that a wave has under way
 
 // A wave copies a run of tokens' rows, sixteen bytes to a lane, eight rows under way.  Bound by the writes: 524,288 rows of 512 bfloat16
-// (537 MB; the table stays in the caches) 113 us, 4.75 TB/s, as much as a copy; 1,000,003 rows of 203 floats 168 us, 4.8 TB/s.
+// (537 MB; the table stays in the caches) 113 us, 4.75 TB/s, as much as a copy; 1,000,003 rows of 203 floats 167 us, 4.9 TB/s (147 in a training
+// step, behind work that leaves fewer writes to finish).
 template <typename T, typename ID>
 __global__ __launch_bounds__(256) void embed_kernel(const ID *ids, int64_t n, int32_t run, const T *weight, int64_t w_stride,
                                                     int64_t vocab, int64_t dim, float scale, T *y)
@@ -128,8 +129,8 @@ __global__ __launch_bounds__(256) void embed_narrow_kernel(const ID *ids, int64_
 // Keys are ids, those outside the table the number behind its last row.  A pass sorts by up to eight of their bits: a workgroup
 // counts its tile's digits, a scan gives each tile its place for each digit, and a workgroup writes its tile there, the tokens of one
 // digit in their order.  So tokens of one id stay in their order, and a sum over them is the same in every call.  Tiles of 1,024 tokens:
-// a pass over 262,144 takes 5 + 3 + 7 us.  (Tiles of 8,192 leave CUs without work: 40,000 tokens and 32,000 ids 108 us for the whole
-// gradient instead of 46, 262,144 163 instead of 99, 8,000,000 no difference.)
+// a pass over 262,144 takes 5 + 3 + 7 us.  (Tiles of 8,192 leave CUs without work: 40,000 tokens and 32,000 ids 107 us for the whole
+// gradient instead of 46, 262,144 159 instead of 95, 8,000,000 450 instead of 433; the same dy each time, partly in the cache behind L2.)
 constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64, kDigits = 256;
 constexpr int kSortPerLane = 4, kSortTile = kSortThreads * kSortPerLane;
 constexpr int kSmallSort = 8192, kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
@@ -399,7 +400,8 @@ template <typename T> __device__ __forceinline__ void put_sum(const GradArgs &a,
 // A wave to a tile of the sorted tokens and 64 x 16 bytes of their rows: it adds up runs of one id.  A run inside the tile is a
 // row of the gradient; one that goes on in front of the tile or behind it leaves its sum in parts [tiles, 2, dim].  Further waves clear the
 // rows of ids that do not occur.  Eight rows of dy under way: 262,144 rows of 512 bfloat16 in the order of 32,000 ids 89 us (301 MB,
-// 3.4 TB/s), 1,000,003 rows of 203 floats and 12 ids 227 us (812 MB, 3.6 TB/s).  (Sixteen rows under way: 118 instead of 89.)
+// 3.4 TB/s), 1,000,003 rows of 203 floats and 12 ids 227 us (812 MB, 3.6 TB/s).  (Sixteen rows under way: the whole gradient of 262,144 rows
+// takes 134 us instead of 95.)
 template <typename T> __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, float *parts, T *grad)
 {
     typedef Words<T> W;
@@ -504,8 +506,8 @@ template <typename T> __global__ __launch_bounds__(256) void embed_grad_narrow_k
 }
 
 // Few tokens: a wave to a row of the gradient looks through all of their ids, and adds up what it finds.  One launch and no sort: 128
-// tokens take 4.3, 4.5 and 9.4 us with 12, 4,096 and 32,000 rows of 512 bfloat16 (sorted 13.9, 22.6 and 25.5), and where all are
-// one id, which one wave then adds up, 16.5, 16.8 and 21.9 (15.0, 24.8 and 27.6); 256 of one id take 31 (27).
+// tokens take 4.1, 4.1 and 9.8 us with 12, 4,096 and 32,000 rows of 512 bfloat16 (sorted 14.4, 22.4 and 25.4), and where all are
+// one id, which one wave then adds up, 16.4, 16.9 and 23.2 (15.2, 25.2 and 27.8); 256 of one id take 31 (17 with 12 rows, 27 with 4,096).
 constexpr int kFewTokens = 128;
 template <typename T, typename ID>
 __global__ __launch_bounds__(256) void embed_grad_few_kernel(const ID *ids, uint32_t n, const T *dy, int64_t dy_stride, int64_t vocab,
@@ -660,8 +662,8 @@ extern "C" int dnatok_embedding(const void *ids, int32_t id_bytes, int64_t n, co
         using T = decltype(t);
         with_ids(id_bytes, [&](auto i) {
             using ID = decltype(i);
-            // two rounds of rows to a wave, or one if that takes no more than 32,768 waves (524,288 rows of 512 bfloat16: 113.1 us with
-            // two, 114.5 with one, 115.9 with four; 1,000,003 of 203 floats: 168 with two, 178 with four, 183 with eight)
+            // two rounds of rows to a wave, or one if that takes no more than 32,768 waves (524,288 rows of 512 bfloat16: 112.9 us with
+            // two, 114.2 with one, 116.1 with four; 1,000,003 of 203 floats: 167 with two, 161 with one, 181 with four)
             const int shift = narrow_shift(dim, sizeof(T));
             if (shift >= 0) {
                 const int64_t once = kEmbedAhead * (64 >> shift);
@@ -698,8 +700,9 @@ static GradPlan plan_of(int64_t n, int64_t vocab, int64_t dim)
     p.bits = (bits + p.passes - 1) / p.passes;
     p.sort_tiles = (uint32_t)((n + kSortTile - 1) / kSortTile);
     // about 2,048 waves of wide rows, of 16-bit elements, or 1,024 with several narrow ones: shorter tiles write more parts of sums, longer
-    // ones leave CUs without work (the whole gradient, bfloat16: 262,144 x 512 95 us, with half or twice the waves 110 and 96; 1,000,003 x
-    // 203 149, 167 and 172; 1,000,000 x 64 86, 106 and 87; 8,000,000 x 32 433, with half 544)
+    // ones leave CUs without work (the whole gradient, bfloat16, ids of falling frequency, the same dy each time, partly in the cache behind
+    // L2: 262,144 x 512, 32,000 ids, 95 us, with half or twice the waves 111 and 97; 1,000,003 x 203, 12 ids, 149, 167 and 172;
+    // 1,000,000 x 64, 4,096 ids, 86, with half 106; 8,000,000 x 32, 32,000 ids, 433, 545 and 438)
     const int64_t narrow = (1 << 19) / (dim < 32 ? 32 : dim), wide = (1 << 20) / (dim < 128 ? 128 : dim);
     p.run = 16;
     while (p.run < (1 << 20) && n / p.run > (narrow > wide ? narrow : wide)) p.run *= 2;

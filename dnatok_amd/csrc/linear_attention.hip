@@ -66,8 +66,8 @@ __global__ __launch_bounds__(256) void shared_sum_kernel(const float *parts, T *
 }
 
 // One token of each row: a workgroup has a head's state, a thread every few rows of VEC of its columns.  The state is
-// read and written once; nothing else weighs anything.  250 rows, 8 heads of 128 x 128: 47.7 us for 262 MB, 5.5 TB/s; one row, 8 heads
-// of 64 x 64: 4.5 us, a call with its allocations 11.
+// read and written once; nothing else weighs anything.  250 rows, 8 heads of 128 x 128: 48 us for 262 MB, 5.5 TB/s; one row, 8 heads
+// of 64 x 64: 4.8 us, a call with its allocations 11.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void linear_step_kernel(Operand q, Operand k, Operand v, const float *log_decay, float scale,
                                                           const float *state, T *y, float *new_state)
@@ -177,9 +177,10 @@ static size_t slots_bytes(const dnatok_linear_shape *s, int64_t cuts) { return (
 // four waves on each of 256 CUs, or one of eight.  Rows (of all heads) that are fewer are cut into as many pieces as run at
 // once; more than that are cut where they are longer than about half of a CU's share, so that no long one is left running alone.  A
 // multiple or a whole part of the mean length, 512 tokens at least, so that rows of one length are cut into equal pieces or not at all.
-// (1 x 262,147 tokens, 4 heads of 128 x 128: 471 us, half as many pieces 767, twice as many 514; 64 x 8,192, 8 heads of 64 x 64: 543, 544
-// and 907.  Long reads, median 2,000 tokens: 1,500 rows, 2 heads of 64 x 64 1,542 us, cut at a quarter of the share 1,705, at the share
-// 1,830, uncut 2,204; 300 rows, 6 heads of 64 x 64 938, 1,040, 1,123 and 1,022, 4 heads of 128 x 128 1,830, 2,050, 2,019 and 1,667.)
+// (bfloat16, forward.  1 x 262,147 tokens, 4 heads of 128 x 128: 475 us, half as many pieces 784, twice as many 530; 64 x 8,192, 8 heads
+// of 64 x 64: 520, 518 and 835.  Long reads, median 2,000 tokens: 1,500 rows, 2 heads of 64 x 64 1,558 us, cut at a quarter of the
+// share 1,642, at the share 1,894, uncut 2,314; 300 rows, 6 heads of 64 x 64 934, 1,005, 1,141 and 1,053, 4 heads of 128 x 128 1,788,
+// 1,965, 2,043 and 1,695.)
 struct Cuts {
     int64_t cut, cuts;
 };
@@ -201,8 +202,8 @@ template <typename T> static void fill_slots(const WalkArgs &w, hipStream_t s)
 {
     if (!w.cuts) return;
     launch_pieces<T>(w, s);
-    // about 8,192 workgroups: most cuts begin no row's slots and leave at once, but one row's may be all that there is (255 cuts of 256
-    // rows, 4 heads of 128 x 128: 10 us, a workgroup to each part 29, 1,024 workgroups 5; 63 cuts of one row 35, 36 and 127)
+    // about 8,192 workgroups: most cuts begin no row's slots and leave at once, but one row's may be all that there is (the whole call, 4
+    // heads of 128 x 128: 256 rows of 1,024 tokens 368 us, a workgroup to each part 377, 1,024 workgroups 366; one row of 262,147 524, 528 and 602)
     const int64_t all = slot_parts(w) * w.heads, some = 8192 / w.cuts + 1;
     slots_kernel<<<dim3((unsigned)w.cuts, (unsigned)(all < some ? all : some)), kSlotThreads, 0, s>>>(w);
 }

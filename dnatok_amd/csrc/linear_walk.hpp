@@ -3,7 +3,9 @@
 // 16-bit operands: scores and T are fed to the products as two parts of T's type each (hi + lo, 2^-17 of themselves), what is added
 // to the state as three parts of a bfloat16 or two of a float16, so that results are as if computed in 32 bits and rounded once, and
 // the states are good to 32 bits.  (With one part, y would be off by 1.4 roundings of its type instead of one.)  float16 has no range for
-// scores and states: each row of scores, each column that is added and each wave's part of T is brought near 2^14 by a power of two.
+// scores and states: each row of scores, each column that is added and each wave's part of T is brought near 2^14 by a power of two, and what
+// is 2^39 below its largest is lost: next to its rounding a state is off by up to 2^-39 of a chunk's largest b and c.  (That is seen
+// only in cells whose last steps add exact zeros while the decay takes them there; y, of 11 bits, is not.)
 #pragma once
 
 #include "linear_common.hpp"
@@ -240,8 +242,8 @@ __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); 
 // ---- chunks in LDS -----------------------------------------------------------------------------------
 
 // Whether LDS holds two chunks of the operands, so that the next one is there when a chunk is done: where a workgroup has the CU to
-// itself.  (256 rows of 1,024 tokens and 4 heads of 128 x 128: 336 us, with one chunk 346; smaller heads have a second workgroup on
-// the CU, and want the room: 128 x 64 takes 209, with two 275; 64 rows of 8,192 and 8 heads of 64 x 64 506, with two 542.)
+// itself.  (256 rows of 1,024 tokens and 4 heads of 128 x 128: 335 us, with one chunk 347; smaller heads have a second workgroup on
+// the CU, and want the room: 128 x 64 takes 210, with two 278; 64 rows of 8,192 and 8 heads of 64 x 64 519, with two 550.)
 template <typename T, int KD, int CD> constexpr bool kTwoChunks = sizeof(T) == 2 && KD > 64 && CD > 64;
 
 template <typename T, int KD, int CD> struct alignas(16) Chunk {
@@ -516,11 +518,12 @@ __device__ __forceinline__ void by_steps(const WalkArgs &w, const Piece &p, int 
 //
 // 64 x 64 of bfloat16, 64 rows of 8,192 tokens, 8 heads: 500 us for 2.15 GB, 4.3 TB/s of the 4.75 that a copy reaches.  128 x 128, 256 rows
 // of 1,024 tokens, 4 heads: 340 us for 1.07 GB, bound by the length of a chunk's chain (scores, barrier, two products, state) with
-// two waves to a SIMD: matrix instructions busy 0.25, vector 0.38; without the loads it takes 12 % less, without the state's
+// two waves to a SIMD: matrix instructions busy 0.25, vector 0.40; without the loads it takes 12 % less, without the state's
 // products 18 %, with one part of scores and T instead of two 7 %.  (The columns of a head in two workgroups, which each compute all
 // scores, took 7 % more.  With 64 x 64, three workgroups to a CU spill registers: 888 us instead of 508.)
-// 48 x 40 in 32 bits, 876,000 tokens of long reads, 6 heads: 1,510 us, matrix instructions of 32 bits busy 0.39.  (As two float16
-// each, three products instead of one: a training step took 8,690 instead of 7,230, with registers spilled.)
+// 48 x 40 in 32 bits, 876,000 tokens of long reads, 6 heads: 1,520 us, matrix instructions of 32 bits busy 0.38: the wave with the last
+// sixteen steps has four tiles of scores where the first has one, and the fourth has no columns.  (As two float16 each, three products
+// instead of one: a training step took 20 % more, with registers spilled.)
 template <typename T, int KD, int CD, bool TAIL>
 __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 64 ? 1 : 2) void walk_kernel(WalkArgs w)
 {
@@ -919,7 +922,9 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
 
 // ---- launches -----------------------------------------------------------------------------------------
 
-// Calls fn with the tiles that hold db x dc, in steps of what a product takes, and whether rows end within 16 bytes.
+// Calls fn with the tiles that hold db x dc, and whether rows end within 16 bytes.  Heads of 32 bits are as deep as products take them in
+// steps of sixteen up to 64 (a training step on 300 long reads, 6 heads of 48 x 40: 7,290 us, with 64 for 48 8,345); of 65 to 80 and 97 to 112
+// they pay for 96 and 128, as 16-bit ones of 65 to 96 elements pay for a product's 32.
 template <typename T, typename Fn> void with_tiles(int32_t db, int32_t dc, Fn fn)
 {
     const auto deep = [&](auto kd) {

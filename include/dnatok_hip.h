@@ -516,7 +516,8 @@ int dnatok_linear_attention(const dnatok_linear_shape *shape_h, const void *q, c
 
 /* Gradients of the same call: dy [total, heads, dim_v] of `dtype` and dlast float[n_rows, heads, dim_k, dim_v] (NULL: zeros) are
  * those of y and last; dq, dk and dv, back to back in q's, k's and v's shapes, and dh0 (NULL allowed) are
- * written.  The decays have no gradient. */
+ * written.  The decays have no gradient.  dlast divided by the scale is held in 32 bits.  The work space for shared keys and values
+ * (heads above kv_heads) is a 32-bit part for each head, total * heads * (dim_k + dim_v) * 4 bytes, next to the states at cuts. */
 int dnatok_linear_attention_backward(const dnatok_linear_shape *shape_h, const void *q, const void *k, const void *v,
                                      const float *log_decay, const int64_t *offsets, const float *h0, const void *dy,
                                      const float *dlast, const float *states, void *dq, void *dk, void *dv, float *dh0, void *work,
