@@ -922,9 +922,9 @@ __global__ __launch_bounds__(threads_of(CD), sizeof(T) == 4 && KD > 64 && CD == 
 
 // ---- launches -----------------------------------------------------------------------------------------
 
-// Calls fn with the tiles that hold db x dc, and whether rows end within 16 bytes.  Heads of 32 bits are as deep as products take them in
-// steps of sixteen up to 64 (a training step on 300 long reads, 6 heads of 48 x 40: 7,290 us, with 64 for 48 8,345); of 65 to 80 and 97 to 112
-// they pay for 96 and 128, as 16-bit ones of 65 to 96 elements pay for a product's 32.
+// Calls fn with the tiles that hold db x dc, and whether rows end within 16 bytes.  Heads of 32 bits are 32, 48 or 64 deep up to 64 elements
+// (a training step on 300 long reads, 6 heads of 48 x 40: 7,290 us, with 64 for 48 8,345); of 65 to 80 and 97 to 112 they pay for
+// 96 and 128, as 16-bit ones of 65 to 80 elements pay for 96.
 template <typename T, typename Fn> void with_tiles(int32_t db, int32_t dc, Fn fn)
 {
     const auto deep = [&](auto kd) {
